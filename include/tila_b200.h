@@ -197,6 +197,75 @@ int tila_mg_gather(void *comm, const void *sendbuf, void *recvbuf, size_t bytes_
 
 int tila_mg_comm_destroy(void *comm);
 
+/* ---- operators of the decode path ---------------------------------------------
+ * Hand-written kernels beside the generated ones: rotary positions, norms of
+ * queries and keys fused with the rotation, the append to a paged key/value
+ * cache, and attention of a batch that shares a long prefix.  The reference has
+ * no counterpart.  Tensors are device addresses with strides in elements; the
+ * last dimension always has stride 1.  Every call is asynchronous on `stream`
+ * and runs on the current device; nothing is allocated and nothing is kept
+ * after the call.  `err` is the address of an error block
+ * (TILA_ERROR_BLOCK_BYTES, 0 = none) that takes device errors: an index outside
+ * its pool (the access is left out) or a wait that gave up. */
+
+/* Element types. */
+enum { TILA_F32 = 0, TILA_F16 = 1, TILA_BF16 = 2 };
+
+/* tila_op_rows.flags */
+#define TILA_ROWS_ROTATE 1u      /* the rows are rotated */
+#define TILA_ROWS_NORM 2u        /* divided by their root mean square, times weight */
+#define TILA_ROWS_PAGED 4u       /* dst is a paged pool, addressed through the slots */
+#define TILA_ROWS_WEIGHT_F32 8u  /* weight has 32-bit elements (else the rows' type) */
+
+/* One tensor of rows: batch x tokens x heads rows of `dim` elements. */
+typedef struct tila_op_rows {
+  uint64_t src, dst, weight, grad;  /* grad: the result's gradient (backward only) */
+  int64_t src_stride[3];            /* batch, token, head */
+  int64_t dst_stride[3];            /* the same; page, row, head with TILA_ROWS_PAGED */
+  int64_t grad_stride[3];
+  int32_t heads;
+  uint32_t flags;
+} tila_op_rows;
+
+typedef struct tila_rotary_args {
+  uint32_t size;          /* sizeof(tila_rotary_args) */
+  int32_t dtype;          /* of src, dst and grad */
+  int64_t batch, tokens;
+  int32_t dim;            /* 1 to 512 */
+  int32_t rotary;         /* leading elements that rotate: even, 0 to dim */
+  int32_t interleaved;    /* pairs (2i, 2i+1); else (i, i + rotary/2) */
+  int32_t inverse;        /* rotate back (the transpose) */
+  float amplitude;        /* factor of the rotated elements */
+  float eps;
+  uint64_t positions;     /* batch x tokens */
+  int64_t position_stride[2];
+  uint64_t inv_freq;      /* rotary/2 doubles: radians per position */
+  uint64_t slots;         /* one per token: page * page_size + row; negative = leave out */
+  int64_t slot_stride;
+  int64_t num_slots;
+  int32_t page_size;
+  int32_t index64;        /* bit 0: positions are 64-bit integers, bit 1: slots are */
+  int32_t num_rows;       /* tensors in rows[] */
+  int32_t reserved;       /* must be 0 */
+  uint64_t err, stream;
+  uint64_t workspace;     /* backward: tila_rotary_workspace() bytes */
+  uint64_t workspace_bytes;
+  uint64_t weight_grad[2];  /* backward: dim floats each */
+  tila_op_rows rows[3];
+} tila_rotary_args;
+
+/* dst = amplitude * R(position) * norm(src), for up to three tensors of the
+ * same tokens in one launch.  src and dst may be the same rows. */
+int tila_rotary_rows(const tila_rotary_args *args, char *log, size_t log_cap);
+
+/* Gradients of tila_rotary_rows with TILA_ROWS_NORM for up to two tensors: dst
+ * = the gradient of src, weight_grad[i] = that of rows[i].weight, in a fixed
+ * order of summation. */
+int tila_rotary_norm_backward(const tila_rotary_args *args, char *log, size_t log_cap);
+
+/* Bytes of workspace that tila_rotary_norm_backward needs (0 for a bad call). */
+uint64_t tila_rotary_workspace(const tila_rotary_args *args);
+
 #ifdef __cplusplus
 }
 #endif

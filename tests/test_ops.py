@@ -1,0 +1,194 @@
+"""The operators' host side on the CPU: frequencies, and the calls they refuse
+(nothing is launched: every refusal comes before that)."""
+
+import math
+
+import pytest
+import torch
+
+from tila_b200 import native, ops
+
+
+class OnDevice(torch.Tensor):
+    """A CPU tensor that says it is a CUDA tensor, so that the checks behind
+    that one can be reached without a GPU."""
+    is_cuda = property(lambda self: True)
+
+
+def dev(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype).as_subclass(OnDevice)
+
+
+def test_frequencies():
+    inv, amplitude = ops.rotary_frequencies(8, base=100.0, device="cpu")
+    assert inv.dtype is torch.float64 and amplitude == 1.0
+    assert inv.tolist() == [100.0 ** (-i / 4) for i in range(4)]
+    linear, _ = ops.rotary_frequencies(8, base=100.0, scaling="linear", factor=4.0, device="cpu")
+    assert torch.equal(linear, inv / 4)
+    ntk, _ = ops.rotary_frequencies(64, scaling="ntk", factor=8.0, device="cpu")
+    plain, _ = ops.rotary_frequencies(64, device="cpu")
+    assert ntk[0] == plain[0] and abs(ntk[-1].item() * 8 / plain[-1].item() - 1) < 1e-12
+    yarn, amplitude = ops.rotary_frequencies(64, scaling="yarn", factor=8.0, original_length=4096, device="cpu")
+    turns = plain * 4096 / (2 * math.pi)
+    assert torch.equal(yarn[turns > 40], plain[turns > 40])           # beyond the ramp's rounding outwards
+    assert torch.allclose(yarn[turns < 0.7], plain[turns < 0.7] / 8, rtol=1e-15)
+    assert bool((yarn <= plain).all()) and bool((yarn >= plain / 8 * (1 - 1e-15)).all())
+    assert amplitude == 0.1 * math.log(8.0) + 1.0
+    assert ops.rotary_frequencies(0, device="cpu")[0].numel() == 0
+    assert ops.rotary_frequencies(2, scaling="ntk", factor=2.0, device="cpu")[0].tolist() == [1.0]
+
+
+@pytest.mark.parametrize("kwargs", [dict(rotary=7), dict(rotary=-2), dict(rotary=8, base=0.0), dict(rotary=8, factor=0.5),
+                                    dict(rotary=8, scaling="other"), dict(rotary=8, scaling="yarn"),
+                                    dict(rotary=8, scaling="yarn", original_length=100, beta_fast=1.0, beta_slow=2.0)])
+def test_frequencies_refuse(kwargs):
+    with pytest.raises(ValueError):
+        ops.rotary_frequencies(device="cpu", **kwargs)
+
+
+INV = torch.ones(32, dtype=torch.float64).as_subclass(OnDevice)
+POS = torch.arange(6).as_subclass(OnDevice)
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(x=torch.zeros(6, 2, 64)), "CUDA"),
+    (dict(x=dev(6, 2, 64, dtype=torch.float64)), "float32"),
+    (dict(x=dev(6, 64)), "tokens, heads, dim"),
+    (dict(x=dev(6, 2, 513)), "512"),
+    (dict(x=dev(6, 2, 128)[..., ::2]), "contiguous"),
+    (dict(x=dev(6, 2, 62)), "rotates 64"),
+    (dict(positions=POS[:5]), "one position per token"),
+    (dict(positions=POS.float()), "int32 or int64"),
+    (dict(positions=torch.arange(6)), "CUDA"),
+    (dict(inv_freq=INV.float()), "float64"),
+    (dict(inv_freq=dev(64, dtype=torch.float64)[::2]), "contiguous"),
+    (dict(layout="other"), "layout"),
+    (dict(out=dev(6, 2, 32)), "shape"),
+    (dict(out=dev(6, 2, 64, dtype=torch.float16)), "float32"),
+    (dict(out=dev(6, 1, 64).expand(6, 2, 64)), "share memory"),
+    (dict(out=dev(6, 2, 128)[..., ::2]), "contiguous"),
+])
+def test_rotate_refuses(change, text):
+    args = dict(x=dev(6, 2, 64), positions=POS, inv_freq=INV) | change
+    x, positions, inv = args.pop("x"), args.pop("positions"), args.pop("inv_freq")
+    with pytest.raises(ValueError, match=text):
+        ops.rotate(x, positions, inv, **args)
+    with pytest.raises(ValueError, match=text):
+        ops.rotate_backward(x, positions, inv, **args)
+
+
+def test_not_a_tensor():
+    with pytest.raises(TypeError):
+        ops.rotate([1.0], POS, INV)
+
+
+def test_rotate_refuses_a_result_across_its_source():
+    flat = dev(6 * 2 * 64 + 64)
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.rotate(flat[:768].view(6, 2, 64), POS, INV, out=flat[64:].view(6, 2, 64))
+
+
+def test_overlap_rules():
+    """Parts of one tensor lie between each other's rows; anything else that
+    shares memory is refused."""
+    qkv = dev(6, 5, 64)
+    q, k = qkv[:, :3], qkv[:, 3:]
+    ops._apart("t", "a", q, "b", k)
+    ops._apart("t", "a", k, "b", q)
+    ops._apart("t", "a", q, "b", q, same=True)
+    both = dev(4, 2, 8, 3, 64)
+    ops._apart("t", "a", both[:, 0], "b", both[:, 1])
+    batch = dev(2, 6, 5, 64)
+    ops._apart("t", "a", batch[:, :, :3], "b", batch[:, :, 3:])
+    for a, b in ((q, q), (qkv[:, :3], qkv[:, 2:]), (q, qkv[:, :2]), (both[:, 0], both[:, 0]), (qkv, q)):
+        with pytest.raises(ValueError, match="overlaps"):
+            ops._apart("t", "a", a, "b", b)
+
+
+NORM = dict(q=dev(6, 4, 64), k=dev(6, 2, 64), q_weight=dev(64), k_weight=dev(64))
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(k=dev(5, 2, 64)), "same tokens"),
+    (dict(k=dev(6, 2, 32)), "same tokens"),
+    (dict(k=dev(6, 2, 64, dtype=torch.float16)), "one dtype"),
+    (dict(q_weight=dev(32)), "64 elements"),
+    (dict(k_weight=dev(64, dtype=torch.bfloat16)), "float32"),
+    (dict(q_weight=dev(128)[::2]), "contiguous"),
+    (dict(k=NORM["q"], k_out=NORM["q"]), "overlaps"),
+    (dict(q_out=dev(6, 4, 32)), "shape"),
+])
+def test_norm_rotate_refuses(change, text):
+    args = NORM | change
+    first = [args.pop(n) for n in ("q", "k", "q_weight", "k_weight")]
+    with pytest.raises(ValueError, match=text):
+        ops.norm_rotate(*first, POS, INV, **args)
+
+
+def test_norm_rotate_backward_refuses():
+    a = list(NORM.values())
+    for grads, kwargs, text in (((dev(6, 4, 32), dev(6, 2, 64)), {}, "shape"),
+                                ((dev(6, 4, 64), dev(6, 2, 64, dtype=torch.float16)), {}, "float32"),
+                                ((dev(6, 4, 64), dev(6, 2, 64)), dict(dk=NORM["q"][:, :2]), "overlaps")):
+        with pytest.raises(ValueError, match=text):
+            ops.norm_rotate_backward(*grads, *a, POS, INV, **kwargs)
+
+
+APPEND = dict(k=dev(6, 2, 64), v=dev(6, 2, 64), k_cache=dev(3, 4, 2, 64), v_cache=dev(3, 4, 2, 64),
+              slots=torch.arange(6).as_subclass(OnDevice))
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(k=dev(1, 6, 2, 64)), "tokens, kv_heads"),
+    (dict(v=dev(6, 2, 32)), "shape of k"),
+    (dict(v=dev(6, 2, 64, dtype=torch.float16)), "float32"),
+    (dict(k_cache=dev(3, 4, 1, 64)), "k_cache must be"),
+    (dict(v_cache=dev(3, 5, 2, 64)), "v_cache must be"),
+    (dict(v_cache=dev(12, 2, 64)), "4 dimensions"),
+    (dict(v_cache=APPEND["k_cache"]), "overlaps"),
+    (dict(k_cache=dev(1, 4, 2, 64).expand(3, 4, 2, 64)), "share memory"),
+    (dict(slots=POS[:4]), "one slot per token"),
+    (dict(slots=POS.float()), "int32 or int64"),
+    (dict(positions=POS), "go together"),
+    (dict(q_out=dev(6, 4, 64)), "need q"),
+    (dict(q=dev(5, 4, 64)), "q must be"),
+    (dict(q=dev(6, 4, 64), q_weight=dev(5)), "64 elements"),
+    (dict(k_weight=dev(64, dtype=torch.float16)), "float32"),
+    (dict(q=dev(6, 2, 64), q_out=APPEND["k"]), "overlaps"),
+])
+def test_append_refuses(change, text):
+    args = APPEND | change
+    first = [args.pop(n) for n in ("k", "v", "k_cache", "v_cache", "slots")]
+    with pytest.raises(ValueError, match=text):
+        ops.append_paged(*first, **args)
+
+
+def rotary_args(rows=1, flags=native.ROWS_ROTATE, **change):
+    """tila_rotary_args with addresses that nothing reads (the call is refused)."""
+    names = ("size", "dtype", "batch", "tokens", "dim", "rotary", "interleaved", "inverse", "amplitude", "eps",
+             "positions", "step_b", "step_t", "inv_freq", "slots", "slot_step", "num_slots", "page", "index64",
+             "num_rows", "reserved", "err", "stream", "workspace", "workspace_bytes", "dw0", "dw1")
+    head = dict(zip(names, (native.ROTARY_BYTES, 0, 1, 4, 64, 64, 0, 0, 1.0, 0.0, 4096, 0, 1, 4096, 0, 0, 0, 0, 1, rows, 0,
+                            0, 0, 0, 0, 0, 0))) | change
+    row = native.ROWS.pack(4096, 4096, 0, 0, 0, 128, 64, 0, 128, 64, 0, 0, 0, 2, flags)
+    return native.ROTARY_HEAD.pack(*(head[n] for n in names)) + row * rows + native.NO_ROWS * (3 - rows)
+
+
+@pytest.mark.parametrize("entry,args", [
+    ("tila_rotary_rows", rotary_args(size=8)),
+    ("tila_rotary_rows", rotary_args(reserved=1)),
+    ("tila_rotary_rows", rotary_args(dtype=3)),
+    ("tila_rotary_rows", rotary_args(dim=513)),
+    ("tila_rotary_rows", rotary_args(rotary=66)),
+    ("tila_rotary_rows", rotary_args(rotary=63)),
+    ("tila_rotary_rows", rotary_args(positions=0)),
+    ("tila_rotary_rows", rotary_args(num_rows=4)),
+    ("tila_rotary_rows", rotary_args(flags=native.ROWS_NORM)),
+    ("tila_rotary_rows", rotary_args(flags=native.ROWS_PAGED)),
+    ("tila_rotary_norm_backward", rotary_args()),
+])
+def test_c_entry_refuses(entry, args):
+    with pytest.raises(native.NativeError) as exc:
+        native.call_op(entry, args)
+    assert exc.value.status == native.TILA_ERR_ARGUMENT and exc.value.log
+    assert native.rotary_workspace(args) == 0

@@ -1,7 +1,8 @@
 """Builds the native part of the backend.
 
 * ``libtila_b200.so``: the C-ABI launcher (csrc/launcher.cpp), linked
-  against NVRTC; libcuda is opened at run time.
+  against NVRTC (libcuda is opened at run time), and the operators' kernels
+  (csrc/ops).
 * a compile check of the tile library for sm_100a with nvcc;
 * optionally, the cubins of the five benchmarked workloads (NVRTC works without
   a GPU), so that a fresh GPU machine does not spend its first launches
@@ -17,6 +18,7 @@ import shutil
 import subprocess
 import sys
 import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -25,18 +27,28 @@ CUDA = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
 
 
 def build_library(verbose=False) -> Path:
-    """nvcc build of the C-ABI library: the launcher (host C++) and the
-    no-allocation entry point (a .cu with a device array, sm_100a)."""
+    """nvcc build of the C-ABI library: the launcher (host C++), the
+    no-allocation entry point (a .cu with a device array, sm_100a) and the
+    hand-written operators (csrc/ops, sm_100a), each source compiled by a
+    process of its own."""
     out = PKG / "libtila_b200.so"
-    srcs = [PKG / "csrc" / "launcher.cpp", PKG / "csrc" / "noalloc.cu", PKG / "csrc" / "mg.cpp"]
-    hdr = ROOT / "include" / "tila_b200.h"
-    if out.exists() and out.stat().st_mtime > max([p.stat().st_mtime for p in srcs] + [hdr.stat().st_mtime]):
+    ops = PKG / "csrc" / "ops"
+    srcs = [PKG / "csrc" / "launcher.cpp", PKG / "csrc" / "noalloc.cu", PKG / "csrc" / "mg.cpp",
+            *sorted(ops.glob("*.cu"))]
+    hdrs = [ROOT / "include" / "tila_b200.h", PKG / "csrc" / "tile" / "tila_tile.cuh", *ops.glob("*.cuh")]
+    if out.exists() and out.stat().st_mtime > max(p.stat().st_mtime for p in srcs + hdrs):
         return out
-    cmd = [str(CUDA / "bin" / "nvcc"), "-std=c++17", "-O2", "-shared", "-Xcompiler", "-fPIC",
-           "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", f"-I{CUDA / 'include'}",
-           *[str(p) for p in srcs], f"-L{CUDA / 'lib64'}", "-lnvrtc", "-ldl",
-           "-Xlinker", f"-rpath,{CUDA / 'lib64'}", "-o", str(out) + ".tmp"]
-    subprocess.run(cmd, check=True, capture_output=not verbose)
+    nvcc = [str(CUDA / "bin" / "nvcc"), "-std=c++17", "-O2", "-Xcompiler", "-fPIC",
+            "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-diag-suppress", "550",
+            f"-I{CUDA / 'include'}"]
+    with tempfile.TemporaryDirectory() as d:
+        objs = [Path(d) / (p.name + ".o") for p in srcs]
+        with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+            list(pool.map(lambda so: subprocess.run([*nvcc, "-c", str(so[0]), "-o", str(so[1])], check=True,
+                                                    capture_output=not verbose), zip(srcs, objs)))
+        subprocess.run([*nvcc, "-shared", *[str(o) for o in objs], f"-L{CUDA / 'lib64'}", "-lnvrtc", "-ldl",
+                        "-Xlinker", f"-rpath,{CUDA / 'lib64'}", "-o", str(out) + ".tmp"],
+                       check=True, capture_output=not verbose)
     os.replace(str(out) + ".tmp", out)
     return out
 

@@ -1,0 +1,63 @@
+// Shared by the hand-written operators: element types, status reporting and
+// launch attributes.
+#pragma once
+
+#include "../../../include/tila_b200.h"
+#include "../tile/tila_tile.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdarg>
+#include <cstdio>
+
+namespace tila_ops {
+
+using tila::i32;
+using tila::i64;
+using tila::u32;
+using tila::u64;
+
+// Device error of the operators, beside tila::ErrorCode: an index read from
+// device memory (a slot, a page) points outside its pool.
+constexpr u32 kErrIndex = 5;
+
+constexpr int kSms = 148;
+
+inline int fail(int status, char *log, size_t cap, const char *fmt, ...) {
+  if (log != nullptr && cap != 0) {
+    va_list ap;
+    va_start(ap, fmt);
+    std::vsnprintf(log, cap, fmt, ap);
+    va_end(ap);
+  }
+  return status;
+}
+
+inline int launch_status(cudaError_t e, const char *what, char *log, size_t cap) {
+  if (e == cudaSuccess) return TILA_OK;
+  cudaGetLastError();  // the error is returned here, not left for the next call
+  int code = (e == cudaErrorInvalidValue || e == cudaErrorLaunchOutOfResources)
+                 ? TILA_ERR_RESOURCES : TILA_ERR_DRIVER;
+  return fail(code, log, cap, "%s: %s", what, cudaGetErrorString(e));
+}
+
+template <typename T> struct Elem;
+template <> struct Elem<float> {
+  static __device__ __forceinline__ float get(float v) { return v; }
+  static __device__ __forceinline__ float put(float v) { return v; }
+};
+template <> struct Elem<__half> {
+  static __device__ __forceinline__ float get(__half v) { return __half2float(v); }
+  static __device__ __forceinline__ __half put(float v) { return __float2half_rn(v); }
+};
+template <> struct Elem<__nv_bfloat16> {
+  static __device__ __forceinline__ float get(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static __device__ __forceinline__ __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
+};
+
+// V elements moved by one access.
+template <typename T, int V> struct __align__(sizeof(T) * V) Vec { T e[V]; };
+
+}  // namespace tila_ops

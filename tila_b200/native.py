@@ -14,6 +14,7 @@ from __future__ import annotations
 import ctypes
 import hashlib
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -39,6 +40,7 @@ EXPORTED_SYMBOLS = (
     "tila_device_info", "tila_status_string", "tila_launch_noalloc",
     "tila_mg_unique_id", "tila_mg_comm_init", "tila_mg_gather", "tila_mg_comm_destroy",
     "tila_host_word_alloc", "tila_host_word_free", "tila_noalloc_read_error",
+    "tila_rotary_rows", "tila_rotary_norm_backward", "tila_rotary_workspace",
 )
 
 #: Size of the error block every generated kernel takes (include/tila_b200.h).
@@ -138,6 +140,10 @@ def library() -> ctypes.CDLL:
         lib.tila_mg_gather.argtypes = [c_void_p, c_void_p, c_void_p, c_size_t, ctypes.c_uint64,
                                        c_char_p, c_size_t]
         lib.tila_mg_comm_destroy.argtypes = [c_void_p]
+        for name in ("tila_rotary_rows", "tila_rotary_norm_backward"):
+            getattr(lib, name).argtypes = [c_char_p, c_char_p, c_size_t]
+        lib.tila_rotary_workspace.argtypes = [c_char_p]
+        lib.tila_rotary_workspace.restype = ctypes.c_uint64
         _lib = lib
         return lib
 
@@ -398,3 +404,34 @@ def mg_gather(comm: int, send_ptr: int, recv_ptr: int, bytes_per_rank: int, stre
 
 def mg_comm_destroy(comm: int) -> None:
     _check(library().tila_mg_comm_destroy(ctypes.c_void_p(comm)), "communicator destroy")
+
+
+# -- operators (csrc/ops): argument structures packed as bytes ----------------
+
+TILA_DTYPE = {"float32": 0, "float16": 1, "bfloat16": 2}
+
+ROWS_ROTATE, ROWS_NORM, ROWS_PAGED, ROWS_WEIGHT_F32 = 1, 2, 4, 8
+
+#: tila_op_rows, and tila_rotary_args without its rows (include/tila_b200.h).
+ROWS = struct.Struct("=4Q9qiI")
+ROTARY_HEAD = struct.Struct("=Iiqq4iffQ2qQQqq4i6Q")
+ROTARY_ROWS = 3
+ROTARY_BYTES = ROTARY_HEAD.size + ROTARY_ROWS * ROWS.size
+NO_ROWS = bytes(ROWS.size)
+
+_op_log = threading.local()
+
+
+def call_op(name: str, args: bytes) -> None:
+    """Call the operator entry point ``name`` with its packed arguments."""
+    log = getattr(_op_log, "buffer", None)
+    if log is None:
+        log = _op_log.buffer = ctypes.create_string_buffer(1024)
+    status = getattr(library(), name)(args, log, 1024)
+    if status != TILA_OK:
+        _check(status, name, log)
+
+
+def rotary_workspace(args: bytes) -> int:
+    """Bytes of workspace that tila_rotary_norm_backward needs."""
+    return library().tila_rotary_workspace(args)
