@@ -266,6 +266,42 @@ int tila_rotary_norm_backward(const tila_rotary_args *args, char *log, size_t lo
 /* Bytes of workspace that tila_rotary_norm_backward needs (0 for a bad call). */
 uint64_t tila_rotary_workspace(const tila_rotary_args *args);
 
+/* Attention of a batch over a paged cache whose sequences share a prefix.
+ * Sequence b has lengths[b] tokens of its own in the cache, found through
+ * page_table[b], the last of which are its new tokens; they follow
+ * prefix_length tokens that all sequences share, found through prefix_pages.
+ * Its new tokens' queries are rows query_offsets[b] to query_offsets[b + 1] of
+ * q (query_offsets 0: row b alone).  Each attends to the whole prefix and to
+ * the sequence's own tokens up to itself; heads h of q share the key and value
+ * head h / (heads / kv_heads).  Pages, lengths and offsets are 32-bit integers.
+ * Rows of q behind the last sequence are neither read nor written; a row with
+ * nothing to attend to becomes 0, its lse -inf. */
+typedef struct tila_attend_args {
+  uint32_t size;            /* sizeof(tila_attend_args) */
+  int32_t dtype;            /* TILA_F16 or TILA_BF16: q, caches, out */
+  int64_t tokens;           /* rows of q */
+  int32_t batch, heads, kv_heads;
+  int32_t dim;              /* a multiple of 8 up to 256 */
+  int32_t page_size, table_width;  /* rows of a page; pages of a table row */
+  int32_t max_queries;      /* most new tokens of one sequence */
+  float scale;
+  int64_t num_pages, prefix_length;
+  uint64_t q, k_cache, v_cache, out;
+  uint64_t lse;             /* tokens x heads floats: log of the sum of exp (0 = not wanted) */
+  int64_t q_stride[2], out_stride[2];  /* token, head */
+  int64_t k_stride[3], v_stride[3];    /* page, row, head */
+  uint64_t page_table;
+  int64_t table_stride;
+  uint64_t lengths, query_offsets, prefix_pages;
+  uint64_t err, stream;
+  uint64_t workspace, workspace_bytes;  /* tila_attend_workspace() bytes, 16-byte aligned */
+} tila_attend_args;
+
+int tila_attend_shared_prefix(const tila_attend_args *args, char *log, size_t log_cap);
+
+/* Bytes of workspace of a call with these sizes (0 also for a bad call). */
+uint64_t tila_attend_workspace(const tila_attend_args *args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from tila_b200 import native, ops
-from ops_support import NORM_ERROR, TURN_ERROR, U, check_turn, half_step, norm, turn
+from ops_support import NORM_ERROR, TURN_ERROR, U, attend, check_turn, half_step, norm, turn
 
 pytestmark = pytest.mark.gpu
 
@@ -258,6 +258,226 @@ def test_append_reports_a_slot_outside_the_cache():
 
 
 # ---------------------------------------------------------------------------
+# attention over the paged cache
+# ---------------------------------------------------------------------------
+
+def paged(seed, counts, lengths, prefix, heads, kv, dim, page, dtype, heads_first=False, spare=0):
+    """Inputs of one call, every cache row that no sequence reaches NaN."""
+    g = gen(seed)
+    batch = len(counts)
+    width = max([1] + [-(-n // page) for n in lengths]) + spare
+    shared = -(-prefix // page)
+    pool = shared + sum(-(-n // page) for n in lengths) + 3
+    order = torch.randperm(pool, generator=g, device="cuda").to(torch.int32)
+    shape = (pool, kv, page, dim) if heads_first else (pool, page, kv, dim)
+    caches = [torch.full(shape, float("nan"), dtype=dtype, device="cuda") for _ in range(2)]
+    caches = [c.transpose(1, 2) if heads_first else c for c in caches]
+    table = torch.full((batch, width), -7, dtype=torch.int32, device="cuda")
+    at = shared
+    fill = [(order[:shared], prefix)]
+    for b, n in enumerate(lengths):
+        pages = order[at:at + -(-n // page)]
+        at += len(pages)
+        table[b, :len(pages)] = pages
+        fill.append((pages, n))
+    for pages, n in fill:
+        for i, x in enumerate(pages.tolist()):
+            rows = min(page, n - i * page)
+            for c in caches:
+                c[x, :rows] = normal(g, rows, kv, dim, dtype=dtype)
+    q = normal(g, sum(counts), heads, dim, dtype=dtype)
+    offsets = torch.tensor([0] + counts, dtype=torch.int32).cumsum(0).to(torch.int32).cuda()
+    return q, *caches, table, torch.tensor(lengths, dtype=torch.int32, device="cuda"), order[:shared].clone(), offsets
+
+
+def check_attend(case, counts, lengths, prefix, scale=None, single=False):
+    q, kc, vc, table, lens, pages, offsets = case
+    extra = {} if single else dict(query_offsets=offsets, max_queries=max(counts + [1]))
+    got, lse = ops.attend_shared_prefix(q, kc, vc, table, lens, prefix_pages=pages, prefix_length=prefix,
+                                        scale=scale, return_lse=True, **extra)
+    again = ops.attend_shared_prefix(q, kc, vc, table, lens, prefix_pages=pages, prefix_length=prefix, scale=scale,
+                                     **extra)
+    assert torch.equal(got, again)
+    want, wlse, tol, ltol = attend(q, kc, vc, table, lens, pages, prefix, counts,
+                                   q.shape[-1] ** -0.5 if scale is None else scale)
+    ops.check_errors()
+    off = (got.double() - want).abs() - tol
+    assert off.max().item() <= 0, f"{off.max().item():.3g} beyond the bound"      # NaN fails too
+    assert torch.equal(lse.isinf(), wlse.isinf())
+    assert ((lse.double() - wlse).abs() <= ltol)[~wlse.isinf()].all()
+    return got, lse
+
+
+SINGLE = [  # own lengths, prefix, heads, kv_heads, dim, page
+    ([1], 0, 1, 1, 64, 16), ([1, 0, 3], 0, 4, 2, 128, 16), ([0, 0], 5, 8, 8, 64, 8), ([17, 64, 1], 1, 8, 1, 128, 16),
+    ([100] * 5, 127, 6, 2, 128, 32), ([300, 5, 77, 129], 1000, 32, 8, 128, 64), ([513, 1], 64, 7, 1, 80, 16),
+    ([65, 200], 129, 5, 5, 96, 24), ([31, 1000], 333, 16, 4, 256, 128), ([9], 4097, 3, 3, 40, 1),
+    ([2000, 3, 1999], 0, 20, 4, 64, 256), ([40] * 40, 260, 16, 2, 64, 16), ([3] * 130, 700, 8, 8, 128, 64),
+    ([5, 600], 2000, 64, 1, 128, 128),
+]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("lengths,prefix,heads,kv,dim,page", SINGLE)
+def test_attend_single_tokens(dtype, lengths, prefix, heads, kv, dim, page):
+    counts = [1] * len(lengths)
+    case = paged(sum(lengths) + prefix, counts, lengths, prefix, heads, kv, dim, page, dtype)
+    got, lse = check_attend(case, counts, lengths, prefix, single=True)
+    if prefix == 0:
+        for b, n in enumerate(lengths):
+            if n == 0:
+                assert not got[b].any() and bool((lse[b] == -math.inf).all())
+
+
+RAGGED = [  # new tokens, own lengths, prefix, heads, kv_heads, dim, page
+    ([1, 2, 3], [1, 2, 3], 0, 4, 4, 64, 16), ([5, 0, 1, 17], [5, 9, 40, 17], 100, 8, 2, 128, 16),
+    ([130], [130], 0, 4, 1, 128, 64), ([64, 1, 33], [200, 70, 33], 300, 4, 4, 64, 32),
+    ([200, 3], [513, 3], 129, 6, 2, 96, 24), ([7] * 20, [7 + 9 * i for i in range(20)], 515, 10, 2, 128, 128),
+    ([1, 300], [1, 300], 64, 3, 1, 256, 16), ([40, 41], [1000, 41], 1111, 32, 8, 80, 8), ([0, 0], [4, 0], 10, 2, 1, 64, 16),
+]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("heads_first", [False, True])
+@pytest.mark.parametrize("counts,lengths,prefix,heads,kv,dim,page", RAGGED)
+def test_attend_several_tokens(dtype, heads_first, counts, lengths, prefix, heads, kv, dim, page):
+    if sum(counts) == 0:
+        case = paged(1, counts, lengths, prefix, heads, kv, dim, page, dtype, heads_first)
+        q, kc, vc, table, lens, pages, offsets = case
+        assert ops.attend_shared_prefix(q, kc, vc, table, lens, prefix_pages=pages, prefix_length=prefix,
+                                        query_offsets=offsets).shape == (0, heads, dim)
+        return
+    case = paged(sum(lengths), counts, lengths, prefix, heads, kv, dim, page, dtype, heads_first, spare=3)
+    check_attend(case, counts, lengths, prefix)
+
+
+@pytest.mark.parametrize("scale", [0.0, 30.0, -0.5])
+def test_attend_scales(scale):
+    """Equal weights, weights that all go to one key, and a negative scale."""
+    case = paged(4, [1, 1], [70, 300], 200, 4, 2, 64, 16, F16)
+    check_attend(case, [1, 1], [70, 300], 200, scale=scale, single=True)
+
+
+def test_attend_leaves_rows_behind_the_last_sequence():
+    counts, lengths = [3, 1], [20, 9]
+    q, kc, vc, table, lens, pages, offsets = paged(8, counts, lengths, 40, 8, 2, 128, 16, BF16)
+    padded = torch.cat([q, torch.full((5, 8, 128), float("nan"), dtype=BF16, device="cuda")])
+    out = torch.full((9, 8 * 2, 128), 7.0, dtype=BF16, device="cuda")[:, ::2]
+    got = ops.attend_shared_prefix(padded, kc, vc, table, lens, prefix_pages=pages, prefix_length=40,
+                                   query_offsets=offsets, max_queries=3, out=out)
+    want = ops.attend_shared_prefix(q, kc, vc, table, lens, prefix_pages=pages, prefix_length=40,
+                                    query_offsets=offsets, max_queries=3)
+    assert got is out and torch.equal(out[:4], want) and bool((out[4:] == 7).all())
+
+
+def test_attend_query_strides():
+    counts, lengths = [1, 1, 1], [20, 9, 33]
+    q, kc, vc, table, lens, pages, _ = paged(8, counts, lengths, 40, 6, 2, 64, 16, F16)
+    want = ops.attend_shared_prefix(q, kc, vc, table, lens, prefix_pages=pages, prefix_length=40)
+    odd = torch.zeros(3, 6, 65, dtype=F16, device="cuda")
+    odd[..., 1:] = q
+    heads_first = q.transpose(0, 1).contiguous().transpose(0, 1)
+    for x in (odd[..., 1:], heads_first, torch.cat([q, q, q], 1)[:, 6:12]):
+        assert torch.equal(ops.attend_shared_prefix(x, kc, vc, table, lens, prefix_pages=pages, prefix_length=40), want)
+
+
+@pytest.mark.parametrize("heads,kv", [(4, 2), (64, 2)])
+def test_attend_reports_bad_pages_lengths_and_offsets(heads, kv):
+    """The kernels check what only the device sees: a bad page reads as zeros,
+    a length beyond the table is cut to it, and the next call raises."""
+    counts, lengths = [1, 1], [40, 64]
+    case = paged(3, counts, lengths, 64, heads, kv, 64, 16, F16)
+    q, kc, vc, table, lens, pages, offsets = case
+    kc.nan_to_num_(0.0), vc.nan_to_num_(0.0)
+    good = ops.attend_shared_prefix(q, kc, vc, table, lens, prefix_pages=pages, prefix_length=64)
+    for bad in (kc.shape[0], -1, 1 << 30):
+        t, shared = table.clone(), pages.clone()
+        t[0, 1] = bad
+        shared[2] = bad
+        got = ops.attend_shared_prefix(q, kc, vc, t, lens, prefix_pages=pages, prefix_length=64)
+        torch.cuda.synchronize()
+        with pytest.raises(native.NativeError, match="outside its pool"):
+            ops.check_errors()
+        assert torch.equal(got[1], good[1]) and bool(got.isfinite().all())
+        ops.attend_shared_prefix(q, kc, vc, table, lens, prefix_pages=shared, prefix_length=64)
+        torch.cuda.synchronize()
+        with pytest.raises(native.NativeError, match="outside its pool"):
+            ops.check_errors()
+    for n in (-3, 1 << 20):
+        other = lens.clone()
+        other[0] = n
+        got = ops.attend_shared_prefix(q, kc, vc, table.clamp_min(0), other, prefix_pages=pages, prefix_length=64)
+        torch.cuda.synchronize()
+        with pytest.raises(native.NativeError, match="outside its pool"):
+            ops.check_errors()
+        assert torch.equal(got[1], good[1])
+    for o in ([0, 1, 99], [-4, 1, 2], [0, 2, 1], [0, 0, 2]):
+        ops.attend_shared_prefix(q, kc, vc, table, lens, prefix_pages=pages, prefix_length=64,
+                                 query_offsets=torch.tensor(o, dtype=torch.int32, device="cuda"), max_queries=1)
+        torch.cuda.synchronize()
+        with pytest.raises(native.NativeError, match="outside its pool"):
+            ops.check_errors()
+    assert torch.equal(ops.attend_shared_prefix(q, kc, vc, table, lens, prefix_pages=pages, prefix_length=64), good)
+
+
+def test_attend_far_into_a_large_cache():
+    """Pages whose rows lie beyond 2^32 bytes of the cache's start."""
+    pages, page, kv, dim = 40000, 64, 4, 256                         # 5.2 GB a cache
+    kc = torch.zeros(pages, page, kv, dim, dtype=F16, device="cuda")
+    vc = torch.zeros_like(kc)
+    g = gen(6)
+    table = torch.tensor([[39999, 3]], dtype=torch.int32, device="cuda")
+    k, v = normal(g, 100, kv, dim, dtype=F16), normal(g, 100, kv, dim, dtype=F16)
+    i = torch.arange(100, device="cuda")
+    ops.append_paged(k, v, kc, vc, table[0].long()[i // page] * page + i % page)
+    lens = torch.tensor([100], dtype=torch.int32, device="cuda")
+    q = normal(g, 1, 8, dim, dtype=F16)
+    shared = torch.tensor([39999, 39998], dtype=torch.int32, device="cuda")
+    check_attend((q, kc, vc, table, lens, shared, None), [1], [100], 70, single=True)
+    q = normal(g, 100, 8, dim, dtype=F16)
+    check_attend((q, kc, vc, table, lens, shared, torch.tensor([0, 100], dtype=torch.int32, device="cuda")), [100], [100], 70)
+
+
+def test_decode_step_through_all_operators():
+    """A prompt and three decode steps of one layer: normed and rotated queries
+    and keys into the cache, attention over prefix and own tokens; against dense
+    attention over everything, in 64 bits of the rows that the operators stored."""
+    g = gen(21)
+    heads, kv, dim, page, batch, prefix = 8, 2, 64, 16, 3, 50
+    inv = freqs(dim)
+    w = 1 + 0.2 * normal(g, dim)
+    kc = torch.full((40, page, kv, dim), float("nan"), dtype=BF16, device="cuda")
+    vc = kc.clone()
+    shared = torch.tensor([7, 2, 30, 11], dtype=torch.int32, device="cuda")
+    table = torch.arange(12, 12 + batch * 4, dtype=torch.int32, device="cuda").view(batch, 4)
+
+    def project(n):
+        x = normal(g, n, heads + 2 * kv, dim, dtype=BF16)
+        return x[:, :heads], x[:, heads:heads + kv], x[:, heads + kv:]
+
+    def slots(pages, first, n):
+        i = torch.arange(first, first + n, device="cuda")
+        return pages.long()[i // page] * page + i % page
+
+    q, k, v = project(prefix)
+    ops.append_paged(k, v, kc, vc, slots(shared, 0, prefix), positions=torch.arange(prefix, device="cuda"), inv_freq=inv,
+                     k_weight=w)
+    have = [0] * batch
+    for counts in ([9, 1, 5], [1, 1, 1], [1, 1, 1], [2, 1, 3]):
+        n = sum(counts)
+        q, k, v = project(n)
+        at = torch.cat([slots(table[b], have[b], c) for b, c in enumerate(counts)])
+        pos = torch.cat([torch.arange(prefix + have[b], prefix + have[b] + c, device="cuda") for b, c in enumerate(counts)])
+        qr, _ = ops.norm_rotate(q, k, w, w, pos, inv)
+        got = ops.append_paged(k, v, kc, vc, at, positions=pos, inv_freq=inv, k_weight=w, q=q, q_weight=w)
+        assert torch.equal(got, qr)
+        have = [h + c for h, c in zip(have, counts)]
+        lens = torch.tensor(have, dtype=torch.int32, device="cuda")
+        offsets = torch.tensor([0] + counts, device="cuda").cumsum(0).to(torch.int32)
+        check_attend((qr, kc, vc, table, lens, shared, offsets), counts, have, prefix)
+
+
+# ---------------------------------------------------------------------------
 # streams and graphs
 # ---------------------------------------------------------------------------
 
@@ -289,6 +509,40 @@ def test_other_stream_and_graph_replay():
     want = step()
     for graph in graphs:
         graph.replay()
+    torch.cuda.synchronize()
+    for got in outs:
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_attend_on_another_stream_and_in_two_graphs():
+    counts, lengths = [1] * 6, [100, 40, 260, 1, 77, 513]
+    q, kc, vc, table, lens, pages, _ = paged(3, counts, lengths, 600, 32, 8, 128, 16, BF16)
+
+    def step():
+        return ops.attend_shared_prefix(q, kc, vc, table, lens, prefix_pages=pages, prefix_length=600, return_lse=True)
+
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    here = step()                                                    # two calls at once
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, got, here))
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step())
+        graphs.append(graph)
+    q.copy_(normal(gen(77), *q.shape, dtype=BF16))
+    lens.sub_(1).clamp_min_(1)
+    want = step()
+    streams = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for graph, s in zip(graphs, streams):
+        with torch.cuda.stream(s):
+            graph.replay()
     torch.cuda.synchronize()
     for got in outs:
         assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -192,3 +192,80 @@ def test_c_entry_refuses(entry, args):
         native.call_op(entry, args)
     assert exc.value.status == native.TILA_ERR_ARGUMENT and exc.value.log
     assert native.rotary_workspace(args) == 0
+
+
+def ints(*shape):
+    return torch.zeros(*shape, dtype=torch.int32).as_subclass(OnDevice)
+
+
+H = torch.float16
+ATTEND = dict(q=dev(3, 4, 64, dtype=H), k_cache=dev(5, 8, 2, 64, dtype=H), v_cache=dev(5, 8, 2, 64, dtype=H),
+              page_table=ints(3, 2), lengths=ints(3))
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(q=torch.zeros(3, 4, 64)), "CUDA"),
+    (dict(q=dev(3, 4, 64)), "float16 or bfloat16"),
+    (dict(q=dev(3, 4, 60, dtype=H)), "multiple of 8"),
+    (dict(q=dev(3, 4, 264, dtype=H)), "up to 256"),
+    (dict(q=dev(3, 64, dtype=H)), "3 dimensions"),
+    (dict(q=dev(3, 5, 64, dtype=H)), "multiple of kv_heads"),
+    (dict(q=dev(4, 4, 64, dtype=H)), "one row per sequence"),
+    (dict(k_cache=dev(5, 8, 2, 32, dtype=H)), "both alike"),
+    (dict(v_cache=dev(5, 9, 2, 64, dtype=H)), "both alike"),
+    (dict(v_cache=dev(5, 8, 2, 64, dtype=torch.bfloat16)), "float16"),
+    (dict(k_cache=dev(5, 8, 2, 68, dtype=H)[..., 4:]), "16-byte"),
+    (dict(page_table=ints(3, 2).long()), "int32"),
+    (dict(page_table=ints(3)), "2 dimensions"),
+    (dict(page_table=ints(3, 4)[:, ::2]), "contiguous"),
+    (dict(lengths=ints(2)), "3 entries"),
+    (dict(lengths=ints(3, 1)), "1 dimensions"),
+    (dict(query_offsets=ints(3)), "4 entries"),
+    (dict(query_offsets=ints(4), max_queries=0), "at least 1"),
+    (dict(max_queries=2), "needs query_offsets"),
+    (dict(prefix_length=-1), "negative"),
+    (dict(prefix_length=5), "needs prefix_pages"),
+    (dict(prefix_length=17, prefix_pages=ints(2)), "fewer than 17"),
+    (dict(out=dev(3, 4, 32, dtype=H)), "shape"),
+    (dict(out=ATTEND["q"]), "overlaps"),
+    (dict(out=ATTEND["k_cache"].view(-1)[:768].view(3, 4, 64)), "overlaps"),
+])
+def test_attend_refuses(change, text):
+    args = ATTEND | change
+    first = [args.pop(n) for n in ("q", "k_cache", "v_cache", "page_table", "lengths")]
+    with pytest.raises(ValueError, match=text):
+        ops.attend_shared_prefix(*first, **args)
+
+
+def attend_args(**change):
+    """tila_attend_args with addresses that nothing reads (the call is refused)."""
+    names = ("size", "dtype", "tokens", "batch", "heads", "kv_heads", "dim", "page_size", "table_width", "max_queries",
+             "scale", "num_pages", "prefix_length", "q", "k_cache", "v_cache", "out", "lse", "qt", "qh", "ot", "oh",
+             "kp", "kr", "kh", "vp", "vr", "vh", "page_table", "table_stride", "lengths", "query_offsets",
+             "prefix_pages", "err", "stream", "workspace", "workspace_bytes")
+    v = dict(zip(names, (native.ATTEND.size, 1, 4, 4, 8, 2, 64, 16, 10, 1, 0.125, 100, 300, 4096, 4096, 4096, 4096, 0,
+                         512, 64, 512, 64, 2048, 128, 64, 2048, 128, 64, 4096, 10, 4096, 0, 4096, 0, 0, 0, 0))) | change
+    return native.ATTEND.pack(*(v[n] for n in names))
+
+
+@pytest.mark.parametrize("change", [
+    dict(size=8), dict(dtype=0), dict(dtype=3), dict(heads=3), dict(kv_heads=0), dict(dim=12), dict(dim=264), dict(page_size=0),
+    dict(max_queries=0), dict(tokens=3), dict(prefix_length=-1), dict(prefix_length=1 << 31), dict(q=0), dict(q=4097),
+    dict(k_cache=4104), dict(vr=4), dict(lengths=0), dict(page_table=0), dict(prefix_pages=0), dict(lse=2),
+    dict(workspace=4096, workspace_bytes=16), dict(workspace=4097, workspace_bytes=1 << 40),
+])
+def test_c_attend_refuses(change):
+    args = attend_args(**change)
+    with pytest.raises(native.NativeError) as exc:
+        native.call_op("tila_attend_shared_prefix", args)
+    assert exc.value.status == native.TILA_ERR_ARGUMENT and exc.value.log
+
+
+def test_c_attend_workspace():
+    """One partial result (dim + 1 floats) for every row and chunk; none where one
+    block does it all; none for a call of no rows."""
+    assert native.attend_workspace(attend_args()) % (4 * 8 * 65 * 4) == 0
+    assert native.attend_workspace(attend_args()) > 0
+    assert native.attend_workspace(attend_args(prefix_length=0, table_width=1)) == 0
+    assert native.attend_workspace(attend_args(tokens=0, batch=0)) == 0
+    native.call_op("tila_attend_shared_prefix", attend_args(tokens=0, batch=0))

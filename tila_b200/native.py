@@ -41,6 +41,7 @@ EXPORTED_SYMBOLS = (
     "tila_mg_unique_id", "tila_mg_comm_init", "tila_mg_gather", "tila_mg_comm_destroy",
     "tila_host_word_alloc", "tila_host_word_free", "tila_noalloc_read_error",
     "tila_rotary_rows", "tila_rotary_norm_backward", "tila_rotary_workspace",
+    "tila_attend_shared_prefix", "tila_attend_workspace",
 )
 
 #: Size of the error block every generated kernel takes (include/tila_b200.h).
@@ -140,10 +141,11 @@ def library() -> ctypes.CDLL:
         lib.tila_mg_gather.argtypes = [c_void_p, c_void_p, c_void_p, c_size_t, ctypes.c_uint64,
                                        c_char_p, c_size_t]
         lib.tila_mg_comm_destroy.argtypes = [c_void_p]
-        for name in ("tila_rotary_rows", "tila_rotary_norm_backward"):
+        for name in ("tila_rotary_rows", "tila_rotary_norm_backward", "tila_attend_shared_prefix"):
             getattr(lib, name).argtypes = [c_char_p, c_char_p, c_size_t]
-        lib.tila_rotary_workspace.argtypes = [c_char_p]
-        lib.tila_rotary_workspace.restype = ctypes.c_uint64
+        for name in ("tila_rotary_workspace", "tila_attend_workspace"):
+            getattr(lib, name).argtypes = [c_char_p]
+            getattr(lib, name).restype = ctypes.c_uint64
         _lib = lib
         return lib
 
@@ -418,6 +420,8 @@ ROTARY_HEAD = struct.Struct("=Iiqq4iffQ2qQQqq4i6Q")
 ROTARY_ROWS = 3
 ROTARY_BYTES = ROTARY_HEAD.size + ROTARY_ROWS * ROWS.size
 NO_ROWS = bytes(ROWS.size)
+#: tila_attend_args.
+ATTEND = struct.Struct("=Iiq7if2q5Q4q6qQq7Q")
 
 _op_log = threading.local()
 
@@ -435,3 +439,8 @@ def call_op(name: str, args: bytes) -> None:
 def rotary_workspace(args: bytes) -> int:
     """Bytes of workspace that tila_rotary_norm_backward needs."""
     return library().tila_rotary_workspace(args)
+
+
+def attend_workspace(args: bytes) -> int:
+    """Bytes of workspace that tila_attend_shared_prefix needs."""
+    return library().tila_attend_workspace(args)

@@ -6,6 +6,8 @@ kernels behind the C ABI (``include/tila_b200.h``, ``csrc/ops``).
   and key head with the rotation in the same pass, and its gradients;
 * :func:`append_paged` - keys and values into a paged cache, rotated (and
   normed) on the way, the queries in the same launch;
+* :func:`attend_shared_prefix` - attention over such a cache, of a batch whose
+  sequences share a prefix that is read once for all;
 * :func:`rotary_frequencies` - the frequencies that these take, scaled for
   long contexts.
 
@@ -487,3 +489,113 @@ def norm_rotate_backward(q_grad, k_grad, q, k, q_weight, k_weight, positions, in
                 turn, layout, amplitude, eps=eps, workspace=True,
                 weight_grad=(sums.data_ptr(), sums.data_ptr() + 4 * q.shape[-1]))
     return dq, dk, sums[0], sums[1]
+
+
+# ---------------------------------------------------------------------------
+# attention over the paged cache
+# ---------------------------------------------------------------------------
+
+def _indexes(name, what, t, device, rank, length=None):
+    _tensor(name, what, t, device, torch.int32, rank)
+    if t.numel() > 1 and t.stride(-1) != 1:
+        _fail(name, f"the last dimension of {what} must be contiguous")
+    if length is not None and t.shape[0] != length:
+        _fail(name, f"{what} must have {length} entries, not {t.shape[0]}")
+    return t.data_ptr()
+
+
+def attend_shared_prefix(q, k_cache, v_cache, page_table, lengths, *, prefix_pages=None, prefix_length=0,
+                         query_offsets=None, max_queries=None, scale=None, out=None, return_lse=False):
+    """Attention of new tokens over a paged cache: ``softmax(scale q K^T) V`` over
+    a prefix that all sequences share and each sequence's own tokens.
+
+    ``q``: (tokens, heads, dim), float16 or bfloat16, dim a multiple of 8 up to 256.
+    ``k_cache``, ``v_cache``: (pages, page_size, kv_heads, dim) in any strides whose rows
+    start on 16-byte boundaries; query heads share key heads in groups.
+    ``page_table`` (batch, width) and ``lengths`` (batch,), int32: the pages of each
+    sequence's own tokens and how many they are, the new ones included (append
+    them first).  ``prefix_pages`` (int32) holds the first ``prefix_length`` tokens of
+    every sequence; it is read once for the whole batch.
+
+    Without ``query_offsets`` row b of ``q`` is the one new token of sequence b.  With
+    it (int32, batch + 1 entries) rows ``query_offsets[b]`` to ``query_offsets[b + 1]`` are
+    its new tokens, at most ``max_queries`` of them; each sees the tokens up to
+    itself.  Rows of ``q`` behind the last sequence may be anything, and theirs of
+    ``out`` are left as they were.  A token that sees nothing gets zeros.
+
+    ``scale`` is 1/sqrt(dim) by default.  Returns ``out`` (q's dtype), and with
+    ``return_lse`` also the log of each row's sum of exponentials, float32 (tokens,
+    heads).  Scores, weights' sums and results are kept in 32 bits; the weights are
+    rounded to the values' type for their product.  The same call gives the same
+    bits.  Values that a new token may not see yet must still be finite, as a
+    weight of 0 is multiplied with them; what lies behind a sequence's length,
+    or in pages that it does not reach, may be anything.
+    """
+    name = "attend_shared_prefix"
+    _tensor(name, "q", q, None, None, 3)
+    if q.dtype is not torch.float16 and q.dtype is not torch.bfloat16:
+        _fail(name, f"q must be float16 or bfloat16, not {q.dtype}")
+    tokens, heads, dim = q.shape
+    if dim % 8 or not 8 <= dim <= 256:
+        _fail(name, f"dim must be a multiple of 8 up to 256, not {dim}")
+    q_stride = _unit_last(name, "q", q)
+    device = q.device
+    strides = []
+    for what, cache in (("k_cache", k_cache), ("v_cache", v_cache)):
+        _tensor(name, what, cache, device, q.dtype, 4)
+        if cache.shape != k_cache.shape or cache.shape[3] != dim or cache.shape[1] < 1:
+            _fail(name, f"{what} must be (pages, page_size, kv_heads, {dim}), both alike, not {tuple(cache.shape)}")
+        st = _unit_last(name, what, cache)
+        if cache.data_ptr() % 16 or st[0] % 8 or st[1] % 8 or st[2] % 8:
+            _fail(name, f"rows of {what} must start on 16-byte boundaries")
+        strides += st[:3]
+    pages, page_size, kv_heads, _ = k_cache.shape
+    if kv_heads < 1 or heads < 1 or heads % kv_heads:
+        _fail(name, f"heads ({heads}) must be a multiple of kv_heads ({kv_heads})")
+    table = _indexes(name, "page_table", page_table, device, 2)
+    batch, width = page_table.shape
+    lens = _indexes(name, "lengths", lengths, device, 1, batch)
+    if query_offsets is None:
+        if tokens != batch:
+            _fail(name, f"q must have one row per sequence, {batch}, not {tokens} (or query_offsets is needed)")
+        if max_queries not in (None, 1):
+            _fail(name, "max_queries needs query_offsets")
+        offsets, most = 0, 1
+    else:
+        offsets = _indexes(name, "query_offsets", query_offsets, device, 1, batch + 1)
+        most = max(1, tokens if max_queries is None else min(max_queries, tokens))
+        if max_queries is not None and max_queries < 1:
+            _fail(name, f"max_queries must be at least 1, not {max_queries}")
+    shared = 0
+    if prefix_length < 0:
+        _fail(name, f"prefix_length must not be negative, is {prefix_length}")
+    if prefix_length > 0:
+        if prefix_pages is None:
+            _fail(name, "prefix_length needs prefix_pages")
+        shared = _indexes(name, "prefix_pages", prefix_pages, device, 1)
+        if prefix_pages.shape[0] * page_size < prefix_length:
+            _fail(name, f"prefix_pages holds {prefix_pages.shape[0] * page_size} tokens, fewer than {prefix_length}")
+    out = _result(name, "out", out, q, (), (("q", q), ("k_cache", k_cache), ("v_cache", v_cache)))
+    lse = torch.empty(tokens, heads, dtype=torch.float32, device=device) if return_lse else None
+    o_stride = out.stride()
+    index = device.index
+
+    def go():
+        args = [native.ATTEND.size, _DTYPES[q.dtype], tokens, batch, heads, kv_heads, dim, page_size, width, most,
+                dim ** -0.5 if scale is None else float(scale), pages, prefix_length, q.data_ptr(),
+                k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+                q_stride[0], q_stride[1], o_stride[0], o_stride[1], *strides, table,
+                page_table.stride(0), lens, offsets, shared, _error_block(index),
+                torch.cuda.current_stream(index).cuda_stream, 0, 0]
+        need = native.attend_workspace(native.ATTEND.pack(*args))
+        if need:
+            space = torch.empty(need, dtype=torch.uint8, device=device)
+            args[-2], args[-1] = space.data_ptr(), need
+        native.call_op("tila_attend_shared_prefix", native.ATTEND.pack(*args))
+
+    if torch.cuda.current_device() == index:
+        go()
+    else:
+        with torch.cuda.device(index):
+            go()
+    return (out, lse) if return_lse else out
