@@ -1,5 +1,6 @@
 // Attention over a paged cache with a shared prefix: the narrow form for up to
-// 16 rows of queries a block, the join of partial results, and the host side.
+// 16 rows of queries a block, the join of partial results, and the host side
+// (the wide form, for more rows, is attend_wide.cu).
 //
 // Narrow form.  Few rows against many keys: bound by reading the keys and
 // values once.  A block of 4 warps takes 16 rows (a sequence's new tokens times
@@ -14,6 +15,7 @@
 // and a rounding of p moves it by 2^-9 of a weight.
 
 #include "attend.cuh"
+#include "attend_wide.cuh"
 
 #include <algorithm>
 
@@ -385,7 +387,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
   float sum = 0.f;
   float acc[8] = {};
   for (int s0 = 0; s0 < slots; s0 += 32) {
-    float w = s0 + lane < slots ? exp2f(p.partial_lse[(s0 + lane) * step + at] - base) : 0.f;
+    const float w = s0 + lane < slots ? exp2f(p.partial_lse[(s0 + lane) * step + at] - base) : 0.f;
     sum += w;
     const int n = min(32, slots - s0);
 #pragma unroll 4
@@ -458,8 +460,24 @@ int check(const tila_attend_args *a, char *log, size_t cap) {
 struct Plan {
   AttendParams p;
   int prefix_tiles, own_tiles;   // 16 rows each
+  bool prefix_wide, own_wide;
   i64 slots;
 };
+
+// Chunks of the wide form: one block a multiprocessor, so that the blocks of all
+// chunks fill whole waves; a block costs about 4 tiles of keys beside its own
+// (filling the ring, the results).
+int wide_chunk_of(i64 keys, i64 blocks, int &chunks) {
+  const i64 tiles = (keys + 127) / 128;
+  i64 best = 1, cost = 0;
+  for (i64 n = 1; n <= std::min<i64>(tiles, 64); ++n) {
+    const i64 c = ((blocks * n + kSms - 1) / kSms) * ((tiles + n - 1) / n + 4);
+    if (n == 1 || c < cost) best = n, cost = c;
+  }
+  const i64 each = (tiles + best - 1) / best;
+  chunks = static_cast<int>((tiles + each - 1) / each);
+  return static_cast<int>(each * 128);
+}
 
 // Chunks: enough blocks for two a multiprocessor and twice that many again, and
 // none longer than 512 keys beyond that, since sequences end at different
@@ -519,9 +537,18 @@ Plan plan(const tila_attend_args &a) {
   const i64 rows = (a.query_offsets == 0 ? a.batch : a.tokens) * p.group;
   r.prefix_tiles = static_cast<int>((rows + 15) / 16);
   r.own_tiles = (p.max_queries * p.group + 15) / 16;
-  p.prefix_chunk = chunk_of(p.prefix, static_cast<i64>(r.prefix_tiles) * p.kv_heads, p.prefix_chunks);
-  p.own_chunk = chunk_of(static_cast<i64>(a.table_width) * a.page_size,
-                         static_cast<i64>(r.own_tiles) * p.kv_heads * p.batch, p.own_chunks);
+  p.q_vectors = a.q % 16 == 0 && a.q_stride[0] % 8 == 0 && a.q_stride[1] % 8 == 0;
+  const i64 own_rows = static_cast<i64>(p.max_queries) * p.group;
+  const i64 own_keys = static_cast<i64>(a.table_width) * a.page_size;
+  const bool wide = wide_possible(a);
+  r.prefix_wide = wide && p.prefix > 0 && rows > 16;
+  r.own_wide = wide && own_keys > 0 && own_rows > 16;
+  p.prefix_chunk = r.prefix_wide
+                       ? wide_chunk_of(p.prefix, (rows + 255) / 256 * p.kv_heads, p.prefix_chunks)
+                       : chunk_of(p.prefix, static_cast<i64>(r.prefix_tiles) * p.kv_heads, p.prefix_chunks);
+  p.own_chunk = r.own_wide
+                    ? wide_chunk_of(own_keys, (own_rows + 255) / 256 * p.kv_heads * p.batch, p.own_chunks)
+                    : chunk_of(own_keys, static_cast<i64>(r.own_tiles) * p.kv_heads * p.batch, p.own_chunks);
   if (p.own_chunks == 0 && p.prefix_chunks == 0) p.own_chunks = 1;   // no keys at all: a block writes the zeros
   r.slots = p.prefix_chunks + p.own_chunks;
   p.direct = r.slots == 1 && p.prefix_chunks == 0;
@@ -534,8 +561,9 @@ u64 workspace_of(const Plan &r) {
 
 template <typename T, int DP>
 cudaError_t launch_narrow(const Plan &r, cudaStream_t stream) {
-  const i64 prefix_items = static_cast<i64>(r.prefix_tiles) * r.p.kv_heads * r.p.prefix_chunks;
-  const i64 own_items = static_cast<i64>(r.own_tiles) * r.p.kv_heads * r.p.own_chunks * r.p.batch;
+  const i64 prefix_items = r.prefix_wide ? 0 : static_cast<i64>(r.prefix_tiles) * r.p.kv_heads * r.p.prefix_chunks;
+  const i64 own_items = r.own_wide ? 0 : static_cast<i64>(r.own_tiles) * r.p.kv_heads * r.p.own_chunks * r.p.batch;
+  if (prefix_items + own_items == 0) return cudaSuccess;
   if (prefix_items + own_items > 0x7fffffff) return cudaErrorInvalidValue;
   cudaError_t e = cudaFuncSetAttribute(attend_narrow_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        Narrow<DP>::kBytes);
@@ -571,6 +599,9 @@ extern "C" int tila_attend_shared_prefix(const tila_attend_args *args, char *log
     r.p.partial_lse = r.p.partial + static_cast<u64>(r.slots) * r.p.tokens * r.p.heads * r.p.dim;
   }
   const cudaStream_t stream = reinterpret_cast<cudaStream_t>(args->stream);
+  if (r.prefix_wide) st = launch_wide(*args, r.p, true, stream, log, log_cap);
+  if (st == TILA_OK && r.own_wide) st = launch_wide(*args, r.p, false, stream, log, log_cap);
+  if (st != TILA_OK) return st;
   const cudaError_t e = args->dtype == TILA_F16 ? launch<__half>(r, stream) : launch<__nv_bfloat16>(r, stream);
   return launch_status(e, "tila_attend_shared_prefix", log, log_cap);
 }

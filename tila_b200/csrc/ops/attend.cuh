@@ -35,7 +35,7 @@ struct AttendParams {
   int prefix_chunk, prefix_chunks;  // chunks = slots 0 .. prefix_chunks - 1
   int own_chunk, own_chunks;        // slots prefix_chunks ..
   int direct;                       // one chunk in all: blocks write the result itself
-  int q_words;                      // q can be read in 32-bit words
+  int q_words, q_vectors;           // q can be read in 4-byte words, in 16-byte vectors
 };
 
 constexpr float kNegInf = -__builtin_huge_valf();

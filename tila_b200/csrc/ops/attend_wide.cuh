@@ -1,0 +1,28 @@
+// The wide form of the attention over a paged cache (attend_wide.cu).
+#pragma once
+
+#include "attend.cuh"
+
+namespace tila_ops {
+
+struct WideGrid {
+  int prefix;        // the shared prefix (rows of all sequences), else own tokens
+  int pairs;         // pairs of row tiles of 128
+};
+
+template <typename T> __device__ __forceinline__ u32 wide_pack(float lo, float hi);
+template <> __device__ __forceinline__ u32 wide_pack<__half>(float lo, float hi) { return tila::pack_f16x2(lo, hi); }
+template <> __device__ __forceinline__ u32 wide_pack<__nv_bfloat16>(float lo, float hi) {
+  u32 r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Whether pages, head size and strides allow TMA boxes of whole pages (or of 128
+// rows of one) in 128-byte swizzled tiles.
+bool wide_possible(const tila_attend_args &a);
+
+int launch_wide(const tila_attend_args &a, const AttendParams &p, bool prefix, cudaStream_t stream, char *log,
+                size_t cap);
+
+}  // namespace tila_ops
