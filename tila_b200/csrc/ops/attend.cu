@@ -3,11 +3,14 @@
 // (the wide form, for more rows, is attend_wide.cu).
 //
 // Narrow form.  Few rows against many keys: bound by reading the keys and
-// values once.  A block of 4 warps takes 16 rows (a sequence's new tokens times
-// the heads that share its key head) and one chunk of keys.  Each warp runs on
-// its own: it brings 16 keys and values at a time into its own ring of shared
-// memory with cp.async (pages may have any size: each lane looks up rows) and
-// needs no barrier with the others, so that loads never wait for arithmetic.
+// values once.  A block takes 16 rows (a sequence's new tokens times the heads that
+// share its key head) and one chunk of keys.  Each warp runs on its own: it brings
+// 16 keys and values at a time into its own ring of shared memory and needs no
+// barrier with the others, so that loads never wait for arithmetic.  Where pages
+// are multiples of 16 rows a step's keys lie in one page and one lane fetches them
+// with TMA (a box for 64 elements of 16 rows); for other pages each lane looks up
+// rows and copies 16-byte pieces with cp.async, whose 32 instructions a step cost a
+// warp 1500 of its 2500 cycles where TMA costs it about 100.
 // Scores and values go through m16n8k16 matrix instructions with 32-bit sums
 // (16 rows do not fill a tcgen05 tile; at these rows the instruction rate is not
 // what bounds).  Weights p are rounded to the values' type for the product with
@@ -26,7 +29,7 @@ using namespace tila_ops;
 constexpr int kWarps = 4;
 constexpr int kSlice = 16;                 // keys of one warp's step
 constexpr int kStep = kWarps * kSlice;     // keys of one block's step
-constexpr int kStages = 3;
+constexpr int kStages = 2;                 // 64 KB a block at 128 elements: three blocks a multiprocessor
 
 template <typename T> __device__ __forceinline__ u32 pack2(float lo, float hi);
 template <> __device__ __forceinline__ u32 pack2<__half>(float lo, float hi) {
@@ -81,19 +84,27 @@ struct Item {
 };
 
 template <int DP> struct Narrow {
-  static constexpr int kRow = DP * 2;                        // bytes of a row in shared memory
-  static constexpr int kStage = 2 * kSlice * kRow;           // keys and values of one step
+  static constexpr int kHalf = kSlice * 128;                 // 64 elements of 16 rows, swizzled
+  static constexpr int kValues = DP / 64 * kHalf;            // of a stage: keys, then values
+  static constexpr int kStage = 2 * kValues;
   static constexpr int kWarpBytes = kStages * kStage;
-  static constexpr int kBytes = kWarps * kWarpBytes;
-  static_assert(kBytes >= kWarps * 16 * DP * 4, "the join of the warps reuses the ring");
+  static constexpr int kBytes = kWarps * kWarpBytes + 1024;  // 1024: alignment of swizzled tiles
+  static_assert(kWarps * kWarpBytes >= kWarps * 16 * DP * 4, "the join of the warps reuses the ring");
 };
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kWarps * 32) attend_narrow_kernel(const __grid_constant__ AttendParams p,
-                                                                    int prefix_items, int prefix_tiles,
-                                                                    int own_tiles) {
+// Where 16 bytes (piece `ch` of row r) lie in a swizzled tile.
+__device__ __forceinline__ u32 piece(int r, int ch) {
+  return (ch >> 3) * (kSlice * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+}
+
+template <typename T, int DP, bool kTma>
+__device__ __forceinline__ void narrow_block(const AttendParams &p, const tila::TensorMap &kmap,
+                                             const tila::TensorMap &vmap, int prefix_items, int prefix_tiles,
+                                             int own_tiles) {
   using N = Narrow<DP>;
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char *smem = smem_raw + ((1024 - (tila::smem_u32(smem_raw) & 1023)) & 1023);
+  __shared__ __align__(8) u64 full[kWarps][kStages];
   __shared__ float row_max[kWarps][16], row_sum[kWarps][16];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 
@@ -140,6 +151,73 @@ __global__ void __launch_bounds__(kWarps * 32) attend_narrow_kernel(const __grid
   }
   const bool causal = it.slot >= p.prefix_chunks;
 
+  // the warp's ring of keys and values
+  unsigned char *ring = smem + warp * N::kWarpBytes;
+  const u32 ring_at = tila::smem_u32(ring);
+  const int begin = it.begin + warp * kSlice;
+  const int steps = it.end > begin ? (it.end - begin + kStep - 1) / kStep : 0;
+  if constexpr (kTma) {
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < kStages; ++i) tila::mbar_init(&full[warp][i], 1);
+      tila::mbar_fence_init();
+    }
+    __syncwarp();
+  }
+  // The page of a step's key is read one step ahead, and looked at when it is
+  // used: that of the step's first key, or each lane's of key lane & 15.
+  const int page_key = kTma ? 0 : lane & 15;
+  auto look_up = [&](int step) {
+    const int key = begin + step * kStep + page_key;
+    if (key >= it.end) return 0;
+    int page, row;
+    split_key(p, key, page, row);
+    return it.pages[page];
+  };
+  int page_ahead = kTma && lane != 0 ? 0 : look_up(0);
+  auto issue = [&](int step) {
+    if (step < steps && (!kTma || lane == 0)) {
+      const int key0 = begin + step * kStep;
+      int index, row;
+      split_key(p, key0 + page_key, index, row);
+      const int page = page_ahead;
+      page_ahead = look_up(step + 1);
+      bool ok = key0 + page_key < it.end;
+      if (ok && (page < 0 || page >= p.num_pages)) {
+        tila::report_error(p.err, kErrIndex, index);
+        ok = false;
+      }
+      if constexpr (kTma) {
+        u64 *bar = &full[warp][step % kStages];
+        unsigned char *stage = ring + (step % kStages) * N::kStage;
+        const int from = ok ? page : p.num_pages;            // outside the tensor: reads as zeros
+        tila::mbar_arrive_expect_tx(bar, N::kStage);
+#pragma unroll
+        for (int i = 0; i < DP / 64; ++i) {
+          tila::tma_load_4d(stage + i * N::kHalf, &kmap, bar, i * 64, row, it.head, from);
+          tila::tma_load_4d(stage + N::kValues + i * N::kHalf, &vmap, bar, i * 64, row, it.head, from);
+        }
+      } else {
+        constexpr int kChunks = DP / 8;                      // 16-byte pieces of a row
+        const i64 koff = ok ? page * p.k_stride[0] + row * p.k_stride[1] + it.head * p.k_stride[2] : -1;
+        const i64 voff = ok ? page * p.v_stride[0] + row * p.v_stride[1] + it.head * p.v_stride[2] : 0;
+        const u32 stage = ring_at + (step % kStages) * N::kStage;
+#pragma unroll
+        for (int i = 0; i < kSlice * kChunks / 32; ++i) {
+          const int r = (i * 32 + lane) / kChunks, ch = (i * 32 + lane) % kChunks;
+          const i64 ko = __shfl_sync(0xffffffffu, koff, r), vo = __shfl_sync(0xffffffffu, voff, r);
+          const bool in = ko >= 0 && ch * 8 < p.dim;
+          const T *k = static_cast<const T *>(p.k), *v = static_cast<const T *>(p.v);
+          copy16(stage + piece(r, ch), in ? k + ko + ch * 8 : k, in ? 16 : 0);
+          copy16(stage + N::kValues + piece(r, ch), in ? v + vo + ch * 8 : v, in ? 16 : 0);
+        }
+      }
+    }
+    if constexpr (!kTma) copy_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) issue(s);
+
   // queries: A fragments of 16 rows, rows g and g + 8 of each lane
   const int g = lane >> 2, c = lane & 3;
   u32 qf[DP / 16][4];
@@ -166,72 +244,43 @@ __global__ void __launch_bounds__(kWarps * 32) attend_narrow_kernel(const __grid
       }
   }
 
-  // the warp's ring of keys and values
-  const u32 ring = tila::smem_u32(smem) + warp * N::kWarpBytes;
-  constexpr int kChunks = DP / 8;                            // 16-byte pieces of a row
-  const int begin = it.begin + warp * kSlice;
-  const int steps = it.end > begin ? (it.end - begin + kStep - 1) / kStep : 0;
-  const T *kbase = static_cast<const T *>(p.k) + it.head * p.k_stride[2];
-  const T *vbase = static_cast<const T *>(p.v) + it.head * p.v_stride[2];
-  // the page of this lane's key (lane & 15) of a step, looked up one step ahead
-  auto look_up = [&](int step) {
-    const int key = begin + step * kStep + (lane & 15);
-    if (key >= it.end) return -1;
-    int page, row;
-    split_key(p, key, page, row);
-    return checked_page(p, it.pages, page);
-  };
-  int page_ahead = steps > 0 ? look_up(0) : -1;
-  auto issue = [&](int step) {
-    if (step < steps) {
-      const int key = begin + step * kStep + (lane & 15);
-      int unused, row;
-      split_key(p, key, unused, row);
-      const int page = page_ahead;
-      i64 koff = -1, voff = 0;
-      if (page >= 0) {
-        koff = page * p.k_stride[0] + row * p.k_stride[1];
-        voff = page * p.v_stride[0] + row * p.v_stride[1];
-      }
-      page_ahead = look_up(step + 1);
-      const u32 stage = ring + (step % kStages) * N::kStage;
-#pragma unroll
-      for (int i = 0; i < kSlice * kChunks / 32; ++i) {
-        const int r = (i * 32 + lane) / kChunks, ch = (i * 32 + lane) % kChunks;
-        const i64 ko = __shfl_sync(0xffffffffu, koff, r), vo = __shfl_sync(0xffffffffu, voff, r);
-        const int bytes = ko >= 0 && ch * 8 < p.dim ? 16 : 0;
-        const u32 at = stage + r * N::kRow + ((ch ^ (r & 7)) << 4);
-        copy16(at, bytes ? kbase + ko + ch * 8 : kbase, bytes);
-        copy16(at + kSlice * N::kRow, bytes ? vbase + vo + ch * 8 : vbase, bytes);
-      }
-    }
-    copy_commit();
-  };
-
   float o[DP / 8][4];
 #pragma unroll
   for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
   float m[2] = {kNegInf, kNegInf}, l[2] = {0.f, 0.f};
 
-#pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) issue(s);
   for (int step = 0; step < steps; ++step) {
-    copy_wait<kStages - 2>();
-    __syncwarp();
-    issue(step + kStages - 1);
-    const u32 stage = ring + (step % kStages) * N::kStage;
+    const u32 stage = ring_at + (step % kStages) * N::kStage;
+    const int key0 = begin + step * kStep;
+    if constexpr (kTma) {
+      // (the barrier across the warp also ends its reads of the stage that is filled next)
+      if (!__all_sync(0xffffffffu, tila::mbar_wait(&full[warp][step % kStages], (step / kStages) & 1, p.err, __LINE__,
+                                                   nullptr)))
+        break;
+      issue(step + kStages - 1);
+      if (key0 + kSlice > it.end) {
+        // values behind the end: whatever the page holds there, for a weight of 0
+        for (int i = lane; i < (key0 + kSlice - it.end) * (DP / 8); i += 32)
+          *reinterpret_cast<uint4 *>(ring + (step % kStages) * N::kStage + N::kValues +
+                                     piece(it.end - key0 + i / (DP / 8), i % (DP / 8))) = make_uint4(0, 0, 0, 0);
+        __syncwarp();
+      }
+    } else {
+      copy_wait<kStages - 2>();
+      __syncwarp();
+      issue(step + kStages - 1);
+    }
     float s[2][4] = {};
     {
       const int r = (lane & 7) + ((lane >> 4) << 3), ch = (lane >> 3) & 1;
 #pragma unroll
       for (int k = 0; k < DP / 16; ++k) {
         u32 b[4];
-        ldmatrix4(b, stage + r * N::kRow + (((k * 2 + ch) ^ (r & 7)) << 4));
+        ldmatrix4(b, stage + piece(r, k * 2 + ch));
         mma16816<T>(s[0], qf[k], b[0], b[1]);
         mma16816<T>(s[1], qf[k], b[2], b[3]);
       }
     }
-    const int key0 = begin + step * kStep;
     u32 pf[4];
     float scale[2];
 #pragma unroll
@@ -276,7 +325,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_narrow_kernel(const __grid
 #pragma unroll
       for (int n = 0; n < DP / 16; ++n) {
         u32 b[4];
-        ldmatrix4t(b, stage + kSlice * N::kRow + r * N::kRow + (((n * 2 + ch) ^ (r & 7)) << 4));
+        ldmatrix4t(b, stage + N::kValues + piece(r, n * 2 + ch));
         mma16816<T>(o[2 * n], pf, b[0], b[1]);
         mma16816<T>(o[2 * n + 1], pf, b[2], b[3]);
       }
@@ -284,7 +333,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_narrow_kernel(const __grid
   }
 
   // join the warps: maxima, sums, then the scaled results through shared memory
-  copy_wait<0>();
+  if constexpr (!kTma) copy_wait<0>();
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
@@ -350,13 +399,26 @@ __global__ void __launch_bounds__(kWarps * 32) attend_narrow_kernel(const __grid
   }
 }
 
+// Launched behind the wide form, whose results it does not read, it may run beside
+// it; the first block ends after it, so that what waits for this grid waits for
+// both.
+template <typename T, int DP, bool kTma>
+__global__ void __launch_bounds__(kWarps * 32)
+attend_narrow_kernel(const __grid_constant__ AttendParams p, const __grid_constant__ tila::TensorMap kmap,
+                     const __grid_constant__ tila::TensorMap vmap, int prefix_items, int prefix_tiles, int own_tiles) {
+  tila::grid_dep_release();
+  narrow_block<T, DP, kTma>(p, kmap, vmap, prefix_items, prefix_tiles, own_tiles);
+  if (blockIdx.x == 0 && threadIdx.x == 0) tila::grid_dep_wait();
+}
+
 // out = sum over slots of 2^(lse_s - lse) * partial_s, lse = log2 sum 2^lse_s: one
 // warp for each row of q and head.  Bound by reading the partial results, which
 // the blocks before left in L2.
-template <typename T>
+template <typename T, int I>
 __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant__ AttendParams p) {
   const int lane = threadIdx.x & 31;
   const i64 at = static_cast<i64>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  tila::grid_dep_wait();
   if (at >= p.tokens * p.heads) return;
   const i64 token = at / p.heads;
   const int head = static_cast<int>(at - token * p.heads);
@@ -379,46 +441,57 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
   const int own = limit <= 0 ? 0 : min((limit + p.own_chunk - 1) / p.own_chunk, p.own_chunks);
   const int slots = p.prefix_chunks + own;
   const i64 step = p.tokens * p.heads;
-  float top = kNegInf;
-  for (int s = lane; s < slots; s += 32) top = fmaxf(top, p.partial_lse[s * step + at]);
+  // the running maximum over slots keeps each slot's lse and row one load away: 8
+  // slots' rows are in flight at a time, and none waits for the weights
+  float top = kNegInf, sum = 0.f;
+  float acc[I * 4] = {};
+  for (int s0 = 0; s0 < slots; s0 += 8) {
+    float lse[8];
+    float4 row[8][I];
 #pragma unroll
-  for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-  const float base = top == kNegInf ? 0.f : top;
-  float sum = 0.f;
-  float acc[8] = {};
-  for (int s0 = 0; s0 < slots; s0 += 32) {
-    const float w = s0 + lane < slots ? exp2f(p.partial_lse[(s0 + lane) * step + at] - base) : 0.f;
-    sum += w;
-    const int n = min(32, slots - s0);
-#pragma unroll 4
-    for (int s = 0; s < n; ++s) {
-      const float ws = __shfl_sync(0xffffffffu, w, s);
-      const float *row = p.partial + ((s0 + s) * step + at) * p.dim;
+    for (int s = 0; s < 8; ++s) {
+      lse[s] = kNegInf;
+      if (s0 + s < slots) {
+        const i64 place = (s0 + s) * step + at;
+        lse[s] = p.partial_lse[place];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int d = lane * 4 + i * 128;
-        if (d < p.dim) {
-          const float4 x = *reinterpret_cast<const float4 *>(row + d);
-          acc[i * 4] = fmaf(ws, x.x, acc[i * 4]);
-          acc[i * 4 + 1] = fmaf(ws, x.y, acc[i * 4 + 1]);
-          acc[i * 4 + 2] = fmaf(ws, x.z, acc[i * 4 + 2]);
-          acc[i * 4 + 3] = fmaf(ws, x.w, acc[i * 4 + 3]);
-        }
+        for (int i = 0; i < I; ++i)
+          if (lane * 4 + i * 128 < p.dim) row[s][i] = *reinterpret_cast<const float4 *>(p.partial + place * p.dim + lane * 4 + i * 128);
       }
     }
-  }
+    float high = top;
 #pragma unroll
-  for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    for (int s = 0; s < 8; ++s) high = fmaxf(high, lse[s]);
+    const float base = high == kNegInf ? 0.f : high;
+    const float f = exp2f(top - base);
+    top = high;
+    sum *= f;
+#pragma unroll
+    for (int i = 0; i < I * 4; ++i) acc[i] *= f;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const float w = exp2f(lse[s] - base);
+      sum += w;
+      if (s0 + s < slots && w != 0.f)
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+          acc[i * 4] = fmaf(w, row[s][i].x, acc[i * 4]);
+          acc[i * 4 + 1] = fmaf(w, row[s][i].y, acc[i * 4 + 1]);
+          acc[i * 4 + 2] = fmaf(w, row[s][i].z, acc[i * 4 + 2]);
+          acc[i * 4 + 3] = fmaf(w, row[s][i].w, acc[i * 4 + 3]);
+        }
+    }
+  }
   const float inverse = sum == 0.f ? 0.f : 1.f / sum;
   T *out = static_cast<T *>(p.out) + token * p.out_stride[0] + head * p.out_stride[1];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < I; ++i) {
     const int d = lane * 4 + i * 128;
     if (d < p.dim)
 #pragma unroll
       for (int e = 0; e < 4; ++e) out[d + e] = Elem<T>::put(acc[i * 4 + e] * inverse);
   }
-  if (lane == 0 && p.lse != nullptr) p.lse[at] = sum == 0.f ? kNegInf : (base + log2f(sum)) * 0.6931471805599453f;
+  if (lane == 0 && p.lse != nullptr) p.lse[at] = sum == 0.f ? kNegInf : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
 // ---------------------------------------------------------------------------
@@ -460,7 +533,7 @@ int check(const tila_attend_args *a, char *log, size_t cap) {
 struct Plan {
   AttendParams p;
   int prefix_tiles, own_tiles;   // 16 rows each
-  bool prefix_wide, own_wide;
+  bool prefix_wide, own_wide, narrow_tma;
   i64 slots;
 };
 
@@ -541,6 +614,7 @@ Plan plan(const tila_attend_args &a) {
   const i64 own_rows = static_cast<i64>(p.max_queries) * p.group;
   const i64 own_keys = static_cast<i64>(a.table_width) * a.page_size;
   const bool wide = wide_possible(a);
+  r.narrow_tma = tma_possible(a) && a.page_size % kSlice == 0;
   r.prefix_wide = wide && p.prefix > 0 && rows > 16;
   r.own_wide = wide && own_keys > 0 && own_rows > 16;
   p.prefix_chunk = r.prefix_wide
@@ -559,28 +633,33 @@ u64 workspace_of(const Plan &r) {
   return r.p.direct ? 0 : static_cast<u64>(r.slots) * r.p.tokens * r.p.heads * (r.p.dim + 1) * sizeof(float);
 }
 
-template <typename T, int DP>
-cudaError_t launch_narrow(const Plan &r, cudaStream_t stream) {
+template <typename T, int DP, bool kTma>
+cudaError_t launch_narrow(const Plan &r, const tila::TensorMap &k, const tila::TensorMap &v, cudaStream_t stream) {
   const i64 prefix_items = r.prefix_wide ? 0 : static_cast<i64>(r.prefix_tiles) * r.p.kv_heads * r.p.prefix_chunks;
   const i64 own_items = r.own_wide ? 0 : static_cast<i64>(r.own_tiles) * r.p.kv_heads * r.p.own_chunks * r.p.batch;
   if (prefix_items + own_items == 0) return cudaSuccess;
   if (prefix_items + own_items > 0x7fffffff) return cudaErrorInvalidValue;
-  cudaError_t e = cudaFuncSetAttribute(attend_narrow_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       Narrow<DP>::kBytes);
+  const auto kernel = attend_narrow_kernel<T, DP, kTma>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Narrow<DP>::kBytes);
   if (e != cudaSuccess) return e;
-  attend_narrow_kernel<T, DP><<<static_cast<unsigned>(prefix_items + own_items), kWarps * 32, Narrow<DP>::kBytes,
-                                stream>>>(r.p, static_cast<int>(prefix_items), r.prefix_tiles, r.own_tiles);
-  return cudaGetLastError();
+  return launch_kernel(kernel, static_cast<unsigned>(prefix_items + own_items), kWarps * 32, Narrow<DP>::kBytes,
+                       stream, r.prefix_wide || r.own_wide, r.p, k, v, static_cast<int>(prefix_items), r.prefix_tiles, r.own_tiles);
+}
+
+template <typename T, int DP>
+cudaError_t launch_narrow(const Plan &r, const tila::TensorMap &k, const tila::TensorMap &v, cudaStream_t stream) {
+  return r.narrow_tma ? launch_narrow<T, DP, true>(r, k, v, stream) : launch_narrow<T, DP, false>(r, k, v, stream);
 }
 
 template <typename T>
-cudaError_t launch(const Plan &r, cudaStream_t stream) {
-  cudaError_t e = r.p.dim <= 64    ? launch_narrow<T, 64>(r, stream)
-                  : r.p.dim <= 128 ? launch_narrow<T, 128>(r, stream)
-                                   : launch_narrow<T, 256>(r, stream);
+cudaError_t launch(const Plan &r, const tila::TensorMap &k, const tila::TensorMap &v, cudaStream_t stream) {
+  cudaError_t e = r.p.dim <= 64    ? launch_narrow<T, 64>(r, k, v, stream)
+                  : r.p.dim <= 128 ? launch_narrow<T, 128>(r, k, v, stream)
+                                   : launch_narrow<T, 256>(r, k, v, stream);
   if (e != cudaSuccess || r.p.direct) return e;
-  attend_join_kernel<T><<<static_cast<unsigned>((r.p.tokens * r.p.heads + 7) / 8), 256, 0, stream>>>(r.p);
-  return cudaGetLastError();
+  const unsigned blocks = static_cast<unsigned>((r.p.tokens * r.p.heads + 7) / 8);
+  return launch_kernel(r.p.dim <= 128 ? attend_join_kernel<T, 1> : attend_join_kernel<T, 2>, blocks, 256, 0, stream,
+                       true, r.p);
 }
 
 }  // namespace
@@ -599,10 +678,14 @@ extern "C" int tila_attend_shared_prefix(const tila_attend_args *args, char *log
     r.p.partial_lse = r.p.partial + static_cast<u64>(r.slots) * r.p.tokens * r.p.heads * r.p.dim;
   }
   const cudaStream_t stream = reinterpret_cast<cudaStream_t>(args->stream);
-  if (r.prefix_wide) st = launch_wide(*args, r.p, true, stream, log, log_cap);
-  if (st == TILA_OK && r.own_wide) st = launch_wide(*args, r.p, false, stream, log, log_cap);
+  if (r.prefix_wide) st = launch_wide(*args, r.p, true, false, stream, log, log_cap);
+  if (st == TILA_OK && r.own_wide) st = launch_wide(*args, r.p, false, r.prefix_wide, stream, log, log_cap);
   if (st != TILA_OK) return st;
-  const cudaError_t e = args->dtype == TILA_F16 ? launch<__half>(r, stream) : launch<__nv_bfloat16>(r, stream);
+  tila::TensorMap k{}, v{};
+  if (r.narrow_tma) st = encode_caches(*args, kSlice, &k, &v, log, log_cap);
+  if (st != TILA_OK) return st;
+  const cudaError_t e =
+      args->dtype == TILA_F16 ? launch<__half>(r, k, v, stream) : launch<__nv_bfloat16>(r, k, v, stream);
   return launch_status(e, "tila_attend_shared_prefix", log, log_cap);
 }
 

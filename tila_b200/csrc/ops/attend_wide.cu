@@ -62,6 +62,29 @@ __device__ __forceinline__ bool warp_wait(u64 *bar, u32 parity, u32 *err, u32 wh
   return __all_sync(0xffffffffu, tila::mbar_wait(bar, parity, err, where, dead));
 }
 
+// A row of O from tensor memory (zeros where nothing was added to it) times `mine`,
+// plus `other` times the partner's row, to shared memory.
+template <int DP>
+__device__ __forceinline__ void write_row(u32 o_col, bool any, float mine, float other, const float *partner,
+                                          float *dst) {
+#pragma unroll 1
+  for (int c = 0; c < DP; c += 32) {
+    float o[32];
+    tila::tmem_ld32(o_col + c, o);
+    tila::tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (any) x = make_float4(o[i] * mine, o[i + 1] * mine, o[i + 2] * mine, o[i + 3] * mine);
+      if (partner != nullptr) {
+        const float4 y = *reinterpret_cast<const float4 *>(partner + c + i);
+        x = make_float4(x.x + other * y.x, x.y + other * y.y, x.z + other * y.z, x.w + other * y.w);
+      }
+      *reinterpret_cast<float4 *>(dst + c + i) = x;
+    }
+  }
+}
+
 struct Barriers {
   u64 full[9], empty[9];
   u64 scores[2];      // S of a warpgroup's tile is there (and P V of its tile before)
@@ -70,15 +93,13 @@ struct Barriers {
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads, 1)
-attend_wide_kernel(const __grid_constant__ AttendParams p, const __grid_constant__ TensorMap kmap,
-                   const __grid_constant__ TensorMap vmap, const __grid_constant__ WideGrid grid) {
+__device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMap &kmap, const TensorMap &vmap,
+                                           const WideGrid &grid) {
   using W = Wide<DP>;
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) Barriers bars;
   __shared__ u32 tmem_slot;
   __shared__ volatile int dead;
-  __shared__ float row_lse[2][kTile];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   unsigned char *smem = smem_raw + ((1024 - (tila::smem_u32(smem_raw) & 1023)) & 1023);
 
@@ -271,30 +292,36 @@ attend_wide_kernel(const __grid_constant__ AttendParams p, const __grid_constant
     const bool valid = row < rows;
     const int token = valid ? row / p.group : 0;
     const int limit = !valid ? 0 : causal ? limit0 + token : limit0;
+    const int out_head = head * p.group + (valid ? row - token * p.group : 0);
     if (!shared_rows || w == 0) {
-      // the row of queries, swizzled as TMA would leave it
-      unsigned char *dst = smem + w * W::kTileBytes + r * 128;
-      const T *q = static_cast<const T *>(p.q) + (token0 + token) * p.q_stride[0] +
-                   (head * p.group + row - token * p.group) * p.q_stride[1];
-#pragma unroll 4
-      for (int c = 0; c < DP / 8; ++c) {
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (valid && c * 8 < p.dim) {
+      // the warp's 32 rows of queries, whole rows at a time, swizzled as TMA would
+      // leave them
+      constexpr int kPieces = DP / 8, kRows = 32 / kPieces;  // 16-byte pieces of a row; rows of one access
+      const i64 from = valid ? (token0 + token) * p.q_stride[0] + out_head * p.q_stride[1] : -1;
+      const int c = lane % kPieces;
+      uint4 x[32 / kRows];
+#pragma unroll
+      for (int i = 0; i < 32 / kRows; ++i) {
+        const i64 at = __shfl_sync(0xffffffffu, from, i * kRows + lane / kPieces);
+        x[i] = make_uint4(0, 0, 0, 0);
+        if (at >= 0 && c * 8 < p.dim) {
+          const T *q = static_cast<const T *>(p.q) + at + c * 8;
           if (p.q_vectors) {
-            x = *reinterpret_cast<const uint4 *>(q + c * 8);
+            x[i] = *reinterpret_cast<const uint4 *>(q);
           } else {
-            const unsigned short *e = reinterpret_cast<const unsigned short *>(q) + c * 8;
-            x = make_uint4(e[0] | static_cast<u32>(e[1]) << 16, e[2] | static_cast<u32>(e[3]) << 16,
-                           e[4] | static_cast<u32>(e[5]) << 16, e[6] | static_cast<u32>(e[7]) << 16);
-          }
-          if (p.scale2 < 0.f) {                             // scores are scaled by |scale|
-            x.x ^= 0x80008000u;
-            x.y ^= 0x80008000u;
-            x.z ^= 0x80008000u;
-            x.w ^= 0x80008000u;
+            const unsigned short *e = reinterpret_cast<const unsigned short *>(q);
+            x[i] = make_uint4(e[0] | static_cast<u32>(e[1]) << 16, e[2] | static_cast<u32>(e[3]) << 16,
+                              e[4] | static_cast<u32>(e[5]) << 16, e[6] | static_cast<u32>(e[7]) << 16);
           }
         }
-        *reinterpret_cast<uint4 *>(dst + (c / 8) * (kTile * 128) + (((c % 8) ^ (r & 7)) << 4)) = x;
+      }
+      const u32 flip = p.scale2 < 0.f ? 0x80008000u : 0u;    // scores are scaled by |scale|
+#pragma unroll
+      for (int i = 0; i < 32 / kRows; ++i) {
+        const int q_row = (warp & 3) * 32 + i * kRows + lane / kPieces;
+        x[i].x ^= flip, x[i].y ^= flip, x[i].z ^= flip, x[i].w ^= flip;
+        *reinterpret_cast<uint4 *>(smem + w * W::kTileBytes + q_row * 128 + (c / 8) * (kTile * 128) +
+                                   (((c % 8) ^ (q_row & 7)) << 4)) = x[i];
       }
       tila::fence_proxy_async_smem();
     }
@@ -363,88 +390,80 @@ attend_wide_kernel(const __grid_constant__ AttendParams p, const __grid_constant
       tila::mbar_arrive(&bars.weights[w]);
     }
 
-    // ---- results: normalised, through the ring (free by now), a row a warp ----------
+    // ---- results: normalised, staged in the ring (free by now), a bulk copy a row -----
     if (tiles > 0) ok = warp_wait(&bars.done, 0, p.err, __LINE__, dead_ptr) && ok;
     tila::tc_fence_after();
-    float *staged = reinterpret_cast<float *>(smem + W::kRing);
-    {
-      const float inverse = sum == 0.f ? 0.f : 1.f / sum;
-      row_lse[w][r] = sum == 0.f ? kNegInf : top + log2f(sum);
-      float *dst = staged + (w * kTile + r) * W::kRowFloats;
-#pragma unroll
-      for (int c = 0; c < DP; c += 32) {
-        float o[32];
-        if (turn > 0) {
-          tila::tmem_ld32(o_col + c, o);
-          tila::tmem_wait_ld();
-        }
-#pragma unroll
-        for (int i = 0; i < 32; i += 4)
-          *reinterpret_cast<float4 *>(dst + c + i) =
-              turn > 0 ? make_float4(o[i] * inverse, o[i + 1] * inverse, o[i + 2] * inverse, o[i + 3] * inverse)
-                       : make_float4(0.f, 0.f, 0.f, 0.f);
+    float *staged = reinterpret_cast<float *>(smem + W::kRing) + (w * kTile + r) * W::kRowFloats;
+    float lse = sum == 0.f ? kNegInf : top + log2f(sum);
+    float mine = sum == 0.f ? 0.f : 1.f / sum, other = 0.f;   // factors of the two warpgroups' sums
+    const float *partner = staged + kTile * W::kRowFloats;
+    if (shared_rows) {
+      // both warpgroups saw a part of the keys: the second leaves its sums, the first joins
+      if (w == 1) {
+        write_row<DP>(o_col, turn > 0, mine, 0.f, nullptr, staged);
+        staged[DP] = lse;
       }
-      tila::tc_fence_before();
-    }
-    asm volatile("bar.sync 1, 256;" ::: "memory");
-    for (int i = warp; i < (shared_rows ? kTile : 2 * kTile); i += 8) {
-      const int out_row = row0 + i;
-      if (out_row >= rows || dead) continue;
-      const i64 out_token = token0 + out_row / p.group;
-      const int out_head = head * p.group + out_row % p.group;
-      const i64 at = out_token * p.heads + out_head;
-      float lse = row_lse[i / kTile][i % kTile], w0 = 1.f, w1 = 0.f;
-      if (shared_rows) {
-        // both warpgroups saw a part of the keys
-        const float other = row_lse[1][i];
-        const float high = fmaxf(lse, other);
-        const float b = high == kNegInf ? 0.f : high;
-        const float e0 = exp2f(lse - b), e1 = exp2f(other - b), all = e0 + e1;
-        const float inv = all == 0.f ? 0.f : 1.f / all;
-        w0 = e0 * inv;
-        w1 = e1 * inv;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (w == 0) {
+        const float second = partner[DP];
+        const float high = fmaxf(lse, second), b = high == kNegInf ? 0.f : high;
+        const float e0 = exp2f(lse - b), e1 = exp2f(second - b), all = e0 + e1;
+        const float inverse = all == 0.f ? 0.f : 1.f / all;
+        mine *= e0 * inverse;
+        other = e1 * inverse;
         lse = all == 0.f ? kNegInf : b + log2f(all);
       }
-      const int d = lane * 4;
-      if (d < p.dim) {
-        float4 x = *reinterpret_cast<const float4 *>(staged + i * W::kRowFloats + d);
-        if (shared_rows) {
-          const float4 y = *reinterpret_cast<const float4 *>(staged + (kTile + i) * W::kRowFloats + d);
-          x = make_float4(w0 * x.x + w1 * y.x, w0 * x.y + w1 * y.y, w0 * x.z + w1 * y.z, w0 * x.w + w1 * y.w);
-        }
+    }
+    if (!shared_rows || w == 0) {
+      write_row<DP>(o_col, turn > 0, mine, other, shared_rows ? partner : nullptr, staged);
+      if (valid && ok) {
+        const i64 at = (token0 + token) * p.heads + out_head;
+        const i64 place = slot * p.tokens * p.heads + at;
         if (p.direct) {
-          T *out = static_cast<T *>(p.out) + out_token * p.out_stride[0] + out_head * p.out_stride[1] + d;
-          out[0] = Elem<T>::put(x.x);
-          out[1] = Elem<T>::put(x.y);
-          out[2] = Elem<T>::put(x.z);
-          out[3] = Elem<T>::put(x.w);
+          T *out = static_cast<T *>(p.out) + (token0 + token) * p.out_stride[0] + out_head * p.out_stride[1];
+          for (int d = 0; d < p.dim; ++d) out[d] = Elem<T>::put(staged[d]);
+          if (p.lse != nullptr) p.lse[at] = lse * 0.6931471805599453f;
         } else {
-          *reinterpret_cast<float4 *>(p.partial + (slot * p.tokens * p.heads + at) * p.dim + d) = x;
+          p.partial_lse[place] = lse;
+          tila::fence_proxy_async_smem();
+          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(p.partial + place * p.dim),
+                       "r"(tila::smem_u32(staged)), "r"(p.dim * 4) : "memory");
+          tila::bulk_commit();
+          tila::bulk_wait_read();
         }
-      }
-      if (lane == 0) {
-        if (!p.direct) p.partial_lse[slot * p.tokens * p.heads + at] = lse;
-        else if (p.lse != nullptr) p.lse[at] = lse * 0.6931471805599453f;
       }
     }
+    tila::tc_fence_before();
   }
   __syncthreads();
   if (warp == 9) tila::tmem_dealloc(tmem, 512);
 }
 
-int encode(TensorMap *map, const tila_attend_args &a, u64 address, const int64_t *stride, char *log, size_t cap) {
+// The first block ends after the previous kernel, beside which this one may run, so
+// that what waits for this grid waits for both.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 1)
+attend_wide_kernel(const __grid_constant__ AttendParams p, const __grid_constant__ TensorMap kmap,
+                   const __grid_constant__ TensorMap vmap, const __grid_constant__ WideGrid grid) {
+  tila::grid_dep_release();
+  wide_block<T, DP>(p, kmap, vmap, grid);
+  if (blockIdx.x == 0 && threadIdx.x == 0) tila::grid_dep_wait();
+}
+
+int encode(TensorMap *map, const tila_attend_args &a, int rows, u64 address, const int64_t *stride, char *log,
+           size_t cap) {
   const uint64_t dims[4] = {static_cast<u64>(a.dim), static_cast<u64>(a.page_size), static_cast<u64>(a.kv_heads),
                             static_cast<u64>(a.num_pages)};
   const uint64_t strides[3] = {static_cast<u64>(stride[1]) * 2, static_cast<u64>(stride[2]) * 2,
                                static_cast<u64>(stride[0]) * 2};
-  const uint32_t box[4] = {64, static_cast<u32>(a.page_size < kTile ? a.page_size : kTile), 1, 1};
+  const uint32_t box[4] = {64, static_cast<u32>(rows), 1, 1};
   // CUtensorMapDataType: 6 = f16, 9 = bf16; swizzle 3 = 128 bytes
   return tila_encode_tensor_map(map, a.dtype == TILA_F16 ? 6 : 9, 4, address, dims, strides, box, 3, log, cap);
 }
 
 template <typename T, int DP>
 cudaError_t launch_form(const AttendParams &p, const TensorMap &k, const TensorMap &v, const WideGrid &grid,
-                        unsigned blocks, cudaStream_t stream) {
+                        unsigned blocks, bool after_previous, cudaStream_t stream) {
   static const cudaError_t registers = [] {
     cudaFuncAttributes attr;
     const cudaError_t e = cudaFuncGetAttributes(&attr, attend_wide_kernel<T, DP>);
@@ -454,16 +473,15 @@ cudaError_t launch_form(const AttendParams &p, const TensorMap &k, const TensorM
   cudaError_t e = cudaFuncSetAttribute(attend_wide_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        Wide<DP>::kBytes);
   if (e != cudaSuccess) return e;
-  attend_wide_kernel<T, DP><<<blocks, kThreads, Wide<DP>::kBytes, stream>>>(p, k, v, grid);
-  return cudaGetLastError();
+  return launch_kernel(attend_wide_kernel<T, DP>, blocks, kThreads, Wide<DP>::kBytes, stream, after_previous, p, k, v,
+                       grid);
 }
 
 }  // namespace
 
-bool wide_possible(const tila_attend_args &a) {
-  if (a.dim > 128 || a.num_pages < 1) return false;
-  if (a.page_size % 8 != 0 || (a.page_size < kTile ? kTile % a.page_size != 0 : a.page_size % kTile != 0)) return false;
-  // a dimension of one element may have any stride in torch; a tensor map's are positive and below 2^40
+bool tma_possible(const tila_attend_args &a) {
+  if (a.num_pages < 1) return false;
+  // a dimension of one element may have any stride in torch; a tensor map's are positive and below 2^40 bytes
   const int64_t *strides[2] = {a.k_stride, a.v_stride};
   for (const int64_t *s : strides)
     for (int i = 0; i < 3; ++i)
@@ -471,11 +489,20 @@ bool wide_possible(const tila_attend_args &a) {
   return true;
 }
 
-int launch_wide(const tila_attend_args &a, const AttendParams &p, bool prefix, cudaStream_t stream, char *log,
-                size_t cap) {
+bool wide_possible(const tila_attend_args &a) {
+  return tma_possible(a) && a.dim <= 128 && a.page_size % 8 == 0 &&
+         (a.page_size < kTile ? kTile % a.page_size == 0 : a.page_size % kTile == 0);
+}
+
+int encode_caches(const tila_attend_args &a, int rows, tila::TensorMap *k, tila::TensorMap *v, char *log, size_t cap) {
+  const int st = encode(k, a, rows, a.k_cache, a.k_stride, log, cap);
+  return st == TILA_OK ? encode(v, a, rows, a.v_cache, a.v_stride, log, cap) : st;
+}
+
+int launch_wide(const tila_attend_args &a, const AttendParams &p, bool prefix, bool after_previous, cudaStream_t stream,
+                char *log, size_t cap) {
   TensorMap k, v;
-  int st = encode(&k, a, a.k_cache, a.k_stride, log, cap);
-  if (st == TILA_OK) st = encode(&v, a, a.v_cache, a.v_stride, log, cap);
+  const int st = encode_caches(a, a.page_size < kTile ? a.page_size : kTile, &k, &v, log, cap);
   if (st != TILA_OK) return st;
   WideGrid grid{};
   const i64 rows = static_cast<i64>(prefix ? (a.query_offsets == 0 ? a.batch : a.tokens) : p.max_queries) * p.group;
@@ -484,13 +511,11 @@ int launch_wide(const tila_attend_args &a, const AttendParams &p, bool prefix, c
   const i64 blocks = static_cast<i64>(grid.pairs) * p.kv_heads *
                      (prefix ? p.prefix_chunks : static_cast<i64>(p.own_chunks) * p.batch);
   if (blocks > 0x7fffffff) return fail(TILA_ERR_ARGUMENT, log, cap, "tila_attend_shared_prefix: too many blocks");
-  cudaError_t e;
   const unsigned n = static_cast<unsigned>(blocks);
-  if (a.dtype == TILA_F16)
-    e = a.dim <= 64 ? launch_form<__half, 64>(p, k, v, grid, n, stream) : launch_form<__half, 128>(p, k, v, grid, n, stream);
-  else
-    e = a.dim <= 64 ? launch_form<__nv_bfloat16, 64>(p, k, v, grid, n, stream)
-                    : launch_form<__nv_bfloat16, 128>(p, k, v, grid, n, stream);
+  const auto launch = [&](auto form) { return form(p, k, v, grid, n, after_previous, stream); };
+  const cudaError_t e = a.dtype == TILA_F16
+                            ? (a.dim <= 64 ? launch(launch_form<__half, 64>) : launch(launch_form<__half, 128>))
+                            : (a.dim <= 64 ? launch(launch_form<__nv_bfloat16, 64>) : launch(launch_form<__nv_bfloat16, 128>));
   return launch_status(e, "tila_attend_shared_prefix", log, cap);
 }
 

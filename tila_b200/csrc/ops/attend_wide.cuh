@@ -18,11 +18,16 @@ template <> __device__ __forceinline__ u32 wide_pack<__nv_bfloat16>(float lo, fl
   return r;
 }
 
-// Whether pages, head size and strides allow TMA boxes of whole pages (or of 128
-// rows of one) in 128-byte swizzled tiles.
+// Whether the caches' strides allow tensor maps; and whether pages and head size
+// also fit the wide form: boxes of whole pages, or of 128 rows of one.
+bool tma_possible(const tila_attend_args &a);
 bool wide_possible(const tila_attend_args &a);
 
-int launch_wide(const tila_attend_args &a, const AttendParams &p, bool prefix, cudaStream_t stream, char *log,
-                size_t cap);
+// Tensor maps of both caches with boxes of 64 elements of `rows` rows, 128-byte
+// swizzled.
+int encode_caches(const tila_attend_args &a, int rows, tila::TensorMap *k, tila::TensorMap *v, char *log, size_t cap);
+
+int launch_wide(const tila_attend_args &a, const AttendParams &p, bool prefix, bool after_previous, cudaStream_t stream,
+                char *log, size_t cap);
 
 }  // namespace tila_ops

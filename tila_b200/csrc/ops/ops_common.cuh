@@ -43,6 +43,25 @@ inline int launch_status(cudaError_t e, const char *what, char *log, size_t cap)
   return fail(code, log, cap, "%s: %s", what, cudaGetErrorString(e));
 }
 
+// Launches `kernel`; `after_previous`: it may start while the previous kernel of
+// the stream still runs (programmatic dependent launch).  Kernels launched so end
+// or begin with tila::grid_dep_wait(), which returns when that kernel is done.
+template <typename... P, typename... A>
+cudaError_t launch_kernel(void (*kernel)(P...), unsigned blocks, unsigned threads, size_t smem, cudaStream_t stream,
+                          bool after_previous, const A &...args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = after_previous ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 template <typename T> struct Elem;
 template <> struct Elem<float> {
   static __device__ __forceinline__ float get(float v) { return v; }
