@@ -3,19 +3,22 @@
 // (the wide form, for more rows, is attend_wide.cu).
 //
 // Narrow form.  Few rows against many keys: bound by reading the keys and
-// values once.  A block takes 16 rows (a sequence's new tokens times the heads that
-// share its key head) and one chunk of keys.  Each warp runs on its own: it brings
-// 16 keys and values at a time into its own ring of shared memory and needs no
-// barrier with the others, so that loads never wait for arithmetic.  Where pages
+// values once.  A block takes 8 or 16 rows (a sequence's new tokens times the heads
+// that share its key head) and one chunk of keys.  Each warp runs on its own: it
+// brings 16 keys and values at a time into its own ring of shared memory and needs
+// no barrier with the others, so that loads never wait for arithmetic.  Where pages
 // are multiples of 16 rows a step's keys lie in one page and one lane fetches them
 // with TMA (a box for 64 elements of 16 rows); for other pages each lane looks up
 // rows and copies 16-byte pieces with cp.async, whose 32 instructions a step cost a
 // warp 1500 of its 2500 cycles where TMA costs it about 100.
-// Scores and values go through m16n8k16 matrix instructions with 32-bit sums
-// (16 rows do not fill a tcgen05 tile; at these rows the instruction rate is not
-// what bounds).  Weights p are rounded to the values' type for the product with
-// the values and summed as they are in 32 bits: the sum is also a result (lse),
-// and a rounding of p moves it by 2^-9 of a weight.
+//
+// Scores and sums go through m16n8k16 matrix instructions with 32-bit sums, keys
+// and values as the 16-row operand and the queries as the 8 columns: S^T = K Q^T and
+// O^T += V^T P^T.  Groups of up to 8 heads waste none of that, where 16 rows of queries
+// would take twice the instructions and registers (these rows do not fill a tcgen05
+// tile, and the instruction rate is not what bounds).  Weights p are rounded to the
+// values' type for the product with the values and summed as they are in 32 bits:
+// the sum is also a result (lse), and a rounding of p moves it by 2^-9 of a weight.
 
 #include "attend.cuh"
 #include "attend_wide.cuh"
@@ -57,6 +60,12 @@ __device__ __forceinline__ void ldmatrix4(u32 (&r)[4], u32 addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
+// The transpose of an 8x8 block of 16-bit elements across the warp.
+__device__ __forceinline__ u32 transposed(u32 x) {
+  u32 r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
 __device__ __forceinline__ void ldmatrix4t(u32 (&r)[4], u32 addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -89,7 +98,8 @@ template <int DP> struct Narrow {
   static constexpr int kStage = 2 * kValues;
   static constexpr int kWarpBytes = kStages * kStage;
   static constexpr int kBytes = kWarps * kWarpBytes + 1024;  // 1024: alignment of swizzled tiles
-  static_assert(kWarps * kWarpBytes >= kWarps * 16 * DP * 4, "the join of the warps reuses the ring");
+  static constexpr int kJoin = DP + 8;                        // floats of a row in the join of the warps
+  static_assert(kWarpBytes >= 16 * kJoin * 4, "the join of the warps reuses the ring");
 };
 
 // Where 16 bytes (piece `ch` of row r) lie in a swizzled tile.
@@ -97,15 +107,16 @@ __device__ __forceinline__ u32 piece(int r, int ch) {
   return (ch >> 3) * (kSlice * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
 }
 
-template <typename T, int DP, bool kTma>
+template <typename T, int DP, int NT, bool kTma>
 __device__ __forceinline__ void narrow_block(const AttendParams &p, const tila::TensorMap &kmap,
                                              const tila::TensorMap &vmap, int prefix_items, int prefix_tiles,
                                              int own_tiles) {
   using N = Narrow<DP>;
+  constexpr int kRows = 8 * NT;                              // of queries
   extern __shared__ unsigned char smem_raw[];
   unsigned char *smem = smem_raw + ((1024 - (tila::smem_u32(smem_raw) & 1023)) & 1023);
   __shared__ __align__(8) u64 full[kWarps][kStages];
-  __shared__ float row_max[kWarps][16], row_sum[kWarps][16];
+  __shared__ float row_max[kWarps][kRows], row_sum[kWarps][kRows];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 
   // which rows and keys: neighbouring blocks take the heads of the same pages
@@ -120,7 +131,7 @@ __device__ __forceinline__ void narrow_block(const AttendParams &p, const tila::
       it.token0 = 0;
       const i64 all = p.offsets == nullptr ? p.batch : min(max(static_cast<i64>(p.offsets[p.batch]), static_cast<i64>(0)), p.tokens);
       it.rows = static_cast<int>(all * p.group);
-      it.row0 = tile * 16;
+      it.row0 = tile * kRows;
       it.begin = it.slot * p.prefix_chunk;
       it.end = min(it.begin + p.prefix_chunk, p.prefix);
       it.limit0 = p.prefix;
@@ -138,10 +149,10 @@ __device__ __forceinline__ void narrow_block(const AttendParams &p, const tila::
       sequence_rows(p, b, it.token0, count);
       const int length = own_length(p, b);
       it.rows = count * p.group;
-      it.row0 = tile * 16;
+      it.row0 = tile * kRows;
       if (it.row0 >= it.rows) return;
       it.limit0 = length - count + 1;
-      const int last = min(it.row0 + 15, it.rows - 1) / p.group;
+      const int last = (min(it.row0 + kRows, it.rows) - 1) / p.group;
       it.begin = chunk * p.own_chunk;
       it.end = min(it.begin + p.own_chunk, it.limit0 + last);
       it.pages = p.table + b * p.table_stride;
@@ -218,15 +229,13 @@ __device__ __forceinline__ void narrow_block(const AttendParams &p, const tila::
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) issue(s);
 
-  // queries: A fragments of 16 rows, rows g and g + 8 of each lane
+  // queries: columns g of 8, as B fragments
   const int g = lane >> 2, c = lane & 3;
-  u32 qf[DP / 16][4];
-  int limit[2];
+  u32 qf[NT][DP / 16][2];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int row = it.row0 + g + 8 * h;
+  for (int t = 0; t < NT; ++t) {
+    const int row = it.row0 + t * 8 + g;
     const int token = row / p.group;
-    limit[h] = row < it.rows ? (causal ? it.limit0 + token : it.limit0) : 0;
     const T *q = static_cast<const T *>(p.q) + (it.token0 + token) * p.q_stride[0] +
                  (it.head * p.group + row - token * p.group) * p.q_stride[1];
 #pragma unroll
@@ -240,14 +249,27 @@ __device__ __forceinline__ void narrow_block(const AttendParams &p, const tila::
           else w = reinterpret_cast<const unsigned short *>(q)[d] |
                    static_cast<u32>(reinterpret_cast<const unsigned short *>(q)[d + 1]) << 16;
         }
-        qf[k][half * 2 + h] = w;
+        qf[t][k][half] = w;
       }
   }
-
-  float o[DP / 8][4];
+  // keys that the rows of this lane's sums (2 c and 2 c + 1 of each 8) see
+  int limit[NT][2];
 #pragma unroll
-  for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-  float m[2] = {kNegInf, kNegInf}, l[2] = {0.f, 0.f};
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int row = it.row0 + t * 8 + c * 2 + e;
+      limit[t][e] = row < it.rows ? min(it.end, causal ? it.limit0 + row / p.group : it.limit0) : 0;
+    }
+
+  float o[NT][DP / 16][4], m[NT][2], l[NT][2];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    m[t][0] = m[t][1] = kNegInf;
+    l[t][0] = l[t][1] = 0.f;
+#pragma unroll
+    for (int n = 0; n < DP / 16; ++n) o[t][n][0] = o[t][n][1] = o[t][n][2] = o[t][n][3] = 0.f;
+  }
 
   for (int step = 0; step < steps; ++step) {
     const u32 stage = ring_at + (step % kStages) * N::kStage;
@@ -270,64 +292,66 @@ __device__ __forceinline__ void narrow_block(const AttendParams &p, const tila::
       __syncwarp();
       issue(step + kStages - 1);
     }
-    float s[2][4] = {};
+    // S^T: keys g and g + 8 in rows, two chains of sums
+    float s[NT][2][4] = {};
+    {
+      const int r = lane & 15, ch = lane >> 4;
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k) {
+        u32 a[4];
+        ldmatrix4(a, stage + piece(r, k * 2 + ch));
+#pragma unroll
+        for (int t = 0; t < NT; ++t) mma16816<T>(s[t][k & 1], a, qf[t][k][0], qf[t][k][1]);
+      }
+    }
+    u32 pf[NT][2];
+    float scale[NT][2];
+    bool moved = false;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float w[2][2];                                         // [key g, key g + 8][row]
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          w[h][e] = key0 + g + h * 8 < limit[t][e] ? (s[t][0][h * 2 + e] + s[t][1][h * 2 + e]) * p.scale2 : kNegInf;
+        float best = fmaxf(w[0][e], w[1][e]);
+        best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 4));
+        best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 8));
+        best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 16));
+        const float top = fmaxf(m[t][e], best);
+        const float base = top == kNegInf ? 0.f : top;       // nothing seen yet: all weights 0
+        scale[t][e] = tila::exp2_ftz(m[t][e] - base);
+        moved = moved || top != m[t][e];
+        m[t][e] = top;
+        w[0][e] = tila::exp2_ftz(w[0][e] - base);
+        w[1][e] = tila::exp2_ftz(w[1][e] - base);
+        l[t][e] = l[t][e] * scale[t][e] + (w[0][e] + w[1][e]);
+      }
+      // P^T as the B operand: keys in rows there, so each 8x8 block turned around
+      pf[t][0] = transposed(pack2<T>(w[0][0], w[0][1]));
+      pf[t][1] = transposed(pack2<T>(w[1][0], w[1][1]));
+    }
+    // the sums follow the maximum only when it moved
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int n = 0; n < DP / 16; ++n) {
+          o[t][n][0] *= scale[t][0];
+          o[t][n][1] *= scale[t][1];
+          o[t][n][2] *= scale[t][0];
+          o[t][n][3] *= scale[t][1];
+        }
+    }
     {
       const int r = (lane & 7) + ((lane >> 4) << 3), ch = (lane >> 3) & 1;
 #pragma unroll
-      for (int k = 0; k < DP / 16; ++k) {
-        u32 b[4];
-        ldmatrix4(b, stage + piece(r, k * 2 + ch));
-        mma16816<T>(s[0], qf[k], b[0], b[1]);
-        mma16816<T>(s[1], qf[k], b[2], b[3]);
-      }
-    }
-    u32 pf[4];
-    float scale[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int end = min(it.end, limit[h]);
-      float best = kNegInf;
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float &x = s[n][h * 2 + e];
-          x = key0 + n * 8 + c * 2 + e < end ? x * p.scale2 : kNegInf;
-          best = fmaxf(best, x);
-        }
-      best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
-      best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
-      const float top = fmaxf(m[h], best);
-      const float base = top == kNegInf ? 0.f : top;         // nothing seen yet: all weights 0
-      scale[h] = exp2f(m[h] - base);
-      m[h] = top;
-      float sum = 0.f;
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const float x = tila::exp2_fast(s[n][h * 2] - base), y = tila::exp2_fast(s[n][h * 2 + 1] - base);
-        sum += x + y;
-        pf[n * 2 + h] = pack2<T>(x, y);
-      }
-      l[h] = l[h] * scale[h] + sum;
-    }
-    // the sums follow the maximum only when it moved
-    if (__any_sync(0xffffffffu, scale[0] != 1.f || scale[1] != 1.f)) {
-#pragma unroll
-      for (int n = 0; n < DP / 8; ++n) {
-        o[n][0] *= scale[0];
-        o[n][1] *= scale[0];
-        o[n][2] *= scale[1];
-        o[n][3] *= scale[1];
-      }
-    }
-    {
-      const int r = (lane & 7) + (((lane >> 3) & 1) << 3), ch = lane >> 4;
-#pragma unroll
       for (int n = 0; n < DP / 16; ++n) {
-        u32 b[4];
-        ldmatrix4t(b, stage + N::kValues + piece(r, n * 2 + ch));
-        mma16816<T>(o[2 * n], pf, b[0], b[1]);
-        mma16816<T>(o[2 * n + 1], pf, b[2], b[3]);
+        u32 a[4];
+        ldmatrix4t(a, stage + N::kValues + piece(r, n * 2 + ch));
+#pragma unroll
+        for (int t = 0; t < NT; ++t) mma16816<T>(o[t][n], a, pf[t][0], pf[t][1]);
       }
     }
   }
@@ -335,32 +359,37 @@ __device__ __forceinline__ void narrow_block(const AttendParams &p, const tila::
   // join the warps: maxima, sums, then the scaled results through shared memory
   if constexpr (!kTma) copy_wait<0>();
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-    if (c == 0) {
-      row_max[warp][g + 8 * h] = m[h];
-      row_sum[warp][g + 8 * h] = l[h];
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 4);
+      l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 8);
+      l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 16);
+      if (g == 0) {
+        row_max[warp][t * 8 + c * 2 + e] = m[t][e];
+        row_sum[warp][t * 8 + c * 2 + e] = l[t][e];
+      }
     }
-  }
   __syncthreads();
-  float *joined = reinterpret_cast<float *>(smem) + warp * 16 * DP;
+  float *joined = reinterpret_cast<float *>(smem) + warp * kRows * N::kJoin;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int r = g + 8 * h;
-    float top = kNegInf;
+  for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, row_max[w][r]);
-    const float f = m[h] == kNegInf ? 1.f : exp2f(m[h] - top);   // nothing seen: 0 times 1
+    for (int e = 0; e < 2; ++e) {
+      const int r = t * 8 + c * 2 + e;
+      float top = kNegInf;
 #pragma unroll
-    for (int n = 0; n < DP / 8; ++n) {
-      float2 v = make_float2(o[n][h * 2] * f, o[n][h * 2 + 1] * f);
-      *reinterpret_cast<float2 *>(joined + r * DP + n * 8 + c * 2) = v;
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, row_max[w][r]);
+      const float f = m[t][e] == kNegInf ? 1.f : exp2f(m[t][e] - top);   // nothing seen: 0 times 1
+#pragma unroll
+      for (int n = 0; n < DP / 16; ++n) {
+        joined[r * N::kJoin + n * 16 + g] = o[t][n][e] * f;
+        joined[r * N::kJoin + n * 16 + 8 + g] = o[t][n][2 + e] * f;
+      }
     }
-  }
   __syncthreads();
   const float *all = reinterpret_cast<const float *>(smem);
-  for (int r = warp; r < 16; r += kWarps) {
+  for (int r = warp; r < kRows; r += kWarps) {
     const int row = it.row0 + r;
     if (row >= it.rows) continue;
     float top = kNegInf, sum = 0.f;
@@ -378,7 +407,7 @@ __device__ __forceinline__ void narrow_block(const AttendParams &p, const tila::
       for (int d = lane; d < p.dim; d += 32) {
         float v = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) v += all[(w * 16 + r) * DP + d];
+        for (int w = 0; w < kWarps; ++w) v += all[(w * kRows + r) * N::kJoin + d];
         out[d] = Elem<T>::put(v * inverse);
       }
       if (lane == 0 && p.lse != nullptr) p.lse[at] = lse2 * 0.6931471805599453f;
@@ -388,7 +417,7 @@ __device__ __forceinline__ void narrow_block(const AttendParams &p, const tila::
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          const float4 x = *reinterpret_cast<const float4 *>(all + (w * 16 + r) * DP + d);
+          const float4 x = *reinterpret_cast<const float4 *>(all + (w * kRows + r) * N::kJoin + d);
           v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
         }
         v.x *= inverse, v.y *= inverse, v.z *= inverse, v.w *= inverse;
@@ -402,12 +431,12 @@ __device__ __forceinline__ void narrow_block(const AttendParams &p, const tila::
 // Launched behind the wide form, whose results it does not read, it may run beside
 // it; the first block ends after it, so that what waits for this grid waits for
 // both.
-template <typename T, int DP, bool kTma>
+template <typename T, int DP, int NT, bool kTma>
 __global__ void __launch_bounds__(kWarps * 32)
 attend_narrow_kernel(const __grid_constant__ AttendParams p, const __grid_constant__ tila::TensorMap kmap,
                      const __grid_constant__ tila::TensorMap vmap, int prefix_items, int prefix_tiles, int own_tiles) {
   tila::grid_dep_release();
-  narrow_block<T, DP, kTma>(p, kmap, vmap, prefix_items, prefix_tiles, own_tiles);
+  narrow_block<T, DP, NT, kTma>(p, kmap, vmap, prefix_items, prefix_tiles, own_tiles);
   if (blockIdx.x == 0 && threadIdx.x == 0) tila::grid_dep_wait();
 }
 
@@ -487,9 +516,14 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
 #pragma unroll
   for (int i = 0; i < I; ++i) {
     const int d = lane * 4 + i * 128;
-    if (d < p.dim)
+    if (d < p.dim) {
+      if (p.out_vectors)
+        *reinterpret_cast<uint2 *>(out + d) = make_uint2(pack2<T>(acc[i * 4] * inverse, acc[i * 4 + 1] * inverse),
+                                                         pack2<T>(acc[i * 4 + 2] * inverse, acc[i * 4 + 3] * inverse));
+      else
 #pragma unroll
-      for (int e = 0; e < 4; ++e) out[d + e] = Elem<T>::put(acc[i * 4 + e] * inverse);
+        for (int e = 0; e < 4; ++e) out[d + e] = Elem<T>::put(acc[i * 4 + e] * inverse);
+    }
   }
   if (lane == 0 && p.lse != nullptr) p.lse[at] = sum == 0.f ? kNegInf : (top + log2f(sum)) * 0.6931471805599453f;
 }
@@ -532,30 +566,37 @@ int check(const tila_attend_args *a, char *log, size_t cap) {
 
 struct Plan {
   AttendParams p;
-  int prefix_tiles, own_tiles;   // 16 rows each
+  int narrow_rows;               // of a block: 8 or 16
+  int prefix_tiles, own_tiles;   // of as many rows
   bool prefix_wide, own_wide, narrow_tma;
   i64 slots;
 };
 
-// Chunks of the wide form: one block a multiprocessor, so that the blocks of all
-// chunks fill whole waves; a block costs about 4 tiles of keys beside its own
-// (filling the ring, the results).
-int wide_chunk_of(i64 keys, i64 blocks, int &chunks) {
+// Chunks of the wide form, one block a multiprocessor.  A block takes about 2.1 us
+// for a tile of 128 keys and 9.5 us beside that (queries, filling the ring, results).
+// Where the narrow form follows (`narrow_bytes`, half of what the longest sequences
+// would be), it starts beside the wide form on the multiprocessors that are left,
+// which fetch about 54 GB/s each, 6 TB/s in all: the split that ends both first.
+int wide_chunk_of(i64 keys, i64 blocks, double narrow_bytes, int &chunks) {
   const i64 tiles = (keys + 127) / 128;
-  i64 best = 1, cost = 0;
+  i64 best = 1;
+  double least = 0;
   for (i64 n = 1; n <= std::min<i64>(tiles, 64); ++n) {
-    const i64 c = ((blocks * n + kSms - 1) / kSms) * ((tiles + n - 1) / n + 4);
-    if (n == 1 || c < cost) best = n, cost = c;
+    const double wide = ((blocks * n + kSms - 1) / kSms) * (9.5e-6 + 2.1e-6 * ((tiles + n - 1) / n));
+    const double beside = std::min(6e12, 54e9 * std::max<i64>(0, kSms - blocks * n));
+    const double left = std::max(0., narrow_bytes - beside * wide);
+    const double cost = left > 0 ? wide + left / 6e12 : std::max(wide, beside > 0 ? narrow_bytes / beside : 0.);
+    if (n == 1 || cost < least) best = n, least = cost;
   }
   const i64 each = (tiles + best - 1) / best;
   chunks = static_cast<int>((tiles + each - 1) / each);
   return static_cast<int>(each * 128);
 }
 
-// Chunks: enough blocks for two a multiprocessor and twice that many again, and
-// none longer than 512 keys beyond that, since sequences end at different
-// lengths and the longest chunk is what the last block waits for.  A chunk's
-// partial result costs 8 bytes an element beside 4 bytes a key for every row.
+// Chunks of the narrow form: enough blocks for four a multiprocessor, and none
+// longer than 512 keys beyond that, since sequences end at different lengths
+// and the longest chunk is what the last block waits for.  A chunk's partial
+// result costs 8 bytes an element beside 4 bytes a key for every row.
 int chunk_of(i64 keys, i64 blocks, int &chunks) {
   if (keys <= 0) {
     chunks = 0;
@@ -608,20 +649,23 @@ Plan plan(const tila_attend_args &a) {
   p.scale2 = a.scale * 1.4426950408889634f;
   p.q_words = a.q % 4 == 0 && a.q_stride[0] % 2 == 0 && a.q_stride[1] % 2 == 0;
   const i64 rows = (a.query_offsets == 0 ? a.batch : a.tokens) * p.group;
-  r.prefix_tiles = static_cast<int>((rows + 15) / 16);
-  r.own_tiles = (p.max_queries * p.group + 15) / 16;
   p.q_vectors = a.q % 16 == 0 && a.q_stride[0] % 8 == 0 && a.q_stride[1] % 8 == 0;
+  p.out_vectors = a.out % 8 == 0 && a.out_stride[0] % 4 == 0 && a.out_stride[1] % 4 == 0;
   const i64 own_rows = static_cast<i64>(p.max_queries) * p.group;
   const i64 own_keys = static_cast<i64>(a.table_width) * a.page_size;
   const bool wide = wide_possible(a);
   r.narrow_tma = tma_possible(a) && a.page_size % kSlice == 0;
   r.prefix_wide = wide && p.prefix > 0 && rows > 16;
   r.own_wide = wide && own_keys > 0 && own_rows > 16;
+  r.narrow_rows = (r.own_wide || own_rows <= 8) && (r.prefix_wide || rows <= 8) ? 8 : 16;
+  r.prefix_tiles = static_cast<int>((rows + r.narrow_rows - 1) / r.narrow_rows);
+  r.own_tiles = static_cast<int>((own_rows + r.narrow_rows - 1) / r.narrow_rows);
   p.prefix_chunk = r.prefix_wide
-                       ? wide_chunk_of(p.prefix, (rows + 255) / 256 * p.kv_heads, p.prefix_chunks)
+                       ? wide_chunk_of(p.prefix, (rows + 255) / 256 * p.kv_heads,
+                                       r.own_wide ? 0. : 2. * own_keys * p.batch * p.kv_heads * p.dim, p.prefix_chunks)
                        : chunk_of(p.prefix, static_cast<i64>(r.prefix_tiles) * p.kv_heads, p.prefix_chunks);
   p.own_chunk = r.own_wide
-                    ? wide_chunk_of(own_keys, (own_rows + 255) / 256 * p.kv_heads * p.batch, p.own_chunks)
+                    ? wide_chunk_of(own_keys, (own_rows + 255) / 256 * p.kv_heads * p.batch, 0., p.own_chunks)
                     : chunk_of(own_keys, static_cast<i64>(r.own_tiles) * p.kv_heads * p.batch, p.own_chunks);
   if (p.own_chunks == 0 && p.prefix_chunks == 0) p.own_chunks = 1;   // no keys at all: a block writes the zeros
   r.slots = p.prefix_chunks + p.own_chunks;
@@ -633,13 +677,13 @@ u64 workspace_of(const Plan &r) {
   return r.p.direct ? 0 : static_cast<u64>(r.slots) * r.p.tokens * r.p.heads * (r.p.dim + 1) * sizeof(float);
 }
 
-template <typename T, int DP, bool kTma>
+template <typename T, int DP, int NT, bool kTma>
 cudaError_t launch_narrow(const Plan &r, const tila::TensorMap &k, const tila::TensorMap &v, cudaStream_t stream) {
   const i64 prefix_items = r.prefix_wide ? 0 : static_cast<i64>(r.prefix_tiles) * r.p.kv_heads * r.p.prefix_chunks;
   const i64 own_items = r.own_wide ? 0 : static_cast<i64>(r.own_tiles) * r.p.kv_heads * r.p.own_chunks * r.p.batch;
   if (prefix_items + own_items == 0) return cudaSuccess;
   if (prefix_items + own_items > 0x7fffffff) return cudaErrorInvalidValue;
-  const auto kernel = attend_narrow_kernel<T, DP, kTma>;
+  const auto kernel = attend_narrow_kernel<T, DP, NT, kTma>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Narrow<DP>::kBytes);
   if (e != cudaSuccess) return e;
   return launch_kernel(kernel, static_cast<unsigned>(prefix_items + own_items), kWarps * 32, Narrow<DP>::kBytes,
@@ -648,7 +692,9 @@ cudaError_t launch_narrow(const Plan &r, const tila::TensorMap &k, const tila::T
 
 template <typename T, int DP>
 cudaError_t launch_narrow(const Plan &r, const tila::TensorMap &k, const tila::TensorMap &v, cudaStream_t stream) {
-  return r.narrow_tma ? launch_narrow<T, DP, true>(r, k, v, stream) : launch_narrow<T, DP, false>(r, k, v, stream);
+  if (r.narrow_rows == 8)
+    return r.narrow_tma ? launch_narrow<T, DP, 1, true>(r, k, v, stream) : launch_narrow<T, DP, 1, false>(r, k, v, stream);
+  return r.narrow_tma ? launch_narrow<T, DP, 2, true>(r, k, v, stream) : launch_narrow<T, DP, 2, false>(r, k, v, stream);
 }
 
 template <typename T>

@@ -36,6 +36,7 @@ struct AttendParams {
   int own_chunk, own_chunks;        // slots prefix_chunks ..
   int direct;                       // one chunk in all: blocks write the result itself
   int q_words, q_vectors;           // q can be read in 4-byte words, in 16-byte vectors
+  int out_vectors;                  // out can be written in vectors of 4 elements
 };
 
 constexpr float kNegInf = -__builtin_huge_valf();

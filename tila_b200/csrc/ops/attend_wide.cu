@@ -45,9 +45,15 @@ constexpr int kThreads = 384;
 // would otherwise wait for registers that do not exist.
 constexpr int kLaunchRegisters = 168;
 constexpr int kTile = 128;                       // keys of a tile, rows of a row tile
+constexpr int kHalf = kTile * 128;               // bytes of 64 elements of a tile
 constexpr float kGrowth = 8.f;                   // log2 of what weights may reach before O is scaled
 
 template <int DP> struct Wide {
+  // At 64 elements tensor memory has room for P beside S: S of the next tile is
+  // issued as soon as the warpgroup has read S, and is there when it comes back.
+  static constexpr bool kEarly = DP == 64;
+  static constexpr u32 kWeightsAt = kEarly ? 256 : 0, kWeightsStep = kEarly ? 64 : 128;   // columns of P
+  static constexpr u32 kSumsAt = kEarly ? 384 : 256;                                      // columns of O
   static constexpr int kTileBytes = kTile * DP * 2;
   static constexpr int kStages = DP == 128 ? 5 : 9;
   static constexpr int kRing = 2 * kTileBytes;   // behind the two query tiles
@@ -56,6 +62,23 @@ template <int DP> struct Wide {
   static_assert(2 * kTile * kRowFloats * 4 <= kStages * kTileBytes, "results are staged in the ring");
   static_assert(kBytes <= 227 * 1024, "shared memory of a block");
 };
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// One lane of the warp, the same one each time, in a form that the compiler knows
+// to be one: what it feeds to tcgen05 instructions stays in uniform registers.
+__device__ __forceinline__ bool elected() {
+  u32 one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
+
+// A value that all lanes hold, as one that the compiler knows to be uniform.
+__device__ __forceinline__ u32 uniform(u32 x) { return __shfl_sync(0xffffffffu, x, 0); }
 
 // A bounded wait by a whole warp: all lanes go on, or none.
 __device__ __forceinline__ bool warp_wait(u64 *bar, u32 parity, u32 *err, u32 where, int *dead) {
@@ -88,7 +111,9 @@ __device__ __forceinline__ void write_row(u32 o_col, bool any, float mine, float
 struct Barriers {
   u64 full[9], empty[9];
   u64 scores[2];      // S of a warpgroup's tile is there (and P V of its tile before)
+  u64 taken[2];       // S has been read (kEarly)
   u64 weights[2];     // P is in tensor memory
+  u64 summed[2];      // P V of a warpgroup's tile is done (kEarly)
   u64 queries, done;
 };
 
@@ -156,6 +181,8 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
     for (int i = 0; i < 2; ++i) {
       tila::mbar_init(&bars.scores[i], 1);
       tila::mbar_init(&bars.weights[i], kTile);
+      tila::mbar_init(&bars.taken[i], kTile);
+      tila::mbar_init(&bars.summed[i], 1);
     }
     tila::mbar_init(&bars.queries, 2 * kTile);
     tila::mbar_init(&bars.done, 1);
@@ -176,113 +203,141 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
   if (warp >= 8) tila::reg_dealloc<64>();
   if (warp == 8) {
     // ---- copies -----------------------------------------------------------------
+    // A lane copies one box: 64 elements of one page's rows in the tile.  Its page
+    // is looked up one tile ahead.
     constexpr int kHalves = DP / 64;
     const int box_rows = min(p.page_size, kTile);
-    auto copy = [&](int item, int tile, const TensorMap *map) -> bool {
+    const int box = lane / kHalves, half = lane % kHalves;
+    auto look_up = [&](int tile) {
+      const int key = begin + tile * kTile + box * box_rows;
+      if (box * box_rows >= kTile || key >= end) return 0;
+      int page, row;
+      split_key(p, key, page, row);
+      return pages[page];
+    };
+    auto copy = [&](int item, int tile, int page, const TensorMap *map) -> bool {
       const int stage = item % W::kStages;
+      const int key0 = begin + tile * kTile;
+      const int boxes = (min(kTile, end - key0) + box_rows - 1) / box_rows;   // pages that hold seen keys
+      int index, row;
+      split_key(p, key0 + box * box_rows, index, row);
       if (item >= W::kStages &&
           !warp_wait(&bars.empty[stage], (item / W::kStages - 1) & 1, p.err, __LINE__, dead_ptr))
         return false;
-      const int key0 = begin + tile * kTile;
-      const int boxes = (min(kTile, end - key0) + box_rows - 1) / box_rows;   // pages that hold seen keys
       if (lane == 0) tila::mbar_arrive_expect_tx(&bars.full[stage], boxes * kHalves * box_rows * 128);
       __syncwarp();
-      unsigned char *dst = smem + W::kRing + stage * W::kTileBytes;
-      if (lane < boxes * kHalves) {
-        const int i = lane / kHalves, half = lane % kHalves;
-        int page, row;
-        split_key(p, key0 + i * box_rows, page, row);
-        page = checked_page(p, pages, page);
-        if (page < 0) page = p.num_pages;                   // outside the tensor: reads as zeros
-        tila::tma_load_4d(dst + half * (kTile * 128) + i * box_rows * 128, map, &bars.full[stage], half * 64, row,
-                          head, page);
+      if (box < boxes) {
+        if (page < 0 || page >= p.num_pages) {
+          tila::report_error(p.err, kErrIndex, index);
+          page = p.num_pages;                               // outside the tensor: reads as zeros
+        }
+        tila::tma_load_4d(smem + W::kRing + stage * W::kTileBytes + half * kHalf + box * box_rows * 128, map,
+                          &bars.full[stage], half * 64, row, head, page);
       }
       return true;
     };
     int item = 0;
     bool ok = true;
-    for (int j = 0; ok && j < first_keys; ++j) ok = copy(item++, j, &kmap);
+    for (int j = 0; ok && j < first_keys; ++j) ok = copy(item++, j, look_up(j), &kmap);
+    int values = look_up(0), keys = look_up(ahead);
     for (int j = 0; ok && j < tiles; ++j) {
-      ok = copy(item++, j, &vmap);
-      if (ok && j + ahead < tiles) ok = copy(item++, j + ahead, &kmap);
+      const int next_values = look_up(j + 1), next_keys = look_up(j + 1 + ahead);
+      ok = copy(item++, j, values, &vmap);
+      if (ok && j + ahead < tiles) ok = copy(item++, j + ahead, keys, &kmap);
+      values = next_values;
+      keys = next_keys;
     }
   } else if (warp == 9) {
     // ---- MMAs -------------------------------------------------------------------
-    const u32 base4 = tila::smem_u32(smem) >> 4;
+    const u32 base4 = uniform(tila::smem_u32(smem)) >> 4, tm = uniform(tmem);
+    const int n_tiles = static_cast<int>(uniform(tiles)), key_end = static_cast<int>(uniform(end));
+    const bool turns = uniform(shared_rows) != 0;                 // the warpgroups take tiles in turn
+    const bool second = uniform(rows - row0 > kTile) != 0;        // the second row tile exists
+    const int lead = turns ? 2 : 1;
     constexpr u32 kFormat = __is_same(T, __half) ? 0u : (1u << 7) | (1u << 10);
     constexpr u32 kScoresDesc = tila::idesc_f16_f32(128, 128, 0, 0) | kFormat;
     constexpr u32 kValuesDesc = tila::idesc_f16_f32(128, DP, 0, 1) | kFormat;
-    auto stage_of = [&](int item) { return W::kRing + (item % W::kStages) * W::kTileBytes; };
     auto wait_full = [&](int item) {
       return warp_wait(&bars.full[item % W::kStages], (item / W::kStages) & 1, p.err, __LINE__, dead_ptr);
     };
+    auto stage_at = [&](int item) -> u32 { return W::kRing + (item % W::kStages) * W::kTileBytes; };
     auto scores = [&](int w, int item) {
-      if (lane == 0) {
-        const u32 q = shared_rows ? 0 : w * W::kTileBytes, k = stage_of(item);
+      const u32 q = turns ? 0 : w * W::kTileBytes, k = stage_at(item);
+      if (elected()) {
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk) {
-          const u32 off = (kk / 4) * (kTile * 128) + (kk % 4) * 32;
-          tila::mma_f16_ss(tmem + w * 128, tila::sdesc<16, 1024, 2>(base4, q + off),
+          const u32 off = (kk / 4) * kHalf + (kk % 4) * 32;
+          tila::mma_f16_ss(tm + w * 128, tila::sdesc<16, 1024, 2>(base4, q + off),
                            tila::sdesc<16, 1024, 2>(base4, k + off), kScoresDesc, kk > 0);
         }
         tila::mma_commit(&bars.scores[w]);
       }
       __syncwarp();
     };
-    bool ok = tiles == 0 || warp_wait(&bars.queries, 0, p.err, __LINE__, dead_ptr);
-    const bool second = !shared_rows && rows - row0 > kTile;      // the second row tile exists
+    bool ok = n_tiles == 0 || warp_wait(&bars.queries, 0, p.err, __LINE__, dead_ptr);
     int item = 0;
-    for (int j = 0; ok && j < first_keys; ++j, ++item) {
+    for (int j = 0; ok && j < min(lead, n_tiles); ++j, ++item) {
       ok = wait_full(item);
       if (!ok) break;
       tila::tc_fence_after();
-      if (shared_rows) {
+      if (turns) {
         scores(j, item);
       } else {
         scores(0, item);
         if (second) scores(1, item);
       }
-      if (lane == 0) tila::mma_commit(&bars.empty[item % W::kStages]);
+      if (elected()) tila::mma_commit(&bars.empty[item % W::kStages]);
+      __syncwarp();
     }
-    for (int j = 0; ok && j < tiles; ++j) {
+    for (int j = 0; ok && j < n_tiles; ++j) {
       const int values = item++;
-      const bool more = j + ahead < tiles;
+      const bool more = j + lead < n_tiles;
       const int keys = more ? item++ : 0;
       ok = wait_full(values) && (!more || wait_full(keys));
       if (!ok) break;
-      const int seen = min(kTile, end - (begin + j * kTile));
-      const int steps = (seen + 15) >> 4;
+      const int seen = min(kTile, key_end - (begin + j * kTile));
+      const int steps = static_cast<int>(uniform((seen + 15) >> 4));
       if (seen & 15) {
         // values behind the end, up to the group of 16 that P V covers
-        unsigned char *v = smem + stage_of(values);
+        unsigned char *v = smem + stage_at(values);
         for (int i = lane; i < (steps * 16 - seen) * (DP / 8); i += 32) {
           const int r = seen + i / (DP / 8), c = i % (DP / 8);
-          *reinterpret_cast<uint4 *>(v + (c / 8) * (kTile * 128) + r * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4 *>(v + (c / 8) * kHalf + r * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
         }
         tila::fence_proxy_async_smem();
         __syncwarp();
       }
-      for (int w = shared_rows ? (j & 1) : 0; ok && w <= (shared_rows ? (j & 1) : (second ? 1 : 0)); ++w) {
-        const int turn = shared_rows ? j >> 1 : j;
+      const int w_first = turns ? (j & 1) : 0, w_last = turns ? (j & 1) : (second ? 1 : 0);
+      const int turn = turns ? j >> 1 : j;
+      for (int w = w_first; ok && w <= w_last; ++w) {
+        if (W::kEarly && more) {
+          ok = warp_wait(&bars.taken[w], turn & 1, p.err, __LINE__, dead_ptr);
+          if (!ok) break;
+          tila::tc_fence_after();
+          scores(w, keys);
+        }
         ok = warp_wait(&bars.weights[w], turn & 1, p.err, __LINE__, dead_ptr);
         if (!ok) break;
         tila::tc_fence_after();
-        if (lane == 0) {
-          const u32 v = stage_of(values);
-          for (int kk = 0; kk < steps; ++kk)
-            tila::mma_f16_ts(tmem + 256 + w * DP, tmem + w * 128 + kk * 8,
-                             tila::sdesc<kTile * 128, 1024, 2>(base4, v + kk * 2048), kValuesDesc, turn > 0 || kk > 0);
+        const u32 v = stage_at(values);
+        if (elected()) {
+#pragma unroll
+          for (int kk = 0; kk < kTile / 16; ++kk)
+            if (kk < steps)
+              tila::mma_f16_ts(tm + W::kSumsAt + w * DP, tm + W::kWeightsAt + w * W::kWeightsStep + kk * 8,
+                               tila::sdesc<kHalf, 1024, 2>(base4, v + kk * 2048), kValuesDesc, turn > 0 || kk > 0);
+          if (W::kEarly) tila::mma_commit(&bars.summed[w]);
         }
         __syncwarp();
-        if (more) scores(w, keys);
+        if (!W::kEarly && more) scores(w, keys);
       }
-      if (ok && lane == 0) {
+      if (ok && elected()) {
         tila::mma_commit(&bars.empty[values % W::kStages]);
         if (more) tila::mma_commit(&bars.empty[keys % W::kStages]);
       }
       __syncwarp();
     }
-    if (ok && tiles > 0 && lane == 0) tila::mma_commit(&bars.done);
+    if (ok && n_tiles > 0 && elected()) tila::mma_commit(&bars.done);
     __syncwarp();
   } else if (warp < 8) {
     // ---- softmax: warpgroup w, one row a thread ------------------------------------
@@ -297,30 +352,34 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
       // the warp's 32 rows of queries, whole rows at a time, swizzled as TMA would
       // leave them
       constexpr int kPieces = DP / 8, kRows = 32 / kPieces;  // 16-byte pieces of a row; rows of one access
-      const i64 from = valid ? (token0 + token) * p.q_stride[0] + out_head * p.q_stride[1] : -1;
+      // (rows that are not there read the first one, so that no load is conditional and
+      // all are in flight together; they are cleared below)
+      const i64 from = (token0 + token) * p.q_stride[0] + out_head * p.q_stride[1];
       const int c = lane % kPieces;
+      const bool in = c * 8 < p.dim;
+      const T *q = static_cast<const T *>(p.q) + (in ? c * 8 : 0);
       uint4 x[32 / kRows];
+      if (p.q_vectors) {
 #pragma unroll
-      for (int i = 0; i < 32 / kRows; ++i) {
-        const i64 at = __shfl_sync(0xffffffffu, from, i * kRows + lane / kPieces);
-        x[i] = make_uint4(0, 0, 0, 0);
-        if (at >= 0 && c * 8 < p.dim) {
-          const T *q = static_cast<const T *>(p.q) + at + c * 8;
-          if (p.q_vectors) {
-            x[i] = *reinterpret_cast<const uint4 *>(q);
-          } else {
-            const unsigned short *e = reinterpret_cast<const unsigned short *>(q);
-            x[i] = make_uint4(e[0] | static_cast<u32>(e[1]) << 16, e[2] | static_cast<u32>(e[3]) << 16,
-                              e[4] | static_cast<u32>(e[5]) << 16, e[6] | static_cast<u32>(e[7]) << 16);
-          }
+        for (int i = 0; i < 32 / kRows; ++i)
+          x[i] = *reinterpret_cast<const uint4 *>(q + __shfl_sync(0xffffffffu, from, i * kRows + lane / kPieces));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32 / kRows; ++i) {
+          const unsigned short *e = reinterpret_cast<const unsigned short *>(
+              q + __shfl_sync(0xffffffffu, from, i * kRows + lane / kPieces));
+          x[i] = make_uint4(e[0] | static_cast<u32>(e[1]) << 16, e[2] | static_cast<u32>(e[3]) << 16,
+                            e[4] | static_cast<u32>(e[5]) << 16, e[6] | static_cast<u32>(e[7]) << 16);
         }
       }
+      const u32 there = __ballot_sync(0xffffffffu, valid);
       const u32 flip = p.scale2 < 0.f ? 0x80008000u : 0u;    // scores are scaled by |scale|
 #pragma unroll
       for (int i = 0; i < 32 / kRows; ++i) {
         const int q_row = (warp & 3) * 32 + i * kRows + lane / kPieces;
         x[i].x ^= flip, x[i].y ^= flip, x[i].z ^= flip, x[i].w ^= flip;
-        *reinterpret_cast<uint4 *>(smem + w * W::kTileBytes + q_row * 128 + (c / 8) * (kTile * 128) +
+        if (!in || !(there >> (q_row & 31) & 1)) x[i] = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4 *>(smem + w * W::kTileBytes + q_row * 128 + (c / 8) * kHalf +
                                    (((c % 8) ^ (q_row & 7)) << 4)) = x[i];
       }
       tila::fence_proxy_async_smem();
@@ -328,7 +387,8 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
     tila::mbar_arrive(&bars.queries);
 
     const u32 lanes = tmem + ((warp & 3) << 21);            // this warp's 32 lanes
-    const u32 s_col = lanes + w * 128, o_col = lanes + 256 + w * DP;
+    const u32 s_col = lanes + w * 128, o_col = lanes + W::kSumsAt + w * DP;
+    const u32 p_col = lanes + W::kWeightsAt + w * W::kWeightsStep;
     const float scale = fmaxf(fabsf(p.scale2), 1e-30f);     // above 0, so that -inf stays what it is
     float top = kNegInf, sum = 0.f;
     const bool works = shared_rows || row0 + w * kTile < rows;
@@ -340,22 +400,35 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
       tila::tc_fence_after();
       float s[kTile];
       tila::tmem_load_row<kTile>(s_col, s);
+      if (W::kEarly) {
+        tila::tc_fence_before();
+        tila::mbar_arrive(&bars.taken[w]);
+      }
       const int key0 = begin + j * kTile;
       const int seen = min(end, limit) - key0;              // columns that the row sees
       if (__any_sync(0xffffffffu, seen < kTile)) {
 #pragma unroll
         for (int i = 0; i < kTile; ++i) s[i] = i < seen ? s[i] : kNegInf;
       }
-      float best[4] = {s[0], s[1], s[2], s[3]};
+      float best[2] = {s[0], s[1]};
 #pragma unroll
-      for (int i = 4; i < kTile; i += 4)
+      for (int i = 2; i < kTile; i += 4)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) best[e] = fmaxf(best[e], s[i + e]);
-      const float high = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3])) * scale;
+        for (int e = 0; e < 2; ++e) {
+          if (i + e + 2 < kTile) best[e] = max3(best[e], s[i + e], s[i + e + 2]);
+          else best[e] = fmaxf(best[e], s[i + e]);
+        }
+      const float high = fmaxf(best[0], best[1]) * scale;
       const bool grew = high > top + kGrowth || (top == kNegInf && high > kNegInf);
       const float factor = grew ? exp2f(top - high) : 1.f;
       if (grew) top = high;
       sum *= factor;
+      if (W::kEarly && turn > 0) {
+        // P V of the tile before reads P, and adds to O
+        ok = warp_wait(&bars.summed[w], (turn - 1) & 1, p.err, __LINE__, dead_ptr);
+        if (!ok) break;
+        tila::tc_fence_after();
+      }
       if (turn > 0 && __any_sync(0xffffffffu, grew)) {
 #pragma unroll
         for (int c = 0; c < DP; c += 32) {
@@ -377,11 +450,11 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
         for (int i = 0; i < 32; ++i) {
           const int k = half * 64 + i * 2;
           const u64 x = tila::fma2(tila::pk2(s[k], s[k + 1]), scale_2, base_2);
-          const float a = tila::exp2_fast(tila::lo2(x)), b = tila::exp2_fast(tila::hi2(x));
+          const float a = tila::exp2_ftz(tila::lo2(x)), b = tila::exp2_ftz(tila::hi2(x));
           sums[i & 1] = tila::add2(sums[i & 1], tila::pk2(a, b));
           packed[i] = __uint_as_float(wide_pack<T>(a, b));
         }
-        tila::tmem_st32(s_col + half * 32, packed);
+        tila::tmem_st32(p_col + half * 32, packed);
       }
       const u64 both = tila::add2(sums[0], sums[1]);
       sum += tila::lo2(both) + tila::hi2(both);
@@ -390,7 +463,7 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
       tila::mbar_arrive(&bars.weights[w]);
     }
 
-    // ---- results: normalised, staged in the ring (free by now), a bulk copy a row -----
+    // ---- results: normalised, staged in the ring (free by now) ---------------
     if (tiles > 0) ok = warp_wait(&bars.done, 0, p.err, __LINE__, dead_ptr) && ok;
     tila::tc_fence_after();
     float *staged = reinterpret_cast<float *>(smem + W::kRing) + (w * kTile + r) * W::kRowFloats;
@@ -416,20 +489,42 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
     }
     if (!shared_rows || w == 0) {
       write_row<DP>(o_col, turn > 0, mine, other, shared_rows ? partner : nullptr, staged);
-      if (valid && ok) {
-        const i64 at = (token0 + token) * p.heads + out_head;
-        const i64 place = slot * p.tokens * p.heads + at;
-        if (p.direct) {
-          T *out = static_cast<T *>(p.out) + (token0 + token) * p.out_stride[0] + out_head * p.out_stride[1];
-          for (int d = 0; d < p.dim; ++d) out[d] = Elem<T>::put(staged[d]);
-          if (p.lse != nullptr) p.lse[at] = lse * 0.6931471805599453f;
-        } else {
-          p.partial_lse[place] = lse;
-          tila::fence_proxy_async_smem();
-          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(p.partial + place * p.dim),
-                       "r"(tila::smem_u32(staged)), "r"(p.dim * 4) : "memory");
-          tila::bulk_commit();
-          tila::bulk_wait_read();
+      const int at = valid && ok ? static_cast<int>((token0 + token) * p.heads + out_head) : -1;
+      const i64 first = slot * p.tokens * p.heads;
+      if (at >= 0) {
+        if (!p.direct) p.partial_lse[first + at] = lse;
+        else if (p.lse != nullptr) p.lse[at] = lse * 0.6931471805599453f;
+      }
+      __syncwarp();
+      // the warp writes its 32 rows, a whole row at a time
+      const float *from = staged - lane * W::kRowFloats + lane * 4;
+      const bool in = lane * 4 < p.dim;
+      if (!p.direct) {
+        float *to = p.partial + first * p.dim + lane * 4;
+#pragma unroll 8
+        for (int i = 0; i < 32; ++i) {
+          const int row_at = __shfl_sync(0xffffffffu, at, i);
+          if (row_at >= 0 && in)
+            *reinterpret_cast<float4 *>(to + static_cast<i64>(row_at) * p.dim) =
+                *reinterpret_cast<const float4 *>(from + i * W::kRowFloats);
+        }
+      } else {
+        const i64 out_at = (token0 + token) * p.out_stride[0] + out_head * p.out_stride[1];
+#pragma unroll 4
+        for (int i = 0; i < 32; ++i) {
+          const i64 row_at = __shfl_sync(0xffffffffu, at >= 0 ? out_at : -1, i);
+          if (row_at >= 0 && in) {
+            const float4 x = *reinterpret_cast<const float4 *>(from + i * W::kRowFloats);
+            T *to = static_cast<T *>(p.out) + row_at + lane * 4;
+            if (p.out_vectors) {
+              *reinterpret_cast<uint2 *>(to) = make_uint2(wide_pack<T>(x.x, x.y), wide_pack<T>(x.z, x.w));
+            } else {
+              to[0] = Elem<T>::put(x.x);
+              to[1] = Elem<T>::put(x.y);
+              to[2] = Elem<T>::put(x.z);
+              to[3] = Elem<T>::put(x.w);
+            }
+          }
         }
       }
     }
