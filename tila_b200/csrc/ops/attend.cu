@@ -440,19 +440,19 @@ attend_narrow_kernel(const __grid_constant__ AttendParams p, const __grid_consta
   if (blockIdx.x == 0 && threadIdx.x == 0) tila::grid_dep_wait();
 }
 
-// out = sum over slots of 2^(lse_s - lse) * partial_s, lse = log2 sum 2^lse_s: one
-// warp for each row of q and head.  Bound by reading the partial results, which
-// the blocks before left in L2.
-template <typename T, int I>
+// out = sum over slots of 2^(lse_s - lse) * partial_s, lse = log2 sum 2^lse_s: L lanes
+// for each row of q and head.  Bound by reading the partial results, which the
+// blocks before left in L2.  Which row, sequence and chunks is found out before the
+// wait for them: lengths and offsets are older than the kernels waited for.
+template <typename T, int L, int I>
 __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant__ AttendParams p) {
-  const int lane = threadIdx.x & 31;
-  const i64 at = static_cast<i64>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  tila::grid_dep_wait();
-  if (at >= p.tokens * p.heads) return;
-  const i64 token = at / p.heads;
-  const int head = static_cast<int>(at - token * p.heads);
+  const int lane = threadIdx.x % L;
+  const i64 at = static_cast<i64>(blockIdx.x) * (256 / L) + threadIdx.x / L;
+  const bool there = at < p.tokens * p.heads;
+  const int token = there ? static_cast<int>(at) / p.heads : 0;
+  const int head = static_cast<int>(at) - token * p.heads;
   // the row's sequence, and the chunks of its own tokens that it saw
-  int b = static_cast<int>(token);
+  int b = token;
   if (p.offsets != nullptr) {
     int lo = 0, hi = p.batch;                 // the last b with offsets[b] <= token
     while (hi - lo > 1) {
@@ -461,14 +461,15 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
     }
     b = lo;
   }
-  if (b >= p.batch) return;
-  i64 first;
-  int count;
-  sequence_rows(p, b, first, count);
-  if (token < first || token >= first + count) return;
-  const int limit = own_length(p, b) - count + 1 + static_cast<int>(token - first);
-  const int own = limit <= 0 ? 0 : min((limit + p.own_chunk - 1) / p.own_chunk, p.own_chunks);
-  const int slots = p.prefix_chunks + own;
+  i64 first = 0;
+  int count = 0, slots = 0;
+  if (there && b < p.batch) {
+    sequence_rows(p, b, first, count);
+    const int limit = own_length(p, b) - count + 1 + static_cast<int>(token - first);
+    slots = p.prefix_chunks + (limit <= 0 ? 0 : min((limit + p.own_chunk - 1) / p.own_chunk, p.own_chunks));
+  }
+  tila::grid_dep_wait();
+  if (!there || token < first || token >= first + count) return;
   const i64 step = p.tokens * p.heads;
   // the running maximum over slots keeps each slot's lse and row one load away: 8
   // slots' rows are in flight at a time, and none waits for the weights
@@ -485,7 +486,8 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
         lse[s] = p.partial_lse[place];
 #pragma unroll
         for (int i = 0; i < I; ++i)
-          if (lane * 4 + i * 128 < p.dim) row[s][i] = *reinterpret_cast<const float4 *>(p.partial + place * p.dim + lane * 4 + i * 128);
+          if (lane * 4 + i * 4 * L < p.dim)
+            row[s][i] = *reinterpret_cast<const float4 *>(p.partial + place * p.dim + lane * 4 + i * 4 * L);
       }
     }
     float high = top;
@@ -512,10 +514,10 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
     }
   }
   const float inverse = sum == 0.f ? 0.f : 1.f / sum;
-  T *out = static_cast<T *>(p.out) + token * p.out_stride[0] + head * p.out_stride[1];
+  T *out = static_cast<T *>(p.out) + static_cast<i64>(token) * p.out_stride[0] + head * p.out_stride[1];
 #pragma unroll
   for (int i = 0; i < I; ++i) {
-    const int d = lane * 4 + i * 128;
+    const int d = lane * 4 + i * 4 * L;
     if (d < p.dim) {
       if (p.out_vectors)
         *reinterpret_cast<uint2 *>(out + d) = make_uint2(pack2<T>(acc[i * 4] * inverse, acc[i * 4 + 1] * inverse),
@@ -703,9 +705,12 @@ cudaError_t launch(const Plan &r, const tila::TensorMap &k, const tila::TensorMa
                   : r.p.dim <= 128 ? launch_narrow<T, 128>(r, k, v, stream)
                                    : launch_narrow<T, 256>(r, k, v, stream);
   if (e != cudaSuccess || r.p.direct) return e;
-  const unsigned blocks = static_cast<unsigned>((r.p.tokens * r.p.heads + 7) / 8);
-  return launch_kernel(r.p.dim <= 128 ? attend_join_kernel<T, 1> : attend_join_kernel<T, 2>, blocks, 256, 0, stream,
-                       true, r.p);
+  const int lanes = r.p.dim <= 64 ? 16 : 32;
+  const unsigned blocks = static_cast<unsigned>((r.p.tokens * r.p.heads * lanes + 255) / 256);
+  return launch_kernel(r.p.dim <= 64    ? attend_join_kernel<T, 16, 1>
+                       : r.p.dim <= 128 ? attend_join_kernel<T, 32, 1>
+                                        : attend_join_kernel<T, 32, 2>,
+                       blocks, 256, 0, stream, true, r.p);
 }
 
 }  // namespace
