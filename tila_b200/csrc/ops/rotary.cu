@@ -12,11 +12,13 @@
 //
 // Bound by memory: a row is read once and written once.  One block takes a few
 // tokens with all their heads, of every tensor of the call, so that the sines
-// of a token are computed once and shared through shared memory.  A row is
-// spread over as many lanes as it has units; a unit is the two V-element vectors
+// of a token are computed once and shared through shared memory; as many tokens as
+// give each thread one sine, where there are enough of them for the whole GPU.  A row
+// is spread over as many lanes as it has units; a unit is the two V-element vectors
 // that hold both halves of V pairs, so that neither layout moves data between
 // lanes, and V elements are one 16-byte access where sizes, strides and
-// addresses allow it.  The first row's loads are issued before the sines.
+// addresses allow it.  A row's loads are issued one row ahead, the first before the
+// sines.
 
 #include "ops_common.cuh"
 
@@ -40,11 +42,15 @@ struct Params {
   Rows rows[3];
   int heads;             // of all tensors
   int num_rows;
-  i64 tokens_all, tokens;
+  int batch;
+  i64 tokens;            // of one batch entry
+  i64 blocks_per_batch;
   int dim, half, interleaved;
   int lanes;             // lanes of a row, a power of two
   int units;
+  int full;              // every lane has whole units
   int tokens_per_block;
+  int step_tokens, step_heads;   // from a group's row to its next one
   int any_norm, any_paged;
   float sign;            // -1 rotates back
   float amplitude, eps, inv_dim;
@@ -78,39 +84,50 @@ __device__ __forceinline__ void unit_at(const Params &p, int u, int &first, int 
 template <typename T, int V, int K>
 struct Raw { Vec<T, V> a[K], b[K]; };
 
+// No load is conditional, so that all of a row's are in flight together: a lane
+// without a unit, or a unit without a second vector, reads another one, which unpack
+// replaces by zeros.
 template <typename T, int V, int K>
 __device__ __forceinline__ void load_row(const Params &p, const T *row, int lane, Raw<T, V, K> &r) {
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int u = lane + k * p.lanes;
-    if (u < p.units) {
-      int first, second;
-      unit_at<V>(p, u, first, second);
-      r.a[k] = *reinterpret_cast<const Vec<T, V> *>(row + first);
-      if (second < p.dim) r.b[k] = *reinterpret_cast<const Vec<T, V> *>(row + second);
-      else
-#pragma unroll
-        for (int i = 0; i < V; ++i) r.b[k].e[i] = Elem<T>::put(0.f);
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) r.a[k].e[i] = r.b[k].e[i] = Elem<T>::put(0.f);
-    }
+    int first, second;
+    unit_at<V>(p, u < p.units ? u : 0, first, second);
+    r.a[k] = *reinterpret_cast<const Vec<T, V> *>(row + first);
+    r.b[k] = *reinterpret_cast<const Vec<T, V> *>(row + (second < p.dim ? second : first));
   }
 }
 
+// A lane's elements of a row as pairs of floats (two 32-bit operations an
+// instruction): element 2 i and 2 i + 1 of the unit's 2 V in pair i.
+template <int V, int K> using Lane = u64[K][V];
+
 template <typename T, int V, int K>
-__device__ __forceinline__ void unpack(const Raw<T, V, K> &r, float (&x)[K][2 * V]) {
+__device__ __forceinline__ void unpack(const Params &p, int lane, const Raw<T, V, K> &r, Lane<V, K> &x) {
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      x[k][i] = Elem<T>::get(r.a[k].e[i]);
-      x[k][V + i] = Elem<T>::get(r.b[k].e[i]);
+      const int e = 2 * i;
+      x[k][i] = tila::pk2(Elem<T>::get(e < V ? r.a[k].e[e % V] : r.b[k].e[e % V]),
+                          Elem<T>::get(e + 1 < V ? r.a[k].e[(e + 1) % V] : r.b[k].e[(e + 1) % V]));
     }
+  if (p.full) return;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int u = lane + k * p.lanes;
+    int first, second;
+    unit_at<V>(p, u, first, second);
+#pragma unroll
+    for (int e = 0; e < 2 * V; ++e)
+      if (u >= p.units || (e >= V && second >= p.dim))
+        x[k][e >> 1] = e & 1 ? tila::pk2(tila::lo2(x[k][e >> 1]), 0.f) : tila::pk2(0.f, tila::hi2(x[k][e >> 1]));
+  }
 }
 
 template <typename T, int V, int K>
-__device__ __forceinline__ void store_row(const Params &p, T *row, int lane, const float (&x)[K][2 * V]) {
+__device__ __forceinline__ void store_row(const Params &p, T *row, int lane, const Lane<V, K> &x) {
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int u = lane + k * p.lanes;
@@ -119,9 +136,9 @@ __device__ __forceinline__ void store_row(const Params &p, T *row, int lane, con
       unit_at<V>(p, u, first, second);
       Vec<T, V> a, b;
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        a.e[i] = Elem<T>::put(x[k][i]);
-        b.e[i] = Elem<T>::put(x[k][V + i]);
+      for (int e = 0; e < 2 * V; ++e) {
+        const float f = e & 1 ? tila::hi2(x[k][e >> 1]) : tila::lo2(x[k][e >> 1]);
+        (e < V ? a.e[e % V] : b.e[e % V]) = Elem<T>::put(f);
       }
       *reinterpret_cast<Vec<T, V> *>(row + first) = a;
       if (second < p.dim) *reinterpret_cast<Vec<T, V> *>(row + second) = b;
@@ -129,49 +146,68 @@ __device__ __forceinline__ void store_row(const Params &p, T *row, int lane, con
   }
 }
 
-// Turns the pairs of a row; `tab` holds (cos, sin) of the row's token, the
-// amplitude in both.
+// V consecutive floats of shared memory (V of them aligned).
+template <int V>
+__device__ __forceinline__ void floats_at(const float *p, float (&x)[V]) {
+  if constexpr (V % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      const float4 f = *reinterpret_cast<const float4 *>(p + i);
+      x[i] = f.x, x[i + 1] = f.y, x[i + 2] = f.z, x[i + 3] = f.w;
+    }
+  } else if constexpr (V == 2) {
+    const float2 f = *reinterpret_cast<const float2 *>(p);
+    x[0] = f.x, x[1] = f.y;
+  } else {
+    x[0] = p[0];
+  }
+}
+
+// Turns the pairs of a row; `tab` holds the cosines, then the sines, of the row's
+// token, the amplitude in both.
 template <int V, int K>
-__device__ __forceinline__ void turn(const Params &p, const float2 *tab, int lane, float (&x)[K][2 * V]) {
-  const int pairs = p.half / V;
+__device__ __forceinline__ void turn(const Params &p, const float *tab, int lane, Lane<V, K> &x) {
+  const int units = p.half / V;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int u = lane + k * p.lanes;
-    if (u < pairs) {
+    if (u < units) {
+      float c[V], s[V];
+      floats_at<V>(tab + u * V, c);
+      floats_at<V>(tab + p.half + u * V, s);
+      if (V == 1 || p.interleaved) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float2 cs = tab[u * V + i];
-        const int m = p.interleaved ? 1 : 0;
-        // both layouts with constant register indices
-        const float a0 = m ? x[k][2 * i] : x[k][i];
-        const float b0 = m ? x[k][2 * i + 1] : x[k][V + i];
-        const float a1 = a0 * cs.x - b0 * cs.y, b1 = b0 * cs.x + a0 * cs.y;
-        if (m) {
-          x[k][2 * i] = a1;
-          x[k][2 * i + 1] = b1;
-        } else {
-          x[k][i] = a1;
-          x[k][V + i] = b1;
+        for (int i = 0; i < V; ++i) {
+          const float a = tila::lo2(x[k][i]), b = tila::hi2(x[k][i]);
+          x[k][i] = tila::pk2(a * c[i] - b * s[i], b * c[i] + a * s[i]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+          const u64 a = x[k][i], b = x[k][V / 2 + i];
+          const u64 cc = tila::pk2(c[2 * i], c[2 * i + 1]), ss = tila::pk2(s[2 * i], s[2 * i + 1]);
+          const u64 minus = tila::pk2(-s[2 * i], -s[2 * i + 1]);
+          x[k][i] = tila::fma2(b, minus, tila::mul2(a, cc));
+          x[k][V / 2 + i] = tila::fma2(a, ss, tila::mul2(b, cc));
         }
       }
     }
   }
 }
 
-// (cos, sin) of the block's tokens, and the norm weights, into shared memory.
-template <typename T>
-__device__ __forceinline__ void fill_tables(const Params &p, i64 token0, int tokens, float2 *tab) {
+// Floats of the table: what follows it is 16-byte aligned.
+__host__ __device__ __forceinline__ int table_size(const Params &p) { return (2 * p.tokens_per_block * p.half + 3) & ~3; }
+
+__device__ __forceinline__ void fill_table(const Params &p, int b, i64 token0, int tokens, float *tab) {
   for (int i = threadIdx.x; i < tokens * p.half; i += blockDim.x) {
     const int t = i / p.half, j = i - t * p.half;
-    const i64 token = token0 + t;
-    const i64 b = token / p.tokens;
-    const i64 pos = index_at(p.positions, b * p.position_stride[0] + (token - b * p.tokens) * p.position_stride[1],
-                             p.index64 & 1);
+    const i64 pos = index_at(p.positions, b * p.position_stride[0] + (token0 + t) * p.position_stride[1], p.index64 & 1);
     double turns = static_cast<double>(pos) * p.inv_freq[j] * 0.15915494309189535;
     turns -= rint(turns);
     float s, c;
     sincospif(static_cast<float>(2.0 * turns), &s, &c);
-    tab[i] = make_float2(c * p.amplitude, s * p.amplitude * p.sign);
+    tab[2 * t * p.half + j] = c * p.amplitude;
+    tab[(2 * t + 1) * p.half + j] = s * p.amplitude * p.sign;
   }
 }
 
@@ -186,239 +222,267 @@ __device__ __forceinline__ void fill_weights(const Params &p, float *weights, in
   }
 }
 
+// Sum over the row of x * y.
 template <int V, int K>
-__device__ __forceinline__ float row_sum(const Params &p, const float (&x)[K][2 * V], const float (&y)[K][2 * V]) {
-  float s = 0.f;
+__device__ __forceinline__ float row_sum(const Params &p, const Lane<V, K> &x, const Lane<V, K> &y) {
+  u64 pair = 0;
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
-    for (int i = 0; i < 2 * V; ++i) s = fmaf(x[k][i], y[k][i], s);
+    for (int i = 0; i < V; ++i) pair = tila::fma2(x[k][i], y[k][i], pair);
+  float s = tila::lo2(pair) + tila::hi2(pair);
   for (int m = p.lanes >> 1; m > 0; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
   return s;
 }
 
-// w of the elements that a lane holds (0 behind the row's end).
+// x * w of the elements that a lane holds.
 template <int V, int K>
-__device__ __forceinline__ void times_weight(const Params &p, const float *w, float scale, int lane,
-                                             float (&x)[K][2 * V]) {
+__device__ __forceinline__ void times_weight(const Params &p, const float *w, int lane, Lane<V, K> &x) {
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int u = lane + k * p.lanes;
     if (u < p.units) {
       int first, second;
       unit_at<V>(p, u, first, second);
+      float w0[V], w1[V];
+      floats_at<V>(w + first, w0);
+      floats_at<V>(w + (second < p.dim ? second : first), w1);   // (behind the row's end: not stored)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        x[k][i] = x[k][i] * scale * w[first + i];
-        if (second < p.dim) x[k][V + i] = x[k][V + i] * scale * w[second + i];
+        const int e = 2 * i;
+        x[k][i] = tila::mul2(x[k][i], tila::pk2(e < V ? w0[e % V] : w1[e % V], e + 1 < V ? w0[(e + 1) % V] : w1[(e + 1) % V]));
       }
     }
   }
 }
 
-// Which row a job of a block is: jobs run over the heads of all tensors of one
-// token, then over the tokens.
-struct Job {
-  int tensor, head;
-  int t;          // token within the block
-  bool valid;
-};
-
-__device__ __forceinline__ Job job_at(const Params &p, int j, int jobs) {
-  Job job;
-  job.valid = j < jobs;
-  j = min(j, jobs - 1);
-  job.t = j / p.heads;
-  int h = j - job.t * p.heads;
-  job.tensor = 0;
-  if (h >= p.rows[0].heads) {
-    h -= p.rows[0].heads;
-    job.tensor = 1;
-    if (h >= p.rows[1].heads) {
-      h -= p.rows[1].heads;
-      job.tensor = 2;
-    }
-  }
-  job.head = h;
-  return job;
+template <int V, int K> __device__ __forceinline__ void times(float f, Lane<V, K> &x) {
+  const u64 ff = tila::pk2(f, f);
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[k][i] = tila::mul2(x[k][i], ff);
 }
 
+// Blocks of 256 threads that run at once on a multiprocessor.
+template <typename T, int V> struct Resident {
+  static constexpr int kForward = sizeof(T) * V == 16 ? 4 : 2;
+  static constexpr int kBackward = 2;
+};
+
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(512) rotary_rows_kernel(const __grid_constant__ Params p) {
-  extern __shared__ float2 tab[];
-  float *weights = reinterpret_cast<float *>(tab + p.tokens_per_block * p.half);
-  const i64 token0 = static_cast<i64>(blockIdx.x) * p.tokens_per_block;
-  const int tokens = static_cast<int>(min(static_cast<i64>(p.tokens_per_block), p.tokens_all - token0));
+__global__ void __launch_bounds__(256, Resident<T, V>::kForward)
+rotary_rows_kernel(const __grid_constant__ Params p) {
+  extern __shared__ __align__(16) float tab[];
+  int2 *places = reinterpret_cast<int2 *>(tab + table_size(p));       // page and row of each token's slot
+  float *weights = reinterpret_cast<float *>(places + (p.any_paged ? ((p.tokens_per_block + 1) & ~1) : 0));
+  const u32 b = p.batch == 1 ? 0 : blockIdx.x / static_cast<u32>(p.blocks_per_batch);
+  const i64 token0 = static_cast<i64>(blockIdx.x - b * static_cast<u32>(p.blocks_per_batch)) * p.tokens_per_block;
+  const int tokens = static_cast<int>(min(static_cast<i64>(p.tokens_per_block), p.tokens - token0));
   const int jobs = tokens * p.heads;
   const int groups = blockDim.x / p.lanes;
   const int lane = threadIdx.x & (p.lanes - 1);
-  const int group = threadIdx.x / p.lanes;
 
-  auto row_of = [&](const Job &job) -> const T * {
-    const Rows &r = p.rows[job.tensor];
-    const i64 token = token0 + job.t, b = token / p.tokens;
-    return static_cast<const T *>(r.src) + b * r.src_stride[0] + (token - b * p.tokens) * r.src_stride[1] +
-           job.head * r.src_stride[2];
+  // a job is a row: jobs run over the heads of all tensors of one token, then over the
+  // tokens; a group's next job is `groups` on
+  int job = threadIdx.x / p.lanes;
+  int t = min(job, jobs - 1) / p.heads, h = min(job, jobs - 1) - t * p.heads;
+  auto which = [&](int &head) {
+    head = h;
+    if (head < p.rows[0].heads) return 0;
+    head -= p.rows[0].heads;
+    if (head < p.rows[1].heads) return 1;
+    head -= p.rows[1].heads;
+    return 2;
+  };
+  auto load = [&](Raw<T, V, K> &raw) {
+    int head;
+    const Rows &r = p.rows[which(head)];
+    load_row<T, V, K>(p, static_cast<const T *>(r.src) + b * r.src_stride[0] + (token0 + t) * r.src_stride[1] +
+                             head * r.src_stride[2], lane, raw);
   };
 
-  Job job = job_at(p, group, jobs);
   Raw<T, V, K> raw;
-  load_row<T, V, K>(p, row_of(job), lane, raw);
-  fill_tables<T>(p, token0, tokens, tab);
+  load(raw);
+  fill_table(p, b, token0, tokens, tab);
   if (p.any_norm) fill_weights<T>(p, weights, p.num_rows);
+  if (p.any_paged)
+    for (int i = threadIdx.x; i < tokens; i += blockDim.x) {
+      const i64 slot = index_at(p.slots, (token0 + i) * p.slot_stride, p.index64 & 2);
+      if (slot >= p.num_slots) tila::report_error(p.err, kErrIndex, static_cast<u32>(token0 + i));
+      const i64 page = slot / p.page_size;
+      places[i] = slot < 0 || slot >= p.num_slots ? make_int2(-1, 0)
+                                                  : make_int2(static_cast<int>(page), static_cast<int>(slot - page * p.page_size));
+    }
   __syncthreads();
 
   // every warp runs the same number of times: the norm's sum is over its lanes
   for (int first = 0; first < jobs; first += groups) {
-    const Job next = job_at(p, group + first + groups, jobs);
-    Raw<T, V, K> ahead;
-    if (first + groups < jobs) load_row<T, V, K>(p, row_of(next), lane, ahead);
-    float x[K][2 * V];
-    unpack<T, V, K>(raw, x);
-    const Rows &r = p.rows[job.tensor];
-    if (p.any_norm) {
-      const float ss = row_sum<V, K>(p, x, x);
-      if (r.flags & TILA_ROWS_NORM)
-        times_weight<V, K>(p, weights + job.tensor * p.dim, rsqrtf(ss * p.inv_dim + p.eps), lane, x);
-    }
-    if (r.flags & TILA_ROWS_ROTATE) turn<V, K>(p, tab + job.t * p.half, lane, x);
-    if (job.valid) {
-      const i64 token = token0 + job.t;
-      T *dst = static_cast<T *>(r.dst) + job.head * r.dst_stride[2];
-      if (r.flags & TILA_ROWS_PAGED) {
-        const i64 slot = index_at(p.slots, token * p.slot_stride, p.index64 & 2);
-        if (slot >= p.num_slots) {
-          tila::report_error(p.err, kErrIndex, static_cast<u32>(token));
-        } else if (slot >= 0) {
-          const i64 page = slot / p.page_size;
-          store_row<T, V, K>(p, dst + page * r.dst_stride[0] + (slot - page * p.page_size) * r.dst_stride[1], lane, x);
-        }
-      } else {
-        const i64 b = token / p.tokens;
-        store_row<T, V, K>(p, dst + b * r.dst_stride[0] + (token - b * p.tokens) * r.dst_stride[1], lane, x);
+    const bool valid = job < jobs;
+    int head;
+    const int tensor = which(head), at = t;
+    Lane<V, K> x;
+    unpack<T, V, K>(p, lane, raw, x);
+    job += groups;
+    if (job < jobs) {                          // (else the same row again, unused)
+      t += p.step_tokens;
+      h += p.step_heads;
+      if (h >= p.heads) {
+        h -= p.heads;
+        ++t;
       }
     }
-    job = next;
-    raw = ahead;
+    if (first + groups < jobs) load(raw);
+    const Rows &r = p.rows[tensor];
+    if (p.any_norm) {
+      const float ss = row_sum<V, K>(p, x, x);
+      if (r.flags & TILA_ROWS_NORM) {
+        times<V, K>(rsqrtf(ss * p.inv_dim + p.eps), x);
+        times_weight<V, K>(p, weights + tensor * p.dim, lane, x);
+      }
+    }
+    if (!valid) continue;
+    if (r.flags & TILA_ROWS_ROTATE) turn<V, K>(p, tab + 2 * at * p.half, lane, x);
+    T *dst = static_cast<T *>(r.dst) + head * r.dst_stride[2];
+    if (r.flags & TILA_ROWS_PAGED) {
+      const int2 place = places[at];
+      if (place.x >= 0)
+        store_row<T, V, K>(p, dst + place.x * r.dst_stride[0] + place.y * r.dst_stride[1], lane, x);
+    } else {
+      store_row<T, V, K>(p, dst + b * r.dst_stride[0] + (token0 + at) * r.dst_stride[1], lane, x);
+    }
   }
 }
 
 // Gradients of y = a R (w * x * r), r = 1 / sqrt(mean(x^2) + eps), xh = x * r:
 //     g = a R^T dy;   dx = r * (w g - xh * mean(w g xh));   dw = sum over rows of g * xh
-// One pass over x and dy.  The blocks are as many as fit the GPU and walk the
-// tokens, so that each sums its rows' dw in registers and leaves one partial sum;
-// the partial sums are added in a fixed order by the kernel below (no atomics:
-// the same call gives the same bits).
-template <typename T, int V, int K, int R>
-__device__ __forceinline__ void backward_tensor(const Params &p, i64 token0, int tokens, const float2 *tab,
-                                                const float *w, float (&sum)[K][2 * V]) {
-  const Rows &r = p.rows[R];
-  const int jobs = tokens * r.heads;
+// One pass over x and dy.  The blocks are as many as run at once, each with an
+// equal share of the tokens, so that each sums its rows' dw in registers (first of the
+// queries, then of the keys) and leaves one partial sum; the partial sums are added in a
+// fixed order by the kernel below (no atomics: the same call gives the same bits).
+template <typename T, int V, int K>
+__global__ void __launch_bounds__(256, Resident<T, V>::kBackward)
+rotary_norm_backward_kernel(const __grid_constant__ Params p) {
+  extern __shared__ __align__(16) float tab[];
+  float *weights = reinterpret_cast<float *>(tab + table_size(p));
+  float *scratch = weights + 2 * p.dim;
   const int groups = blockDim.x / p.lanes;
-  const int lane = threadIdx.x & (p.lanes - 1);
-  const int group = threadIdx.x / p.lanes;
-  for (int first = 0; first < jobs; first += groups) {
-    const bool valid = first + group < jobs;
-    const int j = valid ? first + group : 0;
-    const int t = j / r.heads, h = j - t * r.heads;
-    const i64 token = token0 + t, b = token / p.tokens, at = token - b * p.tokens;
-    Raw<T, V, K> rx, rg;
-    load_row<T, V, K>(p, static_cast<const T *>(r.src) + b * r.src_stride[0] + at * r.src_stride[1] +
-                             h * r.src_stride[2], lane, rx);
-    load_row<T, V, K>(p, static_cast<const T *>(r.grad) + b * r.grad_stride[0] + at * r.grad_stride[1] +
-                             h * r.grad_stride[2], lane, rg);
-    float x[K][2 * V], g[K][2 * V];
-    unpack<T, V, K>(rx, x);
-    unpack<T, V, K>(rg, g);
-    if (r.flags & TILA_ROWS_ROTATE) turn<V, K>(p, tab + t * p.half, lane, g);
-    const float rms = rsqrtf(row_sum<V, K>(p, x, x) * p.inv_dim + p.eps);
+  const int lane = threadIdx.x & (p.lanes - 1), group = threadIdx.x / p.lanes;
+  tila::grid_dep_release();
+  fill_weights<T>(p, weights, p.num_rows);
+  const i64 all = p.batch * p.tokens;
+  const i64 begin = all * blockIdx.x / gridDim.x, end = all * (blockIdx.x + 1) / gridDim.x;
+  for (int tensor = 0; tensor < p.num_rows; ++tensor) {
+    const Rows &r = p.rows[tensor];
+    Lane<V, K> sum;
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int i = 0; i < 2 * V; ++i) {
-        x[k][i] *= rms;                                         // xh
-        if (valid) sum[k][i] = fmaf(g[k][i], x[k][i], sum[k][i]);
+      for (int i = 0; i < V; ++i) sum[k][i] = 0;
+    // pieces of the share that lie in one batch entry and fit the table
+    for (i64 from = begin; from < end;) {
+      const int b = static_cast<int>(from / p.tokens);
+      const i64 token0 = from - b * p.tokens;
+      const int tokens = static_cast<int>(min(min(static_cast<i64>(p.tokens_per_block), end - from), p.tokens - token0));
+      const int jobs = tokens * r.heads;
+      if (jobs == 0) break;
+      int job = group, t = min(job, jobs - 1) / r.heads, h = min(job, jobs - 1) - t * r.heads;
+      const int dt = groups / r.heads, dh = groups - dt * r.heads;
+      Raw<T, V, K> rx, rg;
+      auto load = [&] {
+        load_row<T, V, K>(p, static_cast<const T *>(r.src) + b * r.src_stride[0] + (token0 + t) * r.src_stride[1] +
+                                 h * r.src_stride[2], lane, rx);
+        load_row<T, V, K>(p, static_cast<const T *>(r.grad) + b * r.grad_stride[0] + (token0 + t) * r.grad_stride[1] +
+                                 h * r.grad_stride[2], lane, rg);
+      };
+      load();
+      __syncthreads();
+      fill_table(p, b, token0, tokens, tab);
+      __syncthreads();
+      for (int first = 0; first < jobs; first += groups) {
+        const bool valid = job < jobs;
+        const int at = t, head = h;
+        Lane<V, K> x, g;
+        unpack<T, V, K>(p, lane, rx, x);
+        unpack<T, V, K>(p, lane, rg, g);
+        job += groups;
+        if (job < jobs) {                      // (else the same row again, unused)
+          t += dt;
+          h += dh;
+          if (h >= r.heads) {
+            h -= r.heads;
+            ++t;
+          }
+        }
+        if (first + groups < jobs) load();
+        if (valid && (r.flags & TILA_ROWS_ROTATE)) turn<V, K>(p, tab + 2 * at * p.half, lane, g);
+        const float rms = rsqrtf(row_sum<V, K>(p, x, x) * p.inv_dim + p.eps);
+        times<V, K>(rms, x);                                        // xh
+        if (valid)
+#pragma unroll
+          for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) sum[k][i] = tila::fma2(g[k][i], x[k][i], sum[k][i]);
+        times_weight<V, K>(p, weights + tensor * p.dim, lane, g);   // w g
+        const float mean = row_sum<V, K>(p, g, x) * p.inv_dim;
+        const u64 minus = tila::pk2(-mean, -mean);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int i = 0; i < V; ++i) x[k][i] = tila::fma2(x[k][i], minus, g[k][i]);
+        times<V, K>(rms, x);
+        if (valid)
+          store_row<T, V, K>(p, static_cast<T *>(r.dst) + b * r.dst_stride[0] + (token0 + at) * r.dst_stride[1] +
+                                    head * r.dst_stride[2], lane, x);
       }
-    times_weight<V, K>(p, w, 1.f, lane, g);                     // w g
-    const float mean = row_sum<V, K>(p, g, x) * p.inv_dim;
+      from += tokens;
+    }
+    // the groups' sums, then this block's partial sum
+    __syncthreads();
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int k = 0; k < K; ++k) {
+      const int u = lane + k * p.lanes;
+      if (u < p.units) {
+        int first, second;
+        unit_at<V>(p, u, first, second);
 #pragma unroll
-      for (int i = 0; i < 2 * V; ++i) x[k][i] = rms * (g[k][i] - x[k][i] * mean);
-    if (valid)
-      store_row<T, V, K>(p, static_cast<T *>(r.dst) + b * r.dst_stride[0] + at * r.dst_stride[1] +
-                                h * r.dst_stride[2], lane, x);
-  }
-}
-
-// Adds the groups' sums of a block and writes them as partial sum (block, R).
-template <int V, int K>
-__device__ __forceinline__ void block_sum(const Params &p, float *scratch, const float (&sum)[K][2 * V], int tensor) {
-  const int groups = blockDim.x / p.lanes;
-  const int lane = threadIdx.x & (p.lanes - 1);
-  const int group = threadIdx.x / p.lanes;
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int u = lane + k * p.lanes;
-    if (u < p.units) {
-      int first, second;
-      unit_at<V>(p, u, first, second);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        scratch[group * p.dim + first + i] = sum[k][i];
-        if (second < p.dim) scratch[group * p.dim + second + i] = sum[k][V + i];
+        for (int i = 0; i < V; ++i) {
+          const int e = V + i;
+          scratch[group * p.dim + first + i] = i & 1 ? tila::hi2(sum[k][i >> 1]) : tila::lo2(sum[k][i >> 1]);
+          if (second < p.dim)
+            scratch[group * p.dim + second + i] = e & 1 ? tila::hi2(sum[k][e >> 1]) : tila::lo2(sum[k][e >> 1]);
+        }
       }
     }
-  }
-  __syncthreads();
-  for (int j = threadIdx.x; j < p.dim; j += blockDim.x) {
-    float s = 0.f;
-    for (int g = 0; g < groups; ++g) s += scratch[g * p.dim + j];
-    p.partial[(static_cast<i64>(blockIdx.x) * 2 + tensor) * p.dim + j] = s;
-  }
-}
-
-template <typename T, int V, int K>
-__global__ void __launch_bounds__(256) rotary_norm_backward_kernel(const __grid_constant__ Params p) {
-  extern __shared__ float2 tab[];
-  float *weights = reinterpret_cast<float *>(tab + p.tokens_per_block * p.half);
-  float *scratch = weights + 2 * p.dim;
-  float sum0[K][2 * V], sum1[K][2 * V];
-#pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int i = 0; i < 2 * V; ++i) sum0[k][i] = sum1[k][i] = 0.f;
-  fill_weights<T>(p, weights, p.num_rows);
-  for (i64 token0 = static_cast<i64>(blockIdx.x) * p.tokens_per_block; token0 < p.tokens_all;
-       token0 += static_cast<i64>(gridDim.x) * p.tokens_per_block) {
-    const int tokens = static_cast<int>(min(static_cast<i64>(p.tokens_per_block), p.tokens_all - token0));
     __syncthreads();
-    fill_tables<T>(p, token0, tokens, tab);
-    __syncthreads();
-    backward_tensor<T, V, K, 0>(p, token0, tokens, tab, weights, sum0);
-    if (p.num_rows > 1) backward_tensor<T, V, K, 1>(p, token0, tokens, tab, weights + p.dim, sum1);
+    for (int j = threadIdx.x; j < p.dim; j += blockDim.x) {
+      float s = 0.f;
+      for (int g = 0; g < groups; ++g) s += scratch[g * p.dim + j];
+      p.partial[(static_cast<i64>(blockIdx.x) * 2 + tensor) * p.dim + j] = s;
+    }
   }
-  block_sum<V, K>(p, scratch, sum0, 0);
-  if (p.num_rows > 1) block_sum<V, K>(p, scratch, sum1, 1);
 }
 
 // weight_grad[tensor][j] = sum over blocks of partial[block][tensor][j]: 32
-// columns a block, 8 threads a column, each over every eighth block.
-__global__ void __launch_bounds__(256) weight_grad_kernel(const float *partial, int blocks, int dim, float *g0,
-                                                          float *g1) {
-  __shared__ float s[8][33];
+// columns a block, 32 threads a column, each over every 32nd block.
+__global__ void __launch_bounds__(1024) weight_grad_kernel(const float *partial, int blocks, int dim, float *g0,
+                                                           float *g1) {
+  __shared__ float s[32][33];
   const int c = threadIdx.x & 31, part = threadIdx.x >> 5;
-  const int j = blockIdx.x * 32 + c, tensor = blockIdx.y;
+  const int tensor = blockIdx.x & 1, j = (blockIdx.x >> 1) * 32 + c;
+  tila::grid_dep_wait();
   float a = 0.f;
   if (j < dim)
-    for (int b = part; b < blocks; b += 8) a += partial[(static_cast<i64>(b) * 2 + tensor) * dim + j];
+#pragma unroll 4
+    for (int b = part; b < blocks; b += 32) a += partial[(static_cast<i64>(b) * 2 + tensor) * dim + j];
   s[part][c] = a;
   __syncthreads();
-  if (part == 0 && j < dim) {
-    for (int i = 1; i < 8; ++i) a += s[i][c];
-    (tensor == 0 ? g0 : g1)[j] = a;
-  }
+  // column `part` by one warp, its 32 sums pairwise
+  a = s[c][part];
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) a += __shfl_xor_sync(0xffffffffu, a, x);
+  const int column = (blockIdx.x >> 1) * 32 + part;
+  if (c == 0 && column < dim && (tensor == 0 ? g0 : g1) != nullptr) (tensor == 0 ? g0 : g1)[column] = a;
 }
 
 // ---------------------------------------------------------------------------
@@ -451,7 +515,7 @@ int check(const tila_rotary_args *a, bool backward, char *log, size_t cap) {
   if (a == nullptr || a->size != sizeof(tila_rotary_args) || a->reserved != 0)
     return fail(TILA_ERR_ARGUMENT, log, cap, "%s: args.size is not that of this library's structure", who);
   if (a->dtype < TILA_F32 || a->dtype > TILA_BF16) return fail(TILA_ERR_ARGUMENT, log, cap, "%s: unknown dtype", who);
-  if (a->batch < 0 || a->tokens < 0 || a->dim < 1 || a->dim > 512 || a->rotary < 0 || a->rotary > a->dim ||
+  if (a->batch < 0 || a->tokens < 0 || a->batch > 0x7fffffff || a->dim < 1 || a->dim > 512 || a->rotary < 0 || a->rotary > a->dim ||
       a->rotary % 2 != 0)
     return fail(TILA_ERR_ARGUMENT, log, cap, "%s: dim must be 1 to 512 and rotary an even number up to dim", who);
   if (a->num_rows < 1 || a->num_rows > (backward ? 2 : 3))
@@ -501,8 +565,19 @@ Params make_params(const tila_rotary_args &a, bool backward, int v) {
     rotates = rotates || (r.flags & TILA_ROWS_ROTATE);
   }
   p.num_rows = a.num_rows;
-  p.tokens_all = a.batch * a.tokens;
+  p.batch = static_cast<int>(a.batch);
   p.tokens = a.tokens;
+  // batch entries that lie behind one another are one long entry
+  bool flat = a.batch > 1 && (a.positions == 0 || a.position_stride[0] == a.tokens * a.position_stride[1]);
+  for (int i = 0; flat && i < a.num_rows; ++i) {
+    const tila_op_rows &r = a.rows[i];
+    flat = r.src_stride[0] == a.tokens * r.src_stride[1] && r.dst_stride[0] == a.tokens * r.dst_stride[1] &&
+           (!backward || r.grad_stride[0] == a.tokens * r.grad_stride[1]);
+  }
+  if (flat) {
+    p.tokens *= p.batch;
+    p.batch = 1;
+  }
   p.dim = a.dim;
   p.half = rotates ? a.rotary / 2 : 0;
   p.interleaved = a.interleaved != 0;
@@ -526,34 +601,45 @@ Params make_params(const tila_rotary_args &a, bool backward, int v) {
   return p;
 }
 
-// Tokens of a block: enough rows for about 256 threads.
-int tokens_per_block(const Params &p) {
-  const int threads = std::max(1, p.heads) * p.lanes;
-  return std::max(1, std::min({32, 256 / threads, 4096 / std::max(1, p.half)}));
+// Tokens of a block: rows for 256 threads at least; where there are more than
+// `resident` blocks a multiprocessor could take, as many as fill whole waves.
+int tokens_per_block(const Params &p, int resident) {
+  const i64 most = std::min(32, 2048 / std::max(1, p.half));
+  const i64 rows = 256 / std::max(1, p.heads * p.lanes);
+  const i64 wave = static_cast<i64>(resident) * kSms, all = p.batch * p.tokens;
+  const i64 waves = (all + wave * most - 1) / (wave * most);
+  return static_cast<int>(std::max<i64>(1, std::min<i64>(most, std::max(rows, (all + wave * waves - 1) / (wave * waves)))));
 }
 
 int backward_blocks(const Params &p) {
-  // 4 blocks of 256 threads an SM: two rows of 64 bytes in flight per thread
-  const i64 most = (p.tokens_all + p.tokens_per_block - 1) / p.tokens_per_block;
-  return static_cast<int>(std::min<i64>(most, 4 * kSms));
+  return static_cast<int>(std::min<i64>(p.batch * p.tokens, 2 * kSms));   // as many as run at once (Resident)
 }
 
 template <typename T, int V, int K>
-int launch_forward(const Params &p, cudaStream_t stream, char *log, size_t cap) {
-  const i64 blocks = (p.tokens_all + p.tokens_per_block - 1) / p.tokens_per_block;
+int launch_forward(Params p, cudaStream_t stream, char *log, size_t cap) {
+  p.full = p.dim % (2 * V) == 0 && p.units == p.lanes * K;
+  p.tokens_per_block = tokens_per_block(p, Resident<T, V>::kForward);
+  p.blocks_per_batch = (p.tokens + p.tokens_per_block - 1) / p.tokens_per_block;
+  const i64 blocks = p.blocks_per_batch * p.batch;
   if (blocks > 0x7fffffff) return fail(TILA_ERR_ARGUMENT, log, cap, "tila_rotary_rows: too many tokens for one launch");
   const i64 lanes = static_cast<i64>(p.tokens_per_block) * p.heads * p.lanes;
-  const int threads = static_cast<int>(std::min<i64>(512, std::max<i64>(32, (lanes + 31) / 32 * 32)));
-  const size_t smem = sizeof(float2) * p.tokens_per_block * p.half + (p.any_norm ? 3 * sizeof(float) * p.dim : 0);
+  const int threads = static_cast<int>(std::min<i64>(256, (lanes + 31) / 32 * 32));
+  p.step_tokens = threads / p.lanes / p.heads;
+  p.step_heads = threads / p.lanes - p.step_tokens * p.heads;
+  const size_t smem = sizeof(float) * table_size(p) +
+                      (p.any_paged ? sizeof(int2) * ((p.tokens_per_block + 1) & ~1) : 0) +
+                      (p.any_norm ? 3 * sizeof(float) * p.dim : 0) + 16;
   rotary_rows_kernel<T, V, K><<<static_cast<unsigned>(blocks), threads, smem, stream>>>(p);
   return launch_status(cudaGetLastError(), "tila_rotary_rows", log, cap);
 }
 
 template <typename T, int V, int K>
-int launch_backward(const Params &p, const tila_rotary_args &a, cudaStream_t stream, char *log, size_t cap) {
+int launch_backward(Params p, const tila_rotary_args &a, cudaStream_t stream, char *log, size_t cap) {
+  p.full = p.dim % (2 * V) == 0 && p.units == p.lanes * K;
+  p.tokens_per_block = std::min(32, 2048 / std::max(1, p.half));
   const int blocks = backward_blocks(p);
   const int groups = kBackwardThreads / p.lanes;
-  const size_t smem = sizeof(float2) * p.tokens_per_block * p.half + sizeof(float) * p.dim * (2 + groups);
+  const size_t smem = sizeof(float) * table_size(p) + sizeof(float) * p.dim * (2 + groups) + 16;
   cudaError_t e = cudaSuccess;
   if (smem > 48 * 1024)
     e = cudaFuncSetAttribute(rotary_norm_backward_kernel<T, V, K>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -561,12 +647,10 @@ int launch_backward(const Params &p, const tila_rotary_args &a, cudaStream_t str
   if (e != cudaSuccess) return launch_status(e, "tila_rotary_norm_backward", log, cap);
   rotary_norm_backward_kernel<T, V, K><<<blocks, kBackwardThreads, smem, stream>>>(p);
   e = cudaGetLastError();
-  if (e == cudaSuccess) {
-    weight_grad_kernel<<<dim3((p.dim + 31) / 32, p.num_rows), 256, 0, stream>>>(
-        p.partial, blocks, p.dim, reinterpret_cast<float *>(a.weight_grad[0]),
-        reinterpret_cast<float *>(a.weight_grad[1]));
-    e = cudaGetLastError();
-  }
+  if (e == cudaSuccess)
+    e = launch_kernel(weight_grad_kernel, (p.dim + 31) / 32 * 2, 1024, 0, stream, true,
+                      static_cast<const float *>(p.partial), blocks, p.dim, reinterpret_cast<float *>(a.weight_grad[0]),
+                      p.num_rows > 1 ? reinterpret_cast<float *>(a.weight_grad[1]) : static_cast<float *>(nullptr));
   return launch_status(e, "tila_rotary_norm_backward", log, cap);
 }
 
@@ -593,14 +677,13 @@ int run(const tila_rotary_args *a, bool backward, char *log, size_t cap) {
   const int v = vector_width(*a, backward);
   Params p = make_params(*a, backward, v);
   const cudaStream_t stream = reinterpret_cast<cudaStream_t>(a->stream);
-  if (p.tokens_all == 0 || p.heads == 0) {
+  if (p.batch * p.tokens == 0 || p.heads == 0) {
     // no row: nothing to write, but the weights' gradients are zero
     for (int i = 0; backward && i < a->num_rows; ++i)
       if (cudaMemsetAsync(reinterpret_cast<void *>(a->weight_grad[i]), 0, sizeof(float) * a->dim, stream) != cudaSuccess)
         return fail(TILA_ERR_DRIVER, log, cap, "tila_rotary_norm_backward: clearing a weight gradient failed");
     return TILA_OK;
   }
-  p.tokens_per_block = tokens_per_block(p);
   if (backward) {
     if (a->workspace == 0 || a->workspace % 16 != 0 || a->workspace_bytes < tila_rotary_workspace(a))
       return fail(TILA_ERR_ARGUMENT, log, cap, "tila_rotary_norm_backward: workspace is too small or not 16-byte aligned");
@@ -624,7 +707,6 @@ extern "C" int tila_rotary_norm_backward(const tila_rotary_args *args, char *log
 extern "C" uint64_t tila_rotary_workspace(const tila_rotary_args *a) {
   if (check(a, true, nullptr, 0) != TILA_OK) return 0;
   Params p = make_params(*a, true, vector_width(*a, true));
-  if (p.tokens_all == 0 || p.heads == 0) return 0;
-  p.tokens_per_block = tokens_per_block(p);
+  if (p.batch * p.tokens == 0 || p.heads == 0) return 0;
   return static_cast<uint64_t>(backward_blocks(p)) * 2 * a->dim * sizeof(float);
 }
