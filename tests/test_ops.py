@@ -1,7 +1,9 @@
 """The operators' host side on the CPU: frequencies, and the calls they refuse
 (nothing is launched: every refusal comes before that)."""
 
+import ctypes
 import math
+import struct
 
 import pytest
 import torch
@@ -9,14 +11,9 @@ import torch
 from tila_b200 import native, ops
 
 
-class OnDevice(torch.Tensor):
-    """A CPU tensor that says it is a CUDA tensor, so that the checks behind
-    that one can be reached without a GPU."""
-    is_cuda = property(lambda self: True)
-
-
 def dev(*shape, dtype=torch.float32):
-    return torch.zeros(*shape, dtype=dtype).as_subclass(OnDevice)
+    """What stands for a CUDA tensor: that it is none is the last check."""
+    return torch.zeros(*shape, dtype=dtype)
 
 
 def test_frequencies():
@@ -46,12 +43,12 @@ def test_frequencies_refuse(kwargs):
         ops.rotary_frequencies(device="cpu", **kwargs)
 
 
-INV = torch.ones(32, dtype=torch.float64).as_subclass(OnDevice)
-POS = torch.arange(6).as_subclass(OnDevice)
+INV = torch.ones(32, dtype=torch.float64)
+POS = torch.arange(6)
 
 
 @pytest.mark.parametrize("change,text", [
-    (dict(x=torch.zeros(6, 2, 64)), "CUDA"),
+    (dict(), "x must be a CUDA|grad must be a CUDA"),
     (dict(x=dev(6, 2, 64, dtype=torch.float64)), "float32"),
     (dict(x=dev(6, 64)), "tokens, heads, dim"),
     (dict(x=dev(6, 2, 513)), "512"),
@@ -59,12 +56,12 @@ POS = torch.arange(6).as_subclass(OnDevice)
     (dict(x=dev(6, 2, 62)), "rotates 64"),
     (dict(positions=POS[:5]), "one position per token"),
     (dict(positions=POS.float()), "int32 or int64"),
-    (dict(positions=torch.arange(6)), "CUDA"),
-    (dict(inv_freq=INV.float()), "float64"),
+    (dict(positions=torch.zeros(6, dtype=torch.int64, device="meta")), "other tensors on cpu"),
+    (dict(inv_freq=INV.float()), "Double"),
     (dict(inv_freq=dev(64, dtype=torch.float64)[::2]), "contiguous"),
     (dict(layout="other"), "layout"),
     (dict(out=dev(6, 2, 32)), "shape"),
-    (dict(out=dev(6, 2, 64, dtype=torch.float16)), "float32"),
+    (dict(out=dev(6, 2, 64, dtype=torch.float16)), "Float, not Half"),
     (dict(out=dev(6, 1, 64).expand(6, 2, 64)), "share memory"),
     (dict(out=dev(6, 2, 128)[..., ::2]), "contiguous"),
 ])
@@ -93,22 +90,25 @@ def test_overlap_rules():
     shares memory is refused."""
     qkv = dev(6, 5, 64)
     q, k = qkv[:, :3], qkv[:, 3:]
-    ops._apart("t", "a", q, "b", k)
-    ops._apart("t", "a", k, "b", q)
-    ops._apart("t", "a", q, "b", q, same=True)
+    def apart(a, b, same=False):
+        ops._ops.check_apart("t", "a", a, "b", b, same)
+    apart(q, k)
+    apart(k, q)
+    apart(q, q, same=True)
     both = dev(4, 2, 8, 3, 64)
-    ops._apart("t", "a", both[:, 0], "b", both[:, 1])
+    apart(both[:, 0], both[:, 1])
     batch = dev(2, 6, 5, 64)
-    ops._apart("t", "a", batch[:, :, :3], "b", batch[:, :, 3:])
+    apart(batch[:, :, :3], batch[:, :, 3:])
     for a, b in ((q, q), (qkv[:, :3], qkv[:, 2:]), (q, qkv[:, :2]), (both[:, 0], both[:, 0]), (qkv, q)):
         with pytest.raises(ValueError, match="overlaps"):
-            ops._apart("t", "a", a, "b", b)
+            apart(a, b)
 
 
 NORM = dict(q=dev(6, 4, 64), k=dev(6, 2, 64), q_weight=dev(64), k_weight=dev(64))
 
 
 @pytest.mark.parametrize("change,text", [
+    (dict(), "q must be a CUDA"),
     (dict(k=dev(5, 2, 64)), "same tokens"),
     (dict(k=dev(6, 2, 32)), "same tokens"),
     (dict(k=dev(6, 2, 64, dtype=torch.float16)), "one dtype"),
@@ -128,20 +128,21 @@ def test_norm_rotate_refuses(change, text):
 def test_norm_rotate_backward_refuses():
     a = list(NORM.values())
     for grads, kwargs, text in (((dev(6, 4, 32), dev(6, 2, 64)), {}, "shape"),
-                                ((dev(6, 4, 64), dev(6, 2, 64, dtype=torch.float16)), {}, "float32"),
+                                ((dev(6, 4, 64), dev(6, 2, 64, dtype=torch.float16)), {}, "Float, not Half"),
                                 ((dev(6, 4, 64), dev(6, 2, 64)), dict(dk=NORM["q"][:, :2]), "overlaps")):
         with pytest.raises(ValueError, match=text):
             ops.norm_rotate_backward(*grads, *a, POS, INV, **kwargs)
 
 
 APPEND = dict(k=dev(6, 2, 64), v=dev(6, 2, 64), k_cache=dev(3, 4, 2, 64), v_cache=dev(3, 4, 2, 64),
-              slots=torch.arange(6).as_subclass(OnDevice))
+              slots=torch.arange(6))
 
 
 @pytest.mark.parametrize("change,text", [
+    (dict(), "k must be a CUDA"),
     (dict(k=dev(1, 6, 2, 64)), "tokens, kv_heads"),
     (dict(v=dev(6, 2, 32)), "shape of k"),
-    (dict(v=dev(6, 2, 64, dtype=torch.float16)), "float32"),
+    (dict(v=dev(6, 2, 64, dtype=torch.float16)), "Float, not Half"),
     (dict(k_cache=dev(3, 4, 1, 64)), "k_cache must be"),
     (dict(v_cache=dev(3, 5, 2, 64)), "v_cache must be"),
     (dict(v_cache=dev(12, 2, 64)), "4 dimensions"),
@@ -163,15 +164,34 @@ def test_append_refuses(change, text):
         ops.append_paged(*first, **args)
 
 
-def rotary_args(rows=1, flags=native.ROWS_ROTATE, **change):
+# tila_op_rows, tila_rotary_args without its rows, tila_attend_args (include/tila_b200.h)
+ROWS, HEAD, ATTEND_ARGS = struct.Struct("=4Q9qiI"), struct.Struct("=Iiqq4iffQ2qQQqq4i6Q"), struct.Struct("=Iiq7if2q5Q4q6qQq7Q")
+ROTARY_BYTES = HEAD.size + 3 * ROWS.size
+FLAG_ROTATE, FLAG_NORM, FLAG_PAGED = 1, 2, 4
+
+
+def refused(entry, args):
+    """The C entry's status is that of a bad argument, and the log says why."""
+    log = ctypes.create_string_buffer(512)
+    status = getattr(native.library(), entry)(args, log, ctypes.c_size_t(len(log)))
+    assert status == native.TILA_ERR_ARGUMENT and log.value
+
+
+def workspace(entry, args):
+    f = getattr(native.library(), entry)
+    f.restype = ctypes.c_uint64
+    return f(args)
+
+
+def rotary_args(rows=1, flags=FLAG_ROTATE, **change):
     """tila_rotary_args with addresses that nothing reads (the call is refused)."""
     names = ("size", "dtype", "batch", "tokens", "dim", "rotary", "interleaved", "inverse", "amplitude", "eps",
              "positions", "step_b", "step_t", "inv_freq", "slots", "slot_step", "num_slots", "page", "index64",
              "num_rows", "reserved", "err", "stream", "workspace", "workspace_bytes", "dw0", "dw1")
-    head = dict(zip(names, (native.ROTARY_BYTES, 0, 1, 4, 64, 64, 0, 0, 1.0, 0.0, 4096, 0, 1, 4096, 0, 0, 0, 0, 1, rows, 0,
+    head = dict(zip(names, (ROTARY_BYTES, 0, 1, 4, 64, 64, 0, 0, 1.0, 0.0, 4096, 0, 1, 4096, 0, 0, 0, 0, 1, rows, 0,
                             0, 0, 0, 0, 0, 0))) | change
-    row = native.ROWS.pack(4096, 4096, 0, 0, 0, 128, 64, 0, 128, 64, 0, 0, 0, 2, flags)
-    return native.ROTARY_HEAD.pack(*(head[n] for n in names)) + row * rows + native.NO_ROWS * (3 - rows)
+    row = ROWS.pack(4096, 4096, 0, 0, 0, 128, 64, 0, 128, 64, 0, 0, 0, 2, flags)
+    return HEAD.pack(*(head[n] for n in names)) + row * rows + bytes(ROWS.size) * (3 - rows)
 
 
 @pytest.mark.parametrize("entry,args", [
@@ -183,19 +203,17 @@ def rotary_args(rows=1, flags=native.ROWS_ROTATE, **change):
     ("tila_rotary_rows", rotary_args(rotary=63)),
     ("tila_rotary_rows", rotary_args(positions=0)),
     ("tila_rotary_rows", rotary_args(num_rows=4)),
-    ("tila_rotary_rows", rotary_args(flags=native.ROWS_NORM)),
-    ("tila_rotary_rows", rotary_args(flags=native.ROWS_PAGED)),
+    ("tila_rotary_rows", rotary_args(flags=FLAG_NORM)),
+    ("tila_rotary_rows", rotary_args(flags=FLAG_PAGED)),
     ("tila_rotary_norm_backward", rotary_args()),
 ])
 def test_c_entry_refuses(entry, args):
-    with pytest.raises(native.NativeError) as exc:
-        native.call_op(entry, args)
-    assert exc.value.status == native.TILA_ERR_ARGUMENT and exc.value.log
-    assert native.rotary_workspace(args) == 0
+    refused(entry, args)
+    assert workspace("tila_rotary_workspace", args) == 0
 
 
 def ints(*shape):
-    return torch.zeros(*shape, dtype=torch.int32).as_subclass(OnDevice)
+    return torch.zeros(*shape, dtype=torch.int32)
 
 
 H = torch.float16
@@ -204,7 +222,7 @@ ATTEND = dict(q=dev(3, 4, 64, dtype=H), k_cache=dev(5, 8, 2, 64, dtype=H), v_cac
 
 
 @pytest.mark.parametrize("change,text", [
-    (dict(q=torch.zeros(3, 4, 64)), "CUDA"),
+    (dict(), "q must be a CUDA"),
     (dict(q=dev(3, 4, 64)), "float16 or bfloat16"),
     (dict(q=dev(3, 4, 60, dtype=H)), "multiple of 8"),
     (dict(q=dev(3, 4, 264, dtype=H)), "up to 256"),
@@ -213,9 +231,9 @@ ATTEND = dict(q=dev(3, 4, 64, dtype=H), k_cache=dev(5, 8, 2, 64, dtype=H), v_cac
     (dict(q=dev(4, 4, 64, dtype=H)), "one row per sequence"),
     (dict(k_cache=dev(5, 8, 2, 32, dtype=H)), "both alike"),
     (dict(v_cache=dev(5, 9, 2, 64, dtype=H)), "both alike"),
-    (dict(v_cache=dev(5, 8, 2, 64, dtype=torch.bfloat16)), "float16"),
+    (dict(v_cache=dev(5, 8, 2, 64, dtype=torch.bfloat16)), "Half"),
     (dict(k_cache=dev(5, 8, 2, 68, dtype=H)[..., 4:]), "16-byte"),
-    (dict(page_table=ints(3, 2).long()), "int32"),
+    (dict(page_table=ints(3, 2).long()), "Int, not Long"),
     (dict(page_table=ints(3)), "2 dimensions"),
     (dict(page_table=ints(3, 4)[:, ::2]), "contiguous"),
     (dict(lengths=ints(2)), "3 entries"),
@@ -243,9 +261,9 @@ def attend_args(**change):
              "scale", "num_pages", "prefix_length", "q", "k_cache", "v_cache", "out", "lse", "qt", "qh", "ot", "oh",
              "kp", "kr", "kh", "vp", "vr", "vh", "page_table", "table_stride", "lengths", "query_offsets",
              "prefix_pages", "err", "stream", "workspace", "workspace_bytes")
-    v = dict(zip(names, (native.ATTEND.size, 1, 4, 4, 8, 2, 64, 16, 10, 1, 0.125, 100, 300, 4096, 4096, 4096, 4096, 0,
+    v = dict(zip(names, (ATTEND_ARGS.size, 1, 4, 4, 8, 2, 64, 16, 10, 1, 0.125, 100, 300, 4096, 4096, 4096, 4096, 0,
                          512, 64, 512, 64, 2048, 128, 64, 2048, 128, 64, 4096, 10, 4096, 0, 4096, 0, 0, 0, 0))) | change
-    return native.ATTEND.pack(*(v[n] for n in names))
+    return ATTEND_ARGS.pack(*(v[n] for n in names))
 
 
 @pytest.mark.parametrize("change", [
@@ -255,17 +273,14 @@ def attend_args(**change):
     dict(workspace=4096, workspace_bytes=16), dict(workspace=4097, workspace_bytes=1 << 40),
 ])
 def test_c_attend_refuses(change):
-    args = attend_args(**change)
-    with pytest.raises(native.NativeError) as exc:
-        native.call_op("tila_attend_shared_prefix", args)
-    assert exc.value.status == native.TILA_ERR_ARGUMENT and exc.value.log
+    refused("tila_attend_shared_prefix", attend_args(**change))
 
 
 def test_c_attend_workspace():
     """One partial result (dim + 1 floats) for every row and chunk; none where one
     block does it all; none for a call of no rows."""
-    assert native.attend_workspace(attend_args()) % (4 * 8 * 65 * 4) == 0
-    assert native.attend_workspace(attend_args()) > 0
-    assert native.attend_workspace(attend_args(prefix_length=0, table_width=1)) == 0
-    assert native.attend_workspace(attend_args(tokens=0, batch=0)) == 0
-    native.call_op("tila_attend_shared_prefix", attend_args(tokens=0, batch=0))
+    assert workspace("tila_attend_workspace", attend_args()) % (4 * 8 * 65 * 4) == 0
+    assert workspace("tila_attend_workspace", attend_args()) > 0
+    assert workspace("tila_attend_workspace", attend_args(prefix_length=0, table_width=1)) == 0
+    assert workspace("tila_attend_workspace", attend_args(tokens=0, batch=0)) == 0
+    assert native.library().tila_attend_shared_prefix(attend_args(tokens=0, batch=0), None, ctypes.c_size_t(0)) == native.TILA_OK

@@ -3,6 +3,7 @@
 * ``libtila_b200.so``: the C-ABI launcher (csrc/launcher.cpp), linked
   against NVRTC (libcuda is opened at run time), and the operators' kernels
   (csrc/ops).
+* ``_ops.so``: the operators' Python binding (csrc/ops/binding.cpp);
 * a compile check of the tile library for sm_100a with nvcc;
 * optionally, the cubins of the five benchmarked workloads (NVRTC works without
   a GPU), so that a fresh GPU machine does not spend its first launches
@@ -49,6 +50,29 @@ def build_library(verbose=False) -> Path:
         subprocess.run([*nvcc, "-shared", *[str(o) for o in objs], f"-L{CUDA / 'lib64'}", "-lnvrtc", "-ldl",
                         "-Xlinker", f"-rpath,{CUDA / 'lib64'}", "-o", str(out) + ".tmp"],
                        check=True, capture_output=not verbose)
+    os.replace(str(out) + ".tmp", out)
+    return out
+
+
+def build_binding(verbose=False) -> Path:
+    """The operators' Python binding (csrc/ops/binding.cpp, module
+    ``tila_b200._ops``): host C++ against the installed torch, linked with
+    ``libtila_b200.so`` beside it."""
+    import sysconfig
+    out = PKG / "_ops.so"
+    lib = build_library(verbose)
+    src, hdr = PKG / "csrc" / "ops" / "binding.cpp", ROOT / "include" / "tila_b200.h"
+    if out.exists() and out.stat().st_mtime > max(p.stat().st_mtime for p in (src, hdr)):
+        return out
+    import torch
+    home = Path(torch.__file__).resolve().parent
+    cmd = ["g++", "-std=c++17", "-O2", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f"-I{home / 'include'}", f"-I{home / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
+           f"-I{CUDA / 'include'}", f"-I{sysconfig.get_paths()['include']}", str(src),
+           f"-L{home / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
+           str(lib), "-Wl,-rpath,$ORIGIN", "-o", str(out) + ".tmp"]
+    subprocess.run(cmd, check=True, capture_output=not verbose)
     os.replace(str(out) + ".tmp", out)
     return out
 
@@ -143,6 +167,7 @@ def warm_cubins():
 def main(argv=None):
     argv = sys.argv[1:] if argv is None else argv
     build_library(verbose=True)
+    build_binding(verbose=True)
     check_tile_library()
     if "--warm" in argv:
         print("compiled:", ", ".join(warm_cubins()))

@@ -1,7 +1,7 @@
 """ctypes binding of ``libtila_b200.so`` (C ABI in ``include/tila_b200.h``).
 
-This module is the only place that calls into the native launcher.  It
-provides: NVRTC compilation of generated CUDA C++ into sm_100a cubins (with an
+This module is the only place that calls into the native launcher (the operators
+have a binding of their own, ``csrc/ops/binding.cpp``).  It provides: NVRTC compilation of generated CUDA C++ into sm_100a cubins (with an
 on-disk cubin cache), library loading, kernel lookup, resource queries,
 launching, and TMA tensor-map encoding.
 
@@ -14,7 +14,6 @@ from __future__ import annotations
 import ctypes
 import hashlib
 import os
-import struct
 import threading
 from pathlib import Path
 
@@ -141,11 +140,6 @@ def library() -> ctypes.CDLL:
         lib.tila_mg_gather.argtypes = [c_void_p, c_void_p, c_void_p, c_size_t, ctypes.c_uint64,
                                        c_char_p, c_size_t]
         lib.tila_mg_comm_destroy.argtypes = [c_void_p]
-        for name in ("tila_rotary_rows", "tila_rotary_norm_backward", "tila_attend_shared_prefix"):
-            getattr(lib, name).argtypes = [c_char_p, c_char_p, c_size_t]
-        for name in ("tila_rotary_workspace", "tila_attend_workspace"):
-            getattr(lib, name).argtypes = [c_char_p]
-            getattr(lib, name).restype = ctypes.c_uint64
         _lib = lib
         return lib
 
@@ -406,41 +400,3 @@ def mg_gather(comm: int, send_ptr: int, recv_ptr: int, bytes_per_rank: int, stre
 
 def mg_comm_destroy(comm: int) -> None:
     _check(library().tila_mg_comm_destroy(ctypes.c_void_p(comm)), "communicator destroy")
-
-
-# -- operators (csrc/ops): argument structures packed as bytes ----------------
-
-TILA_DTYPE = {"float32": 0, "float16": 1, "bfloat16": 2}
-
-ROWS_ROTATE, ROWS_NORM, ROWS_PAGED, ROWS_WEIGHT_F32 = 1, 2, 4, 8
-
-#: tila_op_rows, and tila_rotary_args without its rows (include/tila_b200.h).
-ROWS = struct.Struct("=4Q9qiI")
-ROTARY_HEAD = struct.Struct("=Iiqq4iffQ2qQQqq4i6Q")
-ROTARY_ROWS = 3
-ROTARY_BYTES = ROTARY_HEAD.size + ROTARY_ROWS * ROWS.size
-NO_ROWS = bytes(ROWS.size)
-#: tila_attend_args.
-ATTEND = struct.Struct("=Iiq7if2q5Q4q6qQq7Q")
-
-_op_log = threading.local()
-
-
-def call_op(name: str, args: bytes) -> None:
-    """Call the operator entry point ``name`` with its packed arguments."""
-    log = getattr(_op_log, "buffer", None)
-    if log is None:
-        log = _op_log.buffer = ctypes.create_string_buffer(1024)
-    status = getattr(library(), name)(args, log, 1024)
-    if status != TILA_OK:
-        _check(status, name, log)
-
-
-def rotary_workspace(args: bytes) -> int:
-    """Bytes of workspace that tila_rotary_norm_backward needs."""
-    return library().tila_rotary_workspace(args)
-
-
-def attend_workspace(args: bytes) -> int:
-    """Bytes of workspace that tila_attend_shared_prefix needs."""
-    return library().tila_attend_workspace(args)
