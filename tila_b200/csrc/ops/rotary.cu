@@ -10,15 +10,25 @@
 // bits.  All products and sums are 32-bit; a result is rounded once, when it is
 // stored.
 //
-// Bound by memory: a row is read once and written once.  One block takes a few
-// tokens with all their heads, of every tensor of the call, so that the sines
-// of a token are computed once and shared through shared memory; as many tokens as
-// give each thread one sine, where there are enough of them for the whole GPU.  A row
-// is spread over as many lanes as it has units; a unit is the two V-element vectors
-// that hold both halves of V pairs, so that neither layout moves data between
+// Bound by memory: a row is read once and written once (with norms, at 16 bits, the
+// instructions come close: 16 elements of a lane are 64 bytes and about 200
+// instructions).  A block takes a few tokens with all their heads, of every tensor of
+// the call, so that the sines of a token are computed once and shared through shared
+// memory, and so few or many that all blocks are whole waves of the GPU.  A row is
+// spread over as many lanes as it has units; a unit is the two V-element vectors that
+// hold both halves of V pairs, so that neither layout moves data between
 // lanes, and V elements are one 16-byte access where sizes, strides and
-// addresses allow it.  A row's loads are issued one row ahead, the first before the
-// sines.
+// addresses allow it.  Rows are taken tensor by tensor, so that pointers, flags and
+// weights stay where they are from row to row; a row is loaded one ahead, and no load
+// is conditional, so that all of a row's are in flight together.  Arithmetic is on
+// pairs of 32-bit floats.
+//
+// Measured (B200): rotate gradient of 4 x 2048 x 32 heads x 128, 32 bits: 46 us, 5.8
+// TB/s; norm_rotate of 8192 tokens x 40 heads x 128, bf16: 40 us, 4.2 TB/s, its
+// gradient 76 us; append of 16384 tokens with 32 queries heads and 8 key heads 77 us, 5.2 TB/s.
+// Tried and not kept: a warp for each token with sines and weights in registers
+// (norms 57 us), and the same with rows through a ring in shared memory (norms 41 us,
+// the gradient 70 us, but 107 us for the append and 7 us for 64 tokens).
 
 #include "ops_common.cuh"
 
@@ -50,8 +60,8 @@ struct Params {
   int units;
   int full;              // every lane has whole units
   int tokens_per_block;
-  int step_tokens, step_heads;   // from a group's row to its next one
   int any_norm, any_paged;
+  int apart;             // a block for each tensor: few tokens, where latency counts
   float sign;            // -1 rotates back
   float amplitude, eps, inv_dim;
   const void *positions;
@@ -68,34 +78,40 @@ __device__ __forceinline__ i64 index_at(const void *p, i64 i, int wide) {
   return wide ? static_cast<const i64 *>(p)[i] : static_cast<i64>(static_cast<const i32 *>(p)[i]);
 }
 
-// Offsets of a unit's two vectors inside a row.
-template <int V>
-__device__ __forceinline__ void unit_at(const Params &p, int u, int &first, int &second) {
-  const int pairs = p.half / V;                 // units that rotate
-  if (u < pairs && !p.interleaved) {
-    first = u * V;
-    second = p.half + u * V;
-  } else {
-    first = 2 * V * u;                          // also the tail: it starts at 2 * V * pairs
-    second = first + V;
+// A lane's units: where their two vectors lie in a row, and which there are.  A lane
+// without a unit, or a unit without a second vector, has another one's place.
+template <int V, int K> struct Units {
+  int first[K], second[K];
+  bool there[K], both[K], turns[K];
+  __device__ __forceinline__ Units(const Params &p, int lane) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int u = lane + k * p.lanes, pairs = p.half / V;   // units that rotate
+      there[k] = u < p.units;
+      turns[k] = u < pairs;
+      const int at = there[k] ? u : 0;
+      if (at < pairs && !p.interleaved) {
+        first[k] = at * V;
+        second[k] = p.half + at * V;
+      } else {
+        first[k] = 2 * V * at;                                // also the tail: it starts at 2 * V * pairs
+        second[k] = first[k] + V;
+      }
+      both[k] = there[k] && second[k] < p.dim;
+      if (second[k] >= p.dim) second[k] = first[k];
+    }
   }
-}
+};
 
 template <typename T, int V, int K>
 struct Raw { Vec<T, V> a[K], b[K]; };
 
-// No load is conditional, so that all of a row's are in flight together: a lane
-// without a unit, or a unit without a second vector, reads another one, which unpack
-// replaces by zeros.
 template <typename T, int V, int K>
-__device__ __forceinline__ void load_row(const Params &p, const T *row, int lane, Raw<T, V, K> &r) {
+__device__ __forceinline__ void load_row(const Units<V, K> &u, const T *row, Raw<T, V, K> &r) {
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int u = lane + k * p.lanes;
-    int first, second;
-    unit_at<V>(p, u < p.units ? u : 0, first, second);
-    r.a[k] = *reinterpret_cast<const Vec<T, V> *>(row + first);
-    r.b[k] = *reinterpret_cast<const Vec<T, V> *>(row + (second < p.dim ? second : first));
+    r.a[k] = *reinterpret_cast<const Vec<T, V> *>(row + u.first[k]);
+    r.b[k] = *reinterpret_cast<const Vec<T, V> *>(row + u.second[k]);
   }
 }
 
@@ -104,7 +120,7 @@ __device__ __forceinline__ void load_row(const Params &p, const T *row, int lane
 template <int V, int K> using Lane = u64[K][V];
 
 template <typename T, int V, int K>
-__device__ __forceinline__ void unpack(const Params &p, int lane, const Raw<T, V, K> &r, Lane<V, K> &x) {
+__device__ __forceinline__ void unpack(const Params &p, const Units<V, K> &u, const Raw<T, V, K> &r, Lane<V, K> &x) {
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -115,34 +131,25 @@ __device__ __forceinline__ void unpack(const Params &p, int lane, const Raw<T, V
     }
   if (p.full) return;
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int u = lane + k * p.lanes;
-    int first, second;
-    unit_at<V>(p, u, first, second);
+  for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int e = 0; e < 2 * V; ++e)
-      if (u >= p.units || (e >= V && second >= p.dim))
+      if (!(e < V ? u.there[k] : u.both[k]))
         x[k][e >> 1] = e & 1 ? tila::pk2(tila::lo2(x[k][e >> 1]), 0.f) : tila::pk2(0.f, tila::hi2(x[k][e >> 1]));
-  }
 }
 
 template <typename T, int V, int K>
-__device__ __forceinline__ void store_row(const Params &p, T *row, int lane, const Lane<V, K> &x) {
+__device__ __forceinline__ void store_row(const Units<V, K> &u, T *row, const Lane<V, K> &x) {
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int u = lane + k * p.lanes;
-    if (u < p.units) {
-      int first, second;
-      unit_at<V>(p, u, first, second);
-      Vec<T, V> a, b;
+    Vec<T, V> a, b;
 #pragma unroll
-      for (int e = 0; e < 2 * V; ++e) {
-        const float f = e & 1 ? tila::hi2(x[k][e >> 1]) : tila::lo2(x[k][e >> 1]);
-        (e < V ? a.e[e % V] : b.e[e % V]) = Elem<T>::put(f);
-      }
-      *reinterpret_cast<Vec<T, V> *>(row + first) = a;
-      if (second < p.dim) *reinterpret_cast<Vec<T, V> *>(row + second) = b;
+    for (int e = 0; e < 2 * V; ++e) {
+      const float f = e & 1 ? tila::hi2(x[k][e >> 1]) : tila::lo2(x[k][e >> 1]);
+      (e < V ? a.e[e % V] : b.e[e % V]) = Elem<T>::put(f);
     }
+    if (u.there[k]) *reinterpret_cast<Vec<T, V> *>(row + u.first[k]) = a;
+    if (u.both[k]) *reinterpret_cast<Vec<T, V> *>(row + u.second[k]) = b;
   }
 }
 
@@ -166,30 +173,27 @@ __device__ __forceinline__ void floats_at(const float *p, float (&x)[V]) {
 // Turns the pairs of a row; `tab` holds the cosines, then the sines, of the row's
 // token, the amplitude in both.
 template <int V, int K>
-__device__ __forceinline__ void turn(const Params &p, const float *tab, int lane, Lane<V, K> &x) {
-  const int units = p.half / V;
+__device__ __forceinline__ void turn(const Params &p, const Units<V, K> &u, const float *tab, int lane, Lane<V, K> &x) {
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int u = lane + k * p.lanes;
-    if (u < units) {
-      float c[V], s[V];
-      floats_at<V>(tab + u * V, c);
-      floats_at<V>(tab + p.half + u * V, s);
-      if (V == 1 || p.interleaved) {
+    if (!u.turns[k]) continue;                                // (elements behind `rotary` stay bit for bit)
+    float c[V], s[V];
+    floats_at<V>(tab + (lane + k * p.lanes) * V, c);
+    floats_at<V>(tab + p.half + (lane + k * p.lanes) * V, s);
+    if (V == 1 || p.interleaved) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float a = tila::lo2(x[k][i]), b = tila::hi2(x[k][i]);
-          x[k][i] = tila::pk2(a * c[i] - b * s[i], b * c[i] + a * s[i]);
-        }
-      } else {
+      for (int i = 0; i < V; ++i) {
+        const float a = tila::lo2(x[k][i]), b = tila::hi2(x[k][i]);
+        x[k][i] = tila::pk2(a * c[i] - b * s[i], b * c[i] + a * s[i]);
+      }
+    } else {
 #pragma unroll
-        for (int i = 0; i < V / 2; ++i) {
-          const u64 a = x[k][i], b = x[k][V / 2 + i];
-          const u64 cc = tila::pk2(c[2 * i], c[2 * i + 1]), ss = tila::pk2(s[2 * i], s[2 * i + 1]);
-          const u64 minus = tila::pk2(-s[2 * i], -s[2 * i + 1]);
-          x[k][i] = tila::fma2(b, minus, tila::mul2(a, cc));
-          x[k][V / 2 + i] = tila::fma2(a, ss, tila::mul2(b, cc));
-        }
+      for (int i = 0; i < V / 2; ++i) {
+        const u64 a = x[k][i], b = x[k][V / 2 + i];
+        const u64 cc = tila::pk2(c[2 * i], c[2 * i + 1]), ss = tila::pk2(s[2 * i], s[2 * i + 1]);
+        const u64 bs = tila::mul2(b, ss);
+        x[k][i] = tila::fma2(a, cc, bs ^ 0x8000000080000000ull);
+        x[k][V / 2 + i] = tila::fma2(a, ss, tila::mul2(b, cc));
       }
     }
   }
@@ -237,22 +241,18 @@ __device__ __forceinline__ float row_sum(const Params &p, const Lane<V, K> &x, c
 
 // x * w of the elements that a lane holds.
 template <int V, int K>
-__device__ __forceinline__ void times_weight(const Params &p, const float *w, int lane, Lane<V, K> &x) {
+__device__ __forceinline__ void times_weight(const Units<V, K> &u, const float *w, Lane<V, K> &x) {
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int u = lane + k * p.lanes;
-    if (u < p.units) {
-      int first, second;
-      unit_at<V>(p, u, first, second);
-      float w0[V], w1[V];
-      floats_at<V>(w + first, w0);
-      floats_at<V>(w + (second < p.dim ? second : first), w1);   // (behind the row's end: not stored)
+    float e[2 * V], f[V];
+    floats_at<V>(w + u.first[k], f);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int e = 2 * i;
-        x[k][i] = tila::mul2(x[k][i], tila::pk2(e < V ? w0[e % V] : w1[e % V], e + 1 < V ? w0[(e + 1) % V] : w1[(e + 1) % V]));
-      }
-    }
+    for (int i = 0; i < V; ++i) e[i] = f[i];
+    floats_at<V>(w + u.second[k], f);
+#pragma unroll
+    for (int i = 0; i < V; ++i) e[V + i] = f[i];
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[k][i] = tila::mul2(x[k][i], tila::pk2(e[2 * i], e[2 * i + 1]));
   }
 }
 
@@ -274,82 +274,96 @@ template <typename T, int V, int K>
 __global__ void __launch_bounds__(256, Resident<T, V>::kForward)
 rotary_rows_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(16) float tab[];
-  int2 *places = reinterpret_cast<int2 *>(tab + table_size(p));       // page and row of each token's slot
-  float *weights = reinterpret_cast<float *>(places + (p.any_paged ? ((p.tokens_per_block + 1) & ~1) : 0));
-  const u32 b = p.batch == 1 ? 0 : blockIdx.x / static_cast<u32>(p.blocks_per_batch);
-  const i64 token0 = static_cast<i64>(blockIdx.x - b * static_cast<u32>(p.blocks_per_batch)) * p.tokens_per_block;
+  i64 *places = reinterpret_cast<i64 *>(tab + table_size(p));       // offsets of each token's slot in the paged tensors
+  float *weights = reinterpret_cast<float *>(places + (p.any_paged ? 3 * p.tokens_per_block + 1 : 0) / 2 * 2);
+  const u32 block = p.apart ? blockIdx.x / p.num_rows : blockIdx.x;
+  const int first_r = p.apart ? blockIdx.x - block * p.num_rows : 0, last_r = p.apart ? first_r + 1 : p.num_rows;
+  const u32 b = p.batch == 1 ? 0 : block / static_cast<u32>(p.blocks_per_batch);
+  const i64 token0 = static_cast<i64>(block - b * static_cast<u32>(p.blocks_per_batch)) * p.tokens_per_block;
   const int tokens = static_cast<int>(min(static_cast<i64>(p.tokens_per_block), p.tokens - token0));
-  const int jobs = tokens * p.heads;
   const int groups = blockDim.x / p.lanes;
-  const int lane = threadIdx.x & (p.lanes - 1);
+  const int lane = threadIdx.x & (p.lanes - 1), group = threadIdx.x / p.lanes;
+  const Units<V, K> units(p, lane);
 
-  // a job is a row: jobs run over the heads of all tensors of one token, then over the
-  // tokens; a group's next job is `groups` on
-  int job = threadIdx.x / p.lanes;
-  int t = min(job, jobs - 1) / p.heads, h = min(job, jobs - 1) - t * p.heads;
-  auto which = [&](int &head) {
-    head = h;
-    if (head < p.rows[0].heads) return 0;
-    head -= p.rows[0].heads;
-    if (head < p.rows[1].heads) return 1;
-    head -= p.rows[1].heads;
-    return 2;
-  };
-  auto load = [&](Raw<T, V, K> &raw) {
-    int head;
-    const Rows &r = p.rows[which(head)];
-    load_row<T, V, K>(p, static_cast<const T *>(r.src) + b * r.src_stride[0] + (token0 + t) * r.src_stride[1] +
-                             head * r.src_stride[2], lane, raw);
-  };
-
+  // Rows are taken tensor by tensor: its heads of one token, then of the next, one
+  // to a group; each group's next row is `groups` on.  A group that has none left
+  // reads its last one again.
+  int job = 0, t = 0, h = 0, jobs = 0;                       // of the row that is loaded
+  const T *base = nullptr;
   Raw<T, V, K> raw;
-  load(raw);
-  fill_table(p, b, token0, tokens, tab);
+  auto begin = [&](int r) {                                  // the first row of the first tensor from r on that has any
+    for (; r < last_r && p.rows[r].heads == 0; ++r) {}
+    if (r < last_r) {
+      const Rows &rows = p.rows[r];
+      jobs = tokens * rows.heads;
+      job = group;
+      t = min(job, jobs - 1) / rows.heads;
+      h = min(job, jobs - 1) - t * rows.heads;
+      base = static_cast<const T *>(rows.src) + b * rows.src_stride[0] + token0 * rows.src_stride[1];
+      load_row<T, V, K>(units, base + t * rows.src_stride[1] + h * rows.src_stride[2], raw);
+    }
+    return r;
+  };
+  int r = begin(first_r);
+  if (!p.apart || (p.rows[first_r].flags & TILA_ROWS_ROTATE)) fill_table(p, b, token0, tokens, tab);
   if (p.any_norm) fill_weights<T>(p, weights, p.num_rows);
   if (p.any_paged)
     for (int i = threadIdx.x; i < tokens; i += blockDim.x) {
       const i64 slot = index_at(p.slots, (token0 + i) * p.slot_stride, p.index64 & 2);
       if (slot >= p.num_slots) tila::report_error(p.err, kErrIndex, static_cast<u32>(token0 + i));
-      const i64 page = slot / p.page_size;
-      places[i] = slot < 0 || slot >= p.num_slots ? make_int2(-1, 0)
-                                                  : make_int2(static_cast<int>(page), static_cast<int>(slot - page * p.page_size));
+      const bool in = slot >= 0 && slot < p.num_slots;
+      const u64 place = in ? slot : 0;
+      const u64 page = place >> 32 ? place / p.page_size : static_cast<u32>(place) / static_cast<u32>(p.page_size);
+      const i64 row = static_cast<i64>(place - page * p.page_size);
+      for (int k = 0; k < p.num_rows; ++k)
+        places[3 * i + k] = in ? static_cast<i64>(page) * p.rows[k].dst_stride[0] + row * p.rows[k].dst_stride[1] : -1;
     }
   __syncthreads();
 
-  // every warp runs the same number of times: the norm's sum is over its lanes
-  for (int first = 0; first < jobs; first += groups) {
-    const bool valid = job < jobs;
-    int head;
-    const int tensor = which(head), at = t;
-    Lane<V, K> x;
-    unpack<T, V, K>(p, lane, raw, x);
-    job += groups;
-    if (job < jobs) {                          // (else the same row again, unused)
-      t += p.step_tokens;
-      h += p.step_heads;
-      if (h >= p.heads) {
-        h -= p.heads;
-        ++t;
+  while (r < last_r) {
+    const Rows &rows = p.rows[r];
+    const u32 flags = rows.flags;
+    const i64 src_token = rows.src_stride[1], src_head = rows.src_stride[2];
+    const i64 dst_token = rows.dst_stride[1], dst_head = rows.dst_stride[2];
+    const int heads = rows.heads, all = jobs, this_r = r;
+    const int dt = groups / heads, dh = groups - dt * heads;
+    const float *w = weights + r * p.dim;
+    T *dst = static_cast<T *>(rows.dst) + (flags & TILA_ROWS_PAGED ? 0 : b * rows.dst_stride[0] + token0 * dst_token);
+    // every warp runs the same number of times: the norm's sum is over its lanes
+    for (int first = 0; first < all; first += groups) {
+      const bool valid = job < all;
+      const int at = t, head = h;
+      Lane<V, K> x;
+      unpack<T, V, K>(p, units, raw, x);
+      if (first + groups < all) {
+        job += groups;
+        if (job < all) {
+          t += dt;
+          h += dh;
+          if (h >= heads) {
+            h -= heads;
+            ++t;
+          }
+        }
+        load_row<T, V, K>(units, base + t * src_token + h * src_head, raw);
+      } else {
+        r = begin(this_r + 1);
       }
-    }
-    if (first + groups < jobs) load(raw);
-    const Rows &r = p.rows[tensor];
-    if (p.any_norm) {
-      const float ss = row_sum<V, K>(p, x, x);
-      if (r.flags & TILA_ROWS_NORM) {
-        times<V, K>(rsqrtf(ss * p.inv_dim + p.eps), x);
-        times_weight<V, K>(p, weights + tensor * p.dim, lane, x);
+      if (flags & TILA_ROWS_NORM) {
+        times<V, K>(rsqrtf(row_sum<V, K>(p, x, x) * p.inv_dim + p.eps), x);
+        times_weight<V, K>(units, w, x);
       }
-    }
-    if (!valid) continue;
-    if (r.flags & TILA_ROWS_ROTATE) turn<V, K>(p, tab + 2 * at * p.half, lane, x);
-    T *dst = static_cast<T *>(r.dst) + head * r.dst_stride[2];
-    if (r.flags & TILA_ROWS_PAGED) {
-      const int2 place = places[at];
-      if (place.x >= 0)
-        store_row<T, V, K>(p, dst + place.x * r.dst_stride[0] + place.y * r.dst_stride[1], lane, x);
-    } else {
-      store_row<T, V, K>(p, dst + b * r.dst_stride[0] + (token0 + at) * r.dst_stride[1], lane, x);
+      if (flags & TILA_ROWS_ROTATE) turn<V, K>(p, units, tab + 2 * at * p.half, lane, x);
+      i64 to = head * dst_head;
+      bool put = valid;
+      if (flags & TILA_ROWS_PAGED) {
+        const i64 place = places[3 * at + this_r];
+        put = put && place >= 0;
+        to += place;
+      } else {
+        to += at * dst_token;
+      }
+      if (put) store_row<T, V, K>(units, dst + to, x);
     }
   }
 }
@@ -368,6 +382,7 @@ rotary_norm_backward_kernel(const __grid_constant__ Params p) {
   float *scratch = weights + 2 * p.dim;
   const int groups = blockDim.x / p.lanes;
   const int lane = threadIdx.x & (p.lanes - 1), group = threadIdx.x / p.lanes;
+  const Units<V, K> units(p, lane);
   tila::grid_dep_release();
   fill_weights<T>(p, weights, p.num_rows);
   const i64 all = p.batch * p.tokens;
@@ -390,10 +405,10 @@ rotary_norm_backward_kernel(const __grid_constant__ Params p) {
       const int dt = groups / r.heads, dh = groups - dt * r.heads;
       Raw<T, V, K> rx, rg;
       auto load = [&] {
-        load_row<T, V, K>(p, static_cast<const T *>(r.src) + b * r.src_stride[0] + (token0 + t) * r.src_stride[1] +
-                                 h * r.src_stride[2], lane, rx);
-        load_row<T, V, K>(p, static_cast<const T *>(r.grad) + b * r.grad_stride[0] + (token0 + t) * r.grad_stride[1] +
-                                 h * r.grad_stride[2], lane, rg);
+        load_row<T, V, K>(units, static_cast<const T *>(r.src) + b * r.src_stride[0] + (token0 + t) * r.src_stride[1] +
+                                 h * r.src_stride[2], rx);
+        load_row<T, V, K>(units, static_cast<const T *>(r.grad) + b * r.grad_stride[0] + (token0 + t) * r.grad_stride[1] +
+                                 h * r.grad_stride[2], rg);
       };
       load();
       __syncthreads();
@@ -403,8 +418,8 @@ rotary_norm_backward_kernel(const __grid_constant__ Params p) {
         const bool valid = job < jobs;
         const int at = t, head = h;
         Lane<V, K> x, g;
-        unpack<T, V, K>(p, lane, rx, x);
-        unpack<T, V, K>(p, lane, rg, g);
+        unpack<T, V, K>(p, units, rx, x);
+        unpack<T, V, K>(p, units, rg, g);
         job += groups;
         if (job < jobs) {                      // (else the same row again, unused)
           t += dt;
@@ -415,7 +430,7 @@ rotary_norm_backward_kernel(const __grid_constant__ Params p) {
           }
         }
         if (first + groups < jobs) load();
-        if (valid && (r.flags & TILA_ROWS_ROTATE)) turn<V, K>(p, tab + 2 * at * p.half, lane, g);
+        if (valid && (r.flags & TILA_ROWS_ROTATE)) turn<V, K>(p, units, tab + 2 * at * p.half, lane, g);
         const float rms = rsqrtf(row_sum<V, K>(p, x, x) * p.inv_dim + p.eps);
         times<V, K>(rms, x);                                        // xh
         if (valid)
@@ -423,7 +438,7 @@ rotary_norm_backward_kernel(const __grid_constant__ Params p) {
           for (int k = 0; k < K; ++k)
 #pragma unroll
             for (int i = 0; i < V; ++i) sum[k][i] = tila::fma2(g[k][i], x[k][i], sum[k][i]);
-        times_weight<V, K>(p, weights + tensor * p.dim, lane, g);   // w g
+        times_weight<V, K>(units, weights + tensor * p.dim, g);   // w g
         const float mean = row_sum<V, K>(p, g, x) * p.inv_dim;
         const u64 minus = tila::pk2(-mean, -mean);
 #pragma unroll
@@ -432,28 +447,20 @@ rotary_norm_backward_kernel(const __grid_constant__ Params p) {
           for (int i = 0; i < V; ++i) x[k][i] = tila::fma2(x[k][i], minus, g[k][i]);
         times<V, K>(rms, x);
         if (valid)
-          store_row<T, V, K>(p, static_cast<T *>(r.dst) + b * r.dst_stride[0] + (token0 + at) * r.dst_stride[1] +
-                                    head * r.dst_stride[2], lane, x);
+          store_row<T, V, K>(units, static_cast<T *>(r.dst) + b * r.dst_stride[0] + (token0 + at) * r.dst_stride[1] +
+                                    head * r.dst_stride[2], x);
       }
       from += tokens;
     }
     // the groups' sums, then this block's partial sum
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int u = lane + k * p.lanes;
-      if (u < p.units) {
-        int first, second;
-        unit_at<V>(p, u, first, second);
+    for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int e = V + i;
-          scratch[group * p.dim + first + i] = i & 1 ? tila::hi2(sum[k][i >> 1]) : tila::lo2(sum[k][i >> 1]);
-          if (second < p.dim)
-            scratch[group * p.dim + second + i] = e & 1 ? tila::hi2(sum[k][e >> 1]) : tila::lo2(sum[k][e >> 1]);
-        }
-      }
-    }
+      for (int e = 0; e < 2 * V; ++e)
+        if (e < V ? units.there[k] : units.both[k])
+          scratch[group * p.dim + (e < V ? units.first[k] : units.second[k]) + e % V] =
+              e & 1 ? tila::hi2(sum[k][e >> 1]) : tila::lo2(sum[k][e >> 1]);
     __syncthreads();
     for (int j = threadIdx.x; j < p.dim; j += blockDim.x) {
       float s = 0.f;
@@ -620,14 +627,14 @@ int launch_forward(Params p, cudaStream_t stream, char *log, size_t cap) {
   p.full = p.dim % (2 * V) == 0 && p.units == p.lanes * K;
   p.tokens_per_block = tokens_per_block(p, Resident<T, V>::kForward);
   p.blocks_per_batch = (p.tokens + p.tokens_per_block - 1) / p.tokens_per_block;
-  const i64 blocks = p.blocks_per_batch * p.batch;
+  i64 blocks = p.blocks_per_batch * p.batch;
+  p.apart = p.num_rows > 1 && blocks * p.num_rows <= 4 * kSms;
+  if (p.apart) blocks *= p.num_rows;
   if (blocks > 0x7fffffff) return fail(TILA_ERR_ARGUMENT, log, cap, "tila_rotary_rows: too many tokens for one launch");
   const i64 lanes = static_cast<i64>(p.tokens_per_block) * p.heads * p.lanes;
   const int threads = static_cast<int>(std::min<i64>(256, (lanes + 31) / 32 * 32));
-  p.step_tokens = threads / p.lanes / p.heads;
-  p.step_heads = threads / p.lanes - p.step_tokens * p.heads;
   const size_t smem = sizeof(float) * table_size(p) +
-                      (p.any_paged ? sizeof(int2) * ((p.tokens_per_block + 1) & ~1) : 0) +
+                      (p.any_paged ? sizeof(i64) * ((3 * p.tokens_per_block + 1) / 2 * 2) : 0) +
                       (p.any_norm ? 3 * sizeof(float) * p.dim : 0) + 16;
   rotary_rows_kernel<T, V, K><<<static_cast<unsigned>(blocks), threads, smem, stream>>>(p);
   return launch_status(cudaGetLastError(), "tila_rotary_rows", log, cap);
