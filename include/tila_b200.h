@@ -284,7 +284,10 @@ typedef struct tila_attend_args {
   int32_t dim;              /* a multiple of 8 up to 256 */
   int32_t page_size, table_width;  /* rows of a page; pages of a table row */
   int32_t max_queries;      /* most new tokens of one sequence */
+  int32_t max_length;       /* the longest of lengths as far as the host knows (0: the table's
+                               width): a hint for how the work is split */
   float scale;
+  int32_t reserved;         /* must be 0 */
   int64_t num_pages, prefix_length;
   uint64_t q, k_cache, v_cache, out;
   uint64_t lse;             /* tokens x heads floats: log of the sum of exp (0 = not wanted) */

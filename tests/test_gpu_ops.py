@@ -351,6 +351,20 @@ def test_attend_several_tokens(dtype, heads_first, counts, lengths, prefix, head
     check_attend(case, counts, lengths, prefix)
 
 
+@pytest.mark.parametrize("spare,hint", [(0, 300), (0, 1), (500, None), (500, 300)])
+def test_attend_wide_tables_and_hints(spare, hint):
+    """A table far wider than its sequences, and hints about the longest, right or
+    wrong, split the work otherwise and change nothing else."""
+    lengths = [300, 0, 64, 1]
+    for counts in ([1] * 4, [40, 0, 64, 1]):
+        q, kc, vc, table, lens, pages, offsets = paged(5, counts, lengths, 500, 8, 2, 128, 16, BF16, spare=spare)
+        got = ops.attend_shared_prefix(q, kc, vc, table, lens, prefix_pages=pages, prefix_length=500, max_length=hint,
+                                       query_offsets=offsets, max_queries=max(counts))
+        want, _, tol, _ = attend(q, kc, vc, table, lens, pages, 500, counts, 128 ** -0.5)
+        assert ((got.double() - want).abs() <= tol).all()
+    ops.check_errors()
+
+
 @pytest.mark.parametrize("scale", [0.0, 30.0, -0.5])
 def test_attend_scales(scale):
     """Equal weights, weights that all go to one key, and a negative scale."""

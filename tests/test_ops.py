@@ -165,7 +165,7 @@ def test_append_refuses(change, text):
 
 
 # tila_op_rows, tila_rotary_args without its rows, tila_attend_args (include/tila_b200.h)
-ROWS, HEAD, ATTEND_ARGS = struct.Struct("=4Q9qiI"), struct.Struct("=Iiqq4iffQ2qQQqq4i6Q"), struct.Struct("=Iiq7if2q5Q4q6qQq7Q")
+ROWS, HEAD, ATTEND_ARGS = struct.Struct("=4Q9qiI"), struct.Struct("=Iiqq4iffQ2qQQqq4i6Q"), struct.Struct("=Iiq8ifi2q5Q4q6qQq7Q")
 ROTARY_BYTES = HEAD.size + 3 * ROWS.size
 FLAG_ROTATE, FLAG_NORM, FLAG_PAGED = 1, 2, 4
 
@@ -241,6 +241,7 @@ ATTEND = dict(q=dev(3, 4, 64, dtype=H), k_cache=dev(5, 8, 2, 64, dtype=H), v_cac
     (dict(query_offsets=ints(3)), "4 entries"),
     (dict(query_offsets=ints(4), max_queries=0), "at least 1"),
     (dict(max_queries=2), "needs query_offsets"),
+    (dict(max_length=0), "at least 1"),
     (dict(prefix_length=-1), "negative"),
     (dict(prefix_length=5), "needs prefix_pages"),
     (dict(prefix_length=17, prefix_pages=ints(2)), "fewer than 17"),
@@ -258,16 +259,16 @@ def test_attend_refuses(change, text):
 def attend_args(**change):
     """tila_attend_args with addresses that nothing reads (the call is refused)."""
     names = ("size", "dtype", "tokens", "batch", "heads", "kv_heads", "dim", "page_size", "table_width", "max_queries",
-             "scale", "num_pages", "prefix_length", "q", "k_cache", "v_cache", "out", "lse", "qt", "qh", "ot", "oh",
+             "max_length", "scale", "reserved", "num_pages", "prefix_length", "q", "k_cache", "v_cache", "out", "lse", "qt", "qh", "ot", "oh",
              "kp", "kr", "kh", "vp", "vr", "vh", "page_table", "table_stride", "lengths", "query_offsets",
              "prefix_pages", "err", "stream", "workspace", "workspace_bytes")
-    v = dict(zip(names, (ATTEND_ARGS.size, 1, 4, 4, 8, 2, 64, 16, 10, 1, 0.125, 100, 300, 4096, 4096, 4096, 4096, 0,
+    v = dict(zip(names, (ATTEND_ARGS.size, 1, 4, 4, 8, 2, 64, 16, 10, 1, 0, 0.125, 0, 100, 300, 4096, 4096, 4096, 4096, 0,
                          512, 64, 512, 64, 2048, 128, 64, 2048, 128, 64, 4096, 10, 4096, 0, 4096, 0, 0, 0, 0))) | change
     return ATTEND_ARGS.pack(*(v[n] for n in names))
 
 
 @pytest.mark.parametrize("change", [
-    dict(size=8), dict(dtype=0), dict(dtype=3), dict(heads=3), dict(kv_heads=0), dict(dim=12), dict(dim=264), dict(page_size=0),
+    dict(size=8), dict(reserved=1), dict(max_length=-1), dict(dtype=0), dict(dtype=3), dict(heads=3), dict(kv_heads=0), dict(dim=12), dict(dim=264), dict(page_size=0),
     dict(max_queries=0), dict(tokens=3), dict(prefix_length=-1), dict(prefix_length=1 << 31), dict(q=0), dict(q=4097),
     dict(k_cache=4104), dict(vr=4), dict(lengths=0), dict(page_table=0), dict(prefix_pages=0), dict(lse=2),
     dict(workspace=4096, workspace_bytes=16), dict(workspace=4097, workspace_bytes=1 << 40),

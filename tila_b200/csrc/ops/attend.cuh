@@ -33,7 +33,8 @@ struct AttendParams {
   float scale2;                     // scale * log2(e)
   // the split: chunks of keys, and the slots of their partial results
   int prefix_chunk, prefix_chunks;  // chunks = slots 0 .. prefix_chunks - 1
-  int own_chunk, own_chunks;        // slots prefix_chunks ..
+  int own_chunks, own_unit;         // slots prefix_chunks ..: a sequence's own tokens in equal parts of whole units,
+  int own_least;                    // and of so many keys at least
   int direct;                       // one chunk in all: blocks write the result itself
   int q_words, q_vectors;           // q can be read in 4-byte words, in 16-byte vectors
   int out_vectors;                  // out can be written in vectors of 4 elements
@@ -64,12 +65,11 @@ __device__ __forceinline__ int own_length(const AttendParams &p, int b) {
   return static_cast<int>(min(static_cast<i64>(max(n, 0)), most));
 }
 
-// A page's number, or -1 (its keys and values read as zero) outside the pool.
-__device__ __forceinline__ int checked_page(const AttendParams &p, const i32 *pages, int i) {
-  const int page = pages[i];
-  if (page >= 0 && page < p.num_pages) return page;
-  tila::report_error(p.err, kErrIndex, i);
-  return -1;
+// Keys of each chunk of a sequence: by its own length, so that blocks share the
+// work whatever the table's width.
+__device__ __forceinline__ int own_chunk(const AttendParams &p, int length) {
+  const int each = p.own_chunks > 1 ? (length + p.own_chunks - 1) / p.own_chunks : length;
+  return max(p.own_least, (each + p.own_unit - 1) & ~(p.own_unit - 1));
 }
 
 __device__ __forceinline__ void split_key(const AttendParams &p, int key, int &page, int &row) {

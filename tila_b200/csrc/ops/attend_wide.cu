@@ -159,10 +159,11 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
       const int length = own_length(p, b);
       rows = count * p.group;
       limit0 = length - count + 1;
-      begin = chunk * p.own_chunk;
+      const int keys = own_chunk(p, length);
+      begin = chunk * keys;
       // the last token of the block's rows sees furthest
       const int last = min((pair + 1) * 2 * kTile, rows) - 1;
-      end = min(begin + p.own_chunk, limit0 + last / p.group);
+      end = min(begin + keys, limit0 + last / p.group);
       pages = p.table + b * p.table_stride;
       causal = true;
     }

@@ -14,6 +14,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <optional>
 #include <string>
@@ -569,7 +571,7 @@ uint64_t indexes(const char *fn, const char *what, const Tensor &t, const Tensor
 }
 
 // attend_shared_prefix(q, k_cache, v_cache, page_table, lengths, prefix_pages, prefix_length, query_offsets,
-//                      max_queries, scale, out, return_lse)
+//                      max_queries, scale, out, return_lse, max_length)
 PyObject *attend_shared_prefix(PyObject *const *o) {
   const char *fn = "attend_shared_prefix";
   const Tensor &q = tensor(fn, "q", o[0]);
@@ -629,6 +631,11 @@ PyObject *attend_shared_prefix(PyObject *const *o) {
     if (pages.size(0) * page_size < a.prefix_length)
       refuse("%s: prefix_pages holds %lld tokens, fewer than %lld", fn, static_cast<long long>(pages.size(0) * page_size),
              static_cast<long long>(a.prefix_length));
+  }
+  if (o[12] != Py_None) {
+    const int64_t longest = whole(o[12]);
+    if (longest < 1) refuse("%s: max_length must be at least 1, not %lld", fn, static_cast<long long>(longest));
+    a.max_length = static_cast<int32_t>(std::min<int64_t>(longest, INT32_MAX));
   }
   constexpr int64_t limit = int64_t{1} << 30;
   if (tokens > limit || batch > limit || table.size(1) > limit || most > limit)
@@ -734,7 +741,7 @@ PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
 
 PyMethodDef g_methods[] = {
     TILA_ENTRY(rotate, 7),      TILA_ENTRY(norm_rotate, 11),          TILA_ENTRY(norm_rotate_backward, 13),
-    TILA_ENTRY(append_paged, 14), TILA_ENTRY(attend_shared_prefix, 12), TILA_ENTRY(check_apart, 6),
+    TILA_ENTRY(append_paged, 14), TILA_ENTRY(attend_shared_prefix, 13), TILA_ENTRY(check_apart, 6),
     TILA_ENTRY(setup, 3),       TILA_ENTRY(set_error_block, 3),       {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_ops", "Binding of tila_b200's operators.", -1, g_methods,

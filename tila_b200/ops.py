@@ -220,7 +220,8 @@ def norm_rotate_backward(q_grad, k_grad, q, k, q_weight, k_weight, positions, in
 # ---------------------------------------------------------------------------
 
 def attend_shared_prefix(q, k_cache, v_cache, page_table, lengths, *, prefix_pages=None, prefix_length=0,
-                         query_offsets=None, max_queries=None, scale=None, out=None, return_lse=False):
+                         query_offsets=None, max_queries=None, max_length=None, scale=None, out=None,
+                         return_lse=False):
     """Attention of new tokens over a paged cache: ``softmax(scale q K^T) V`` over
     a prefix that all sequences share and each sequence's own tokens.
 
@@ -238,6 +239,8 @@ def attend_shared_prefix(q, k_cache, v_cache, page_table, lengths, *, prefix_pag
     itself.  Rows of ``q`` behind the last sequence may be anything, and theirs of
     ``out`` are left as they were.  A token that sees nothing gets zeros.
 
+    ``max_length``, the longest of ``lengths`` where the host knows it, only steers how
+    the work is split (by default the table's width, which may be far more).
     ``scale`` is 1/sqrt(dim) by default.  Returns ``out`` (q's dtype), and with
     ``return_lse`` also the log of each row's sum of exponentials, float32 (tokens,
     heads).  Scores, weights' sums and results are kept in 32 bits; the weights are
@@ -247,4 +250,4 @@ def attend_shared_prefix(q, k_cache, v_cache, page_table, lengths, *, prefix_pag
     or in pages that it does not reach, may be anything.
     """
     return _ops.attend_shared_prefix(q, k_cache, v_cache, page_table, lengths, prefix_pages, prefix_length, query_offsets,
-                                     max_queries, scale, out, bool(return_lse))
+                                     max_queries, scale, out, bool(return_lse), max_length)
