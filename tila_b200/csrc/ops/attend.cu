@@ -228,7 +228,7 @@ __device__ __forceinline__ void narrow_block(const AttendParams &p, const tila::
     if constexpr (!kTma) copy_commit();
   };
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) issue(s);
+  for (int s = 0; s < kStages; ++s) issue(s);
 
   // queries: columns g of 8, as B fragments
   const int g = lane >> 2, c = lane & 3;
@@ -276,11 +276,9 @@ __device__ __forceinline__ void narrow_block(const AttendParams &p, const tila::
     const u32 stage = ring_at + (step % kStages) * N::kStage;
     const int key0 = begin + step * kStep;
     if constexpr (kTma) {
-      // (the barrier across the warp also ends its reads of the stage that is filled next)
       if (!__all_sync(0xffffffffu, tila::mbar_wait(&full[warp][step % kStages], (step / kStages) & 1, p.err, __LINE__,
                                                    nullptr)))
         break;
-      issue(step + kStages - 1);
       if (key0 + kSlice > it.end) {
         // values behind the end: whatever the page holds there, for a weight of 0
         for (int i = lane; i < (key0 + kSlice - it.end) * (DP / 8); i += 32)
@@ -289,9 +287,8 @@ __device__ __forceinline__ void narrow_block(const AttendParams &p, const tila::
         __syncwarp();
       }
     } else {
-      copy_wait<kStages - 2>();
+      copy_wait<kStages - 1>();
       __syncwarp();
-      issue(step + kStages - 1);
     }
     // S^T: keys g and g + 8 in rows, two chains of sums
     float s[NT][2][4] = {};
@@ -355,6 +352,8 @@ __device__ __forceinline__ void narrow_block(const AttendParams &p, const tila::
         for (int t = 0; t < NT; ++t) mma16816<T>(o[t][n], a, pf[t][0], pf[t][1]);
       }
     }
+    __syncwarp();                                            // all lanes have read the stage
+    issue(step + kStages);
   }
 
   // join the warps: maxima, sums, then the scaled results through shared memory
@@ -580,9 +579,11 @@ struct Plan {
 // for a tile of 128 keys and 9.5 us beside that (queries, filling the ring, results).
 // Where the narrow form follows (`narrow_bytes`, half of what the longest sequences
 // would be), it starts beside the wide form on the multiprocessors that are left,
-// which fetch about 54 GB/s each, 6 TB/s in all: the split that ends both first (of
-// those that give the wide form 64 multiprocessors at least, since lengths may be
-// far below what the table could hold).
+// which fetch about 58 GB/s each, 6.7 TB/s in all, and takes 8 us beside that: the
+// split that ends both first (of those that give the wide form 64 multiprocessors at
+// least, since lengths may be far below what the table could hold).  128 sequences of up
+// to 4096 own tokens on 32768 shared ones: 207 us so, 237 us with the wide form on
+// every multiprocessor first; 64 of up to 1024 on 8192: 40 and 46 us.
 int wide_chunk_of(i64 keys, i64 blocks, double narrow_bytes, int &chunks) {
   const i64 tiles = (keys + 127) / 128;
   const i64 most = std::min<i64>(tiles, 64);
@@ -591,9 +592,10 @@ int wide_chunk_of(i64 keys, i64 blocks, double narrow_bytes, int &chunks) {
   for (i64 n = 1; n <= most; ++n) {
     if (narrow_bytes > 0 && blocks * n < 64 && n < most) continue;
     const double wide = ((blocks * n + kSms - 1) / kSms) * (9.5e-6 + 2.1e-6 * ((tiles + n - 1) / n));
-    const double beside = std::min(6e12, 54e9 * std::max<i64>(0, kSms - blocks * n));
+    const double beside = std::min(6.7e12, 58e9 * std::max<i64>(0, kSms - blocks * n));
     const double left = std::max(0., narrow_bytes - beside * wide);
-    const double cost = left > 0 ? wide + left / 6e12 : std::max(wide, beside > 0 ? narrow_bytes / beside : 0.);
+    const double narrow = narrow_bytes <= 0 ? 0. : 8e-6 + (left > 0 ? wide + left / 6.7e12 : narrow_bytes / beside);
+    const double cost = std::max(wide, narrow);
     if (best == 0 || cost < least) best = n, least = cost;
   }
   const i64 each = (tiles + best - 1) / best;
