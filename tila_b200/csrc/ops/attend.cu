@@ -580,9 +580,9 @@ struct Plan {
 // Where the narrow form follows (`narrow_bytes`, half of what the longest sequences
 // would be), it starts beside the wide form on the multiprocessors that are left,
 // which fetch about 58 GB/s each, 6.7 TB/s in all, and takes 8 us beside that: the
-// split that ends both first (of those that give the wide form 64 multiprocessors at
+// split that ends both first (of those that give the wide form 48 multiprocessors at
 // least, since lengths may be far below what the table could hold).  128 sequences of up
-// to 4096 own tokens on 32768 shared ones: 207 us so, 237 us with the wide form on
+// to 4096 own tokens on 32768 shared ones: 199 us so, 237 us with the wide form on
 // every multiprocessor first; 64 of up to 1024 on 8192: 40 and 46 us.
 int wide_chunk_of(i64 keys, i64 blocks, double narrow_bytes, int &chunks) {
   const i64 tiles = (keys + 127) / 128;
@@ -590,7 +590,7 @@ int wide_chunk_of(i64 keys, i64 blocks, double narrow_bytes, int &chunks) {
   i64 best = 0;
   double least = 0;
   for (i64 n = 1; n <= most; ++n) {
-    if (narrow_bytes > 0 && blocks * n < 64 && n < most) continue;
+    if (narrow_bytes > 0 && blocks * n < 48 && n < most) continue;
     const double wide = ((blocks * n + kSms - 1) / kSms) * (9.5e-6 + 2.1e-6 * ((tiles + n - 1) / n));
     const double beside = std::min(6.7e12, 58e9 * std::max<i64>(0, kSms - blocks * n));
     const double left = std::max(0., narrow_bytes - beside * wide);
