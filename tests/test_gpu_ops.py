@@ -386,6 +386,61 @@ def test_attend_leaves_rows_behind_the_last_sequence():
     check_attend((q, kc, vc, table, lens, pages, offsets), counts, lengths, 40)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("counts,lengths,prefix,heads,kv,dim", [
+    ([6, 2], [40, 2], 30, 2, 2, 64), ([3], [20], 0, 4, 1, 128), ([150, 40], [300, 40], 64, 4, 2, 128), ([200], [210], 0, 1, 1, 64),
+    ([5, 9], [100, 9], 20, 2, 1, 256), ([70, 3], [1000, 200], 0, 4, 2, 80),
+])
+def test_attend_odd_values_reach_only_who_sees_them(dtype, counts, lengths, prefix, heads, kv, dim):
+    """Keys and values of new tokens that are infinite or not a number: tokens
+    before them keep their results, tokens from them on show them."""
+    case = paged(7, counts, lengths, prefix, heads, kv, dim, 16, dtype)
+    q, kc, vc, table, lens, pages, offsets = case
+    args = dict(prefix_pages=pages, prefix_length=prefix, query_offsets=offsets, max_queries=max(counts))
+    want, _, tol, _ = attend(q, kc, vc, table, lens, pages, prefix, counts, dim ** -0.5)
+    group = heads // kv
+
+    def as_before(got, rows):
+        return bool(((got.double() - want).abs() <= tol)[rows].all())
+
+    def place(b, token):                                             # of a sequence's own token in the cache
+        return int(table[b, token // 16]), token % 16
+
+    b, n = 0, counts[0]
+    at = lengths[0] - n // 2                                         # the middle of the new tokens
+    first = n - n // 2                                               # the first query that sees it
+    page, row = place(b, at)
+    old = vc[page, row].clone()
+    for value, d in ((float("nan"), 3), (float("inf"), 0), (float("-inf"), dim - 1)):
+        vc[page, row, kv - 1, d] = value
+        got = ops.attend_shared_prefix(q, kc, vc, table, lens, **args)
+        vc[page, row] = old
+        heads_of = slice((kv - 1) * group, None)
+        touched = torch.zeros_like(got, dtype=torch.bool)
+        touched[first:n, heads_of, d] = True
+        assert as_before(got, ~touched)
+        seen = got[first:n, heads_of, d]
+        assert bool((seen.isnan() if value != value else seen == value).all())
+    # both infinities in one column, the second one token later: a number, then one, then none
+    if n >= 4:
+        vc[page, row, 0, 1], (p2, r2) = float("inf"), place(b, at + 1)
+        keep = vc[p2, r2].clone()
+        vc[p2, r2, 0, 1] = float("-inf")
+        got = ops.attend_shared_prefix(q, kc, vc, table, lens, **args)
+        vc[page, row], vc[p2, r2] = old, keep
+        assert bool((got[first, :group, 1] == float("inf")).all()) and bool(got[first + 1:n, :group, 1].isnan().all())
+        assert as_before(got, slice(0, first)) and as_before(got, slice(n, None))
+    # a key that is not a number: rows that see it are lost, the others are not
+    old = kc[page, row].clone()
+    kc[page, row, 0, 2] = float("nan")
+    got = ops.attend_shared_prefix(q, kc, vc, table, lens, **args)
+    kc[page, row] = old
+    touched = torch.zeros_like(got, dtype=torch.bool)
+    touched[first:n, :group] = True
+    assert as_before(got, ~touched) and bool(got[first:n, :group].isnan().all())
+    ops.check_errors()
+
+
 def test_attend_query_strides():
     counts, lengths = [1, 1, 1], [20, 9, 33]
     q, kc, vc, table, lens, pages, _ = paged(8, counts, lengths, 40, 6, 2, 64, 16, F16)

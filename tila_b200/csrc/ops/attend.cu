@@ -263,6 +263,8 @@ __device__ __forceinline__ void narrow_block(const AttendParams &p, const tila::
       limit[t][e] = row < it.rows ? min(it.end, causal ? it.limit0 + row / p.group : it.limit0) : 0;
     }
 
+  // keys up to here are seen by all rows or by none
+  const int sees_least = causal && it.limit0 + it.row0 / p.group < it.end ? it.limit0 + it.row0 / p.group : 0x7fffffff;
   float o[NT][DP / 16][4], m[NT][2], l[NT][2];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -303,11 +305,11 @@ __device__ __forceinline__ void narrow_block(const AttendParams &p, const tila::
       }
     }
     u32 pf[NT][2];
-    float scale[NT][2];
+    float scale[NT][2], weights[NT][2][2];                   // [key g, key g + 8][row]
     bool moved = false;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      float w[2][2];                                         // [key g, key g + 8][row]
+      float (&w)[2][2] = weights[t];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
@@ -342,7 +344,32 @@ __device__ __forceinline__ void narrow_block(const AttendParams &p, const tila::
           o[t][n][3] *= scale[t][1];
         }
     }
-    {
+    // Where some rows see keys that others do not, a value that is no number must
+    // not reach the others through its weight of 0: such slices (new tokens' own,
+    // and of them only those with such values) are summed one key at a time.
+    bool odd = false;
+    if (key0 + kSlice > sees_least)
+      for (int i = lane; i < kSlice * (DP / 8); i += 32)
+        odd = odd || any_odd<T>(*reinterpret_cast<const uint4 *>(ring + (step % kStages) * N::kStage + N::kValues + i * 16));
+    if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll 1
+      for (int j = 0; j < kSlice; ++j) {
+        const T *v = reinterpret_cast<const T *>(ring + (step % kStages) * N::kStage + N::kValues);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float w = Elem<T>::get(Elem<T>::put(
+                __shfl_sync(0xffffffffu, j < 8 ? weights[t][0][e] : weights[t][1][e], (j & 7) * 4 + c)));
+            if (key0 + j < limit[t][e])
+#pragma unroll
+              for (int n = 0; n < DP / 16; ++n) {
+                o[t][n][e] += w * Elem<T>::get(v[piece(j, n * 2) / 2 + g]);
+                o[t][n][2 + e] += w * Elem<T>::get(v[piece(j, n * 2 + 1) / 2 + g]);
+              }
+          }
+      }
+    } else {
       const int r = (lane & 7) + ((lane >> 4) << 3), ch = (lane >> 3) & 1;
 #pragma unroll
       for (int n = 0; n < DP / 16; ++n) {

@@ -72,6 +72,15 @@ __device__ __forceinline__ int own_chunk(const AttendParams &p, int length) {
   return max(p.own_least, (each + p.own_unit - 1) & ~(p.own_unit - 1));
 }
 
+// Whether any of 8 elements is infinite or not a number: its exponent bits are all
+// ones, and adding their lowest carries into the sign's place.
+template <typename T> __device__ __forceinline__ bool any_odd(uint4 x) {
+  constexpr u32 kLowest = __is_same(T, __half) ? 0x04000400u : 0x00800080u, kExponent = 0x80008000u - kLowest;
+  const u32 carried = ((x.x & kExponent) + kLowest) | ((x.y & kExponent) + kLowest) | ((x.z & kExponent) + kLowest) |
+                      ((x.w & kExponent) + kLowest);
+  return (carried & 0x80008000u) != 0;
+}
+
 __device__ __forceinline__ void split_key(const AttendParams &p, int key, int &page, int &row) {
   if (p.page_shift >= 0) {
     page = key >> p.page_shift;

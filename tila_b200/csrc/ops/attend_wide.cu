@@ -9,7 +9,11 @@
 //   * a copy warp that streams tiles of 128 keys, then of their values, through
 //     one ring in shared memory: a TMA box for each page and each 64 elements of
 //     the heads, so that a tile takes its pages from anywhere in the pool;
-//   * an MMA warp that issues S = Q K^T and O += P V.
+//   * an MMA warp that issues S = Q K^T and O += P V;
+//   * two warps that look through the values of the tiles where some rows see keys
+//     that others do not (new tokens): a value that is no number must not reach the
+//     others through its weight of 0, so it is cleared there and put into the rows
+//     that see it at the end.
 //
 // With more than 128 rows the warpgroups hold two row tiles and share every
 // tile of keys (half the traffic from L2, which at 128 rows a tile would bound:
@@ -31,6 +35,8 @@
 
 #include "attend.cuh"
 #include "attend_wide.cuh"
+
+#include <type_traits>
 
 namespace tila_ops {
 namespace {
@@ -85,6 +91,14 @@ __device__ __forceinline__ bool warp_wait(u64 *bar, u32 parity, u32 *err, u32 wh
   return __all_sync(0xffffffffu, tila::mbar_wait(bar, parity, err, where, dead));
 }
 
+// First key of the tiles looked through whose value at an element is not a number,
+// +inf, -inf.
+constexpr int kNever = 0x7fffffff;
+template <int DP> struct OddValues {
+  int first[3][DP];
+  int any;
+};
+
 // A row of O from tensor memory (zeros where nothing was added to it) times `mine`,
 // plus `other` times the partner's row, to shared memory.
 template <int DP>
@@ -108,21 +122,35 @@ __device__ __forceinline__ void write_row(u32 o_col, bool any, float mine, float
   }
 }
 
+// The values cleared from the tiles, into the row of a token that sees `limit` keys.
+template <int DP>
+__device__ __noinline__ void put_odd(float *dst, const OddValues<DP> &odd, int limit) {
+  for (int i = 0; i < DP; ++i) {
+    const bool nan = odd.first[0][i] < limit, up = odd.first[1][i] < limit, down = odd.first[2][i] < limit;
+    if (nan || (up && down)) dst[i] = __int_as_float(0x7fffffff);
+    else if (up || down) dst[i] += up ? __builtin_huge_valf() : -__builtin_huge_valf();
+  }
+}
+
 struct Barriers {
   u64 full[9], empty[9];
   u64 scores[2];      // S of a warpgroup's tile is there (and P V of its tile before)
   u64 taken[2];       // S has been read (kEarly)
   u64 weights[2];     // P is in tensor memory
   u64 summed[2];      // P V of a warpgroup's tile is done (kEarly)
+  u64 loaded[4], checked[4];   // values of the n-th tile that rows see differently: there, looked through
   u64 queries, done;
 };
 
-template <typename T, int DP>
+// `kOwn`: sequences' own tokens, each of which sees its own number of keys; else the
+// shared prefix, which all rows of the batch see.
+template <typename T, int DP, bool kOwn>
 __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMap &kmap, const TensorMap &vmap,
                                            const WideGrid &grid) {
   using W = Wide<DP>;
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) Barriers bars;
+  __shared__ OddValues<kOwn ? DP : 1> odd;
   __shared__ u32 tmem_slot;
   __shared__ volatile int dead;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -132,10 +160,9 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
   i64 token0;
   int rows, head, begin, end, limit0, slot, pair;
   const i32 *pages;
-  bool causal = false;
   {
     int i = blockIdx.x;
-    if (grid.prefix) {
+    if constexpr (!kOwn) {
       pair = i % grid.pairs;
       i /= grid.pairs;
       head = i % p.kv_heads;
@@ -165,7 +192,6 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
       const int last = min((pair + 1) * 2 * kTile, rows) - 1;
       end = min(begin + keys, limit0 + last / p.group);
       pages = p.table + b * p.table_stride;
-      causal = true;
     }
   }
   const int row0 = pair * 2 * kTile;
@@ -173,6 +199,10 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
   const bool shared_rows = rows - row0 <= kTile;     // one row tile: the warpgroups take tiles in turn
   const int tiles = end > begin ? (end - begin + kTile - 1) / kTile : 0;
   const int ahead = shared_rows ? 2 : 1;             // S is issued so many tiles ahead of P V
+  // tiles from here on hold keys that some rows see and others do not (3 at most: a
+  // block's tokens are 256 or fewer)
+  const int least = kOwn ? limit0 + row0 / p.group : end;
+  const int mixed = least >= end ? tiles : max(0, least - begin) / kTile;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < W::kStages; ++i) {
@@ -185,11 +215,18 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
       tila::mbar_init(&bars.taken[i], kTile);
       tila::mbar_init(&bars.summed[i], 1);
     }
+    for (int i = 0; i < 4; ++i) {
+      tila::mbar_init(&bars.loaded[i], 1);
+      tila::mbar_init(&bars.checked[i], 2);
+    }
     tila::mbar_init(&bars.queries, 2 * kTile);
     tila::mbar_init(&bars.done, 1);
     dead = 0;
+    odd.any = 0;
     tila::mbar_fence_init();
   }
+  if (kOwn && warp >= 10 && mixed < tiles)
+    for (int i = threadIdx.x - 320; i < 3 * DP; i += 64) odd.first[i / DP][i % DP] = kNever;
   if (warp == 9) tila::tmem_alloc(&tmem_slot, 512);
   tila::tc_fence_before();
   __syncthreads();
@@ -254,7 +291,7 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
     const int n_tiles = static_cast<int>(uniform(tiles)), key_end = static_cast<int>(uniform(end));
     const bool turns = uniform(shared_rows) != 0;                 // the warpgroups take tiles in turn
     const bool second = uniform(rows - row0 > kTile) != 0;        // the second row tile exists
-    const int lead = turns ? 2 : 1;
+    const int lead = turns ? 2 : 1, first_mixed = static_cast<int>(uniform(mixed));
     constexpr u32 kFormat = __is_same(T, __half) ? 0u : (1u << 7) | (1u << 10);
     constexpr u32 kScoresDesc = tila::idesc_f16_f32(128, 128, 0, 0) | kFormat;
     constexpr u32 kValuesDesc = tila::idesc_f16_f32(128, DP, 0, 1) | kFormat;
@@ -296,6 +333,7 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
       const int keys = more ? item++ : 0;
       ok = wait_full(values) && (!more || wait_full(keys));
       if (!ok) break;
+      if (kOwn && j >= first_mixed && elected()) tila::mbar_arrive(&bars.loaded[j - first_mixed]);
       const int seen = min(kTile, key_end - (begin + j * kTile));
       const int steps = static_cast<int>(uniform((seen + 15) >> 4));
       if (seen & 15) {
@@ -340,6 +378,36 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
     }
     if (ok && n_tiles > 0 && elected()) tila::mma_commit(&bars.done);
     __syncwarp();
+  } else if (warp >= 10) {
+    if constexpr (kOwn) {
+      // ---- values of mixed tiles -----------------------------------------------------
+      bool ok = true;
+      for (int j = mixed; ok && j < tiles; ++j) {
+        const int item = first_keys + j + min(j, tiles - first_keys);
+        unsigned char *v = smem + W::kRing + (item % W::kStages) * W::kTileBytes;
+        // (not the ring's own barrier, whose phases this warp does not follow)
+        ok = warp_wait(&bars.loaded[j - mixed], 0, p.err, __LINE__, dead_ptr);
+        const int seen = min(kTile, end - (begin + j * kTile));
+        for (int i = threadIdx.x - 320; ok && i < seen * (DP / 8); i += 64) {
+          const int r = i / (DP / 8), c = i % (DP / 8);
+          unsigned char *at = v + (c / 8) * kHalf + r * 128 + (((c % 8) ^ (r & 7)) << 4);
+          if (any_odd<T>(*reinterpret_cast<const uint4 *>(at))) {
+            T *e = reinterpret_cast<T *>(at);
+  #pragma unroll 1
+            for (int k = 0; k < 8; ++k) {
+              const float x = Elem<T>::get(e[k]);
+              if (fabsf(x) < __builtin_huge_valf()) continue;
+              atomicMin(&odd.first[x != x ? 0 : x > 0.f ? 1 : 2][c * 8 + k], begin + j * kTile + r);
+              odd.any = 1;
+              e[k] = Elem<T>::put(0.f);
+            }
+          }
+        }
+        tila::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) tila::mbar_arrive(&bars.checked[j - mixed]);
+      }
+    }
   } else if (warp < 8) {
     // ---- softmax: warpgroup w, one row a thread ------------------------------------
     tila::reg_alloc<216>();
@@ -347,7 +415,7 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
     const int row = row0 + (shared_rows ? 0 : w * kTile) + r;
     const bool valid = row < rows;
     const int token = valid ? row / p.group : 0;
-    const int limit = !valid ? 0 : causal ? limit0 + token : limit0;
+    const int limit = !valid ? 0 : kOwn ? limit0 + token : limit0;
     const int out_head = head * p.group + (valid ? row - token * p.group : 0);
     if (!shared_rows || w == 0) {
       // the warp's 32 rows of queries, whole rows at a time, swizzled as TMA would
@@ -461,6 +529,11 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
       sum += tila::lo2(both) + tila::hi2(both);
       tila::tmem_wait_st();
       tila::tc_fence_before();
+      if (kOwn && j >= mixed) {
+        // P V waits for the weights, and they for the look through the values
+        ok = warp_wait(&bars.checked[j - mixed], 0, p.err, __LINE__, dead_ptr);
+        if (!ok) break;
+      }
       tila::mbar_arrive(&bars.weights[w]);
     }
 
@@ -490,6 +563,8 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
     }
     if (!shared_rows || w == 0) {
       write_row<DP>(o_col, turn > 0, mine, other, shared_rows ? partner : nullptr, staged);
+      if constexpr (kOwn)
+        if (odd.any) put_odd<DP>(staged, odd, limit);
       const int at = valid && ok ? static_cast<int>((token0 + token) * p.heads + out_head) : -1;
       const i64 first = slot * p.tokens * p.heads;
       if (at >= 0) {
@@ -537,12 +612,12 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
 
 // The first block ends after the previous kernel, beside which this one may run, so
 // that what waits for this grid waits for both.
-template <typename T, int DP>
+template <typename T, int DP, bool kOwn>
 __global__ void __launch_bounds__(kThreads, 1)
 attend_wide_kernel(const __grid_constant__ AttendParams p, const __grid_constant__ TensorMap kmap,
                    const __grid_constant__ TensorMap vmap, const __grid_constant__ WideGrid grid) {
   tila::grid_dep_release();
-  wide_block<T, DP>(p, kmap, vmap, grid);
+  wide_block<T, DP, kOwn>(p, kmap, vmap, grid);
   if (blockIdx.x == 0 && threadIdx.x == 0) tila::grid_dep_wait();
 }
 
@@ -557,19 +632,19 @@ int encode(TensorMap *map, const tila_attend_args &a, int rows, u64 address, con
   return tila_encode_tensor_map(map, a.dtype == TILA_F16 ? 6 : 9, 4, address, dims, strides, box, 3, log, cap);
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool kOwn>
 cudaError_t launch_form(const AttendParams &p, const TensorMap &k, const TensorMap &v, const WideGrid &grid,
                         unsigned blocks, bool after_previous, cudaStream_t stream) {
   static const cudaError_t registers = [] {
     cudaFuncAttributes attr;
-    const cudaError_t e = cudaFuncGetAttributes(&attr, attend_wide_kernel<T, DP>);
+    const cudaError_t e = cudaFuncGetAttributes(&attr, attend_wide_kernel<T, DP, kOwn>);
     return e != cudaSuccess ? e : attr.numRegs == kLaunchRegisters ? cudaSuccess : cudaErrorLaunchOutOfResources;
   }();
   if (registers != cudaSuccess) return registers;
-  cudaError_t e = cudaFuncSetAttribute(attend_wide_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  cudaError_t e = cudaFuncSetAttribute(attend_wide_kernel<T, DP, kOwn>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        Wide<DP>::kBytes);
   if (e != cudaSuccess) return e;
-  return launch_kernel(attend_wide_kernel<T, DP>, blocks, kThreads, Wide<DP>::kBytes, stream, after_previous, p, k, v,
+  return launch_kernel(attend_wide_kernel<T, DP, kOwn>, blocks, kThreads, Wide<DP>::kBytes, stream, after_previous, p, k, v,
                        grid);
 }
 
@@ -602,16 +677,21 @@ int launch_wide(const tila_attend_args &a, const AttendParams &p, bool prefix, b
   if (st != TILA_OK) return st;
   WideGrid grid{};
   const i64 rows = static_cast<i64>(prefix ? (a.query_offsets == 0 ? a.batch : a.tokens) : p.max_queries) * p.group;
-  grid.prefix = prefix;
   grid.pairs = static_cast<int>((rows + 2 * kTile - 1) / (2 * kTile));
   const i64 blocks = static_cast<i64>(grid.pairs) * p.kv_heads *
                      (prefix ? p.prefix_chunks : static_cast<i64>(p.own_chunks) * p.batch);
   if (blocks > 0x7fffffff) return fail(TILA_ERR_ARGUMENT, log, cap, "tila_attend_shared_prefix: too many blocks");
   const unsigned n = static_cast<unsigned>(blocks);
-  const auto launch = [&](auto form) { return form(p, k, v, grid, n, after_previous, stream); };
-  const cudaError_t e = a.dtype == TILA_F16
-                            ? (a.dim <= 64 ? launch(launch_form<__half, 64>) : launch(launch_form<__half, 128>))
-                            : (a.dim <= 64 ? launch(launch_form<__nv_bfloat16, 64>) : launch(launch_form<__nv_bfloat16, 128>));
+  const auto launch = [&](auto type, auto own) {
+    using T = decltype(type);
+    constexpr bool kOwn = decltype(own)::value;
+    return a.dim <= 64 ? launch_form<T, 64, kOwn>(p, k, v, grid, n, after_previous, stream)
+                       : launch_form<T, 128, kOwn>(p, k, v, grid, n, after_previous, stream);
+  };
+  const auto of_type = [&](auto own) {
+    return a.dtype == TILA_F16 ? launch(__half{}, own) : launch(__nv_bfloat16{}, own);
+  };
+  const cudaError_t e = prefix ? of_type(std::false_type{}) : of_type(std::true_type{});
   return launch_status(e, "tila_attend_shared_prefix", log, cap);
 }
 

@@ -6,7 +6,6 @@
 namespace tila_ops {
 
 struct WideGrid {
-  int prefix;        // the shared prefix (rows of all sequences), else own tokens
   int pairs;         // pairs of row tiles of 128
 };
 

@@ -245,9 +245,9 @@ def attend_shared_prefix(q, k_cache, v_cache, page_table, lengths, *, prefix_pag
     ``return_lse`` also the log of each row's sum of exponentials, float32 (tokens,
     heads).  Scores, weights' sums and results are kept in 32 bits; the weights are
     rounded to the values' type for their product.  The same call gives the same
-    bits.  Values that a new token may not see yet must still be finite, as a
-    weight of 0 is multiplied with them; what lies behind a sequence's length,
-    or in pages that it does not reach, may be anything.
+    bits.  What a token does not see may be anything, infinities and NaN included:
+    new tokens behind it, cache rows behind a sequence's length, pages that no
+    sequence reaches.
     """
     return _ops.attend_shared_prefix(q, k_cache, v_cache, page_table, lengths, prefix_pages, prefix_length, query_offsets,
                                      max_queries, scale, out, bool(return_lse), max_length)
