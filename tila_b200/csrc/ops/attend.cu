@@ -740,8 +740,8 @@ cudaError_t launch_narrow(const Plan &r, const tila::TensorMap &k, const tila::T
   const i64 own_items = r.own_wide ? 0 : static_cast<i64>(r.own_tiles) * r.p.kv_heads * r.p.own_chunks * r.p.batch;
   if (prefix_items + own_items == 0) return cudaSuccess;
   if (prefix_items + own_items > 0x7fffffff) return cudaErrorInvalidValue;
-  const auto kernel = attend_narrow_kernel<T, DP, NT, kTma>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Narrow<DP>::kBytes);
+  constexpr auto kernel = attend_narrow_kernel<T, DP, NT, kTma>;
+  const cudaError_t e = allow_shared_memory<kernel>(Narrow<DP>::kBytes);
   if (e != cudaSuccess) return e;
   return launch_kernel(kernel, static_cast<unsigned>(prefix_items + own_items), kWarps * 32, Narrow<DP>::kBytes,
                        stream, r.prefix_wide || r.own_wide, r.p, k, v, static_cast<int>(prefix_items), r.prefix_tiles, r.own_tiles);

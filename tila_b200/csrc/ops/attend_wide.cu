@@ -641,8 +641,7 @@ cudaError_t launch_form(const AttendParams &p, const TensorMap &k, const TensorM
     return e != cudaSuccess ? e : attr.numRegs == kLaunchRegisters ? cudaSuccess : cudaErrorLaunchOutOfResources;
   }();
   if (registers != cudaSuccess) return registers;
-  cudaError_t e = cudaFuncSetAttribute(attend_wide_kernel<T, DP, kOwn>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       Wide<DP>::kBytes);
+  const cudaError_t e = allow_shared_memory<attend_wide_kernel<T, DP, kOwn>>(Wide<DP>::kBytes);
   if (e != cudaSuccess) return e;
   return launch_kernel(attend_wide_kernel<T, DP, kOwn>, blocks, kThreads, Wide<DP>::kBytes, stream, after_previous, p, k, v,
                        grid);

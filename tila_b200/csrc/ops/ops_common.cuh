@@ -9,6 +9,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 
@@ -60,6 +61,19 @@ cudaError_t launch_kernel(void (*kernel)(P...), unsigned blocks, unsigned thread
   cfg.attrs = &attr;
   cfg.numAttrs = after_previous ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// Lets `kernel` have `bytes` of dynamic shared memory, once for each device.
+template <auto kernel> cudaError_t allow_shared_memory(int bytes) {
+  static std::atomic<u64> allowed{0};
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  const u64 bit = device < 64 ? u64{1} << device : 0;
+  if (allowed.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) allowed.fetch_or(bit, std::memory_order_relaxed);
+  return e;
 }
 
 template <typename T> struct Elem;
