@@ -217,7 +217,8 @@ enum { TILA_F32 = 0, TILA_F16 = 1, TILA_BF16 = 2 };
 #define TILA_ROWS_PAGED 4u       /* dst is a paged pool, addressed through the slots */
 #define TILA_ROWS_WEIGHT_F32 8u  /* weight has 32-bit elements (else the rows' type) */
 
-/* One tensor of rows: batch x tokens x heads rows of `dim` elements. */
+/* One tensor of rows: batch x tokens x heads rows of `dim` elements.  Strides of
+ * tokens and heads are below 2^32 elements. */
 typedef struct tila_op_rows {
   uint64_t src, dst, weight, grad;  /* grad: the result's gradient (backward only) */
   int64_t src_stride[3];            /* batch, token, head */

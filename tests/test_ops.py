@@ -183,14 +183,14 @@ def workspace(entry, args):
     return f(args)
 
 
-def rotary_args(rows=1, flags=FLAG_ROTATE, **change):
+def rotary_args(rows=1, flags=FLAG_ROTATE, token_stride=128, **change):
     """tila_rotary_args with addresses that nothing reads (the call is refused)."""
     names = ("size", "dtype", "batch", "tokens", "dim", "rotary", "interleaved", "inverse", "amplitude", "eps",
              "positions", "step_b", "step_t", "inv_freq", "slots", "slot_step", "num_slots", "page", "index64",
              "num_rows", "reserved", "err", "stream", "workspace", "workspace_bytes", "dw0", "dw1")
     head = dict(zip(names, (ROTARY_BYTES, 0, 1, 4, 64, 64, 0, 0, 1.0, 0.0, 4096, 0, 1, 4096, 0, 0, 0, 0, 1, rows, 0,
                             0, 0, 0, 0, 0, 0))) | change
-    row = ROWS.pack(4096, 4096, 0, 0, 0, 128, 64, 0, 128, 64, 0, 0, 0, 2, flags)
+    row = ROWS.pack(4096, 4096, 0, 0, 0, token_stride, 64, 0, 128, 64, 0, 0, 0, 2, flags)
     return HEAD.pack(*(head[n] for n in names)) + row * rows + bytes(ROWS.size) * (3 - rows)
 
 
@@ -203,6 +203,7 @@ def rotary_args(rows=1, flags=FLAG_ROTATE, **change):
     ("tila_rotary_rows", rotary_args(rotary=63)),
     ("tila_rotary_rows", rotary_args(positions=0)),
     ("tila_rotary_rows", rotary_args(num_rows=4)),
+    ("tila_rotary_rows", rotary_args(token_stride=1 << 32)),
     ("tila_rotary_rows", rotary_args(flags=FLAG_NORM)),
     ("tila_rotary_rows", rotary_args(flags=FLAG_PAGED)),
     ("tila_rotary_norm_backward", rotary_args()),

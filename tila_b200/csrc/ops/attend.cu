@@ -34,16 +34,6 @@ constexpr int kSlice = 16;                 // keys of one warp's step
 constexpr int kStep = kWarps * kSlice;     // keys of one block's step
 constexpr int kStages = 2;                 // 64 KB a block at 128 elements: three blocks a multiprocessor
 
-template <typename T> __device__ __forceinline__ u32 pack2(float lo, float hi);
-template <> __device__ __forceinline__ u32 pack2<__half>(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const u32 *>(&h);
-}
-template <> __device__ __forceinline__ u32 pack2<__nv_bfloat16>(float lo, float hi) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const u32 *>(&h);
-}
-
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], const u32 (&a)[4], u32 b0, u32 b1) {
   if constexpr (sizeof(T) == 2 && __is_same(T, __half))
@@ -329,8 +319,8 @@ __device__ __forceinline__ void narrow_block(const AttendParams &p, const tila::
         l[t][e] = l[t][e] * scale[t][e] + (w[0][e] + w[1][e]);
       }
       // P^T as the B operand: keys in rows there, so each 8x8 block turned around
-      pf[t][0] = transposed(pack2<T>(w[0][0], w[0][1]));
-      pf[t][1] = transposed(pack2<T>(w[1][0], w[1][1]));
+      pf[t][0] = transposed(pack_pair<T>(w[0][0], w[0][1]));
+      pf[t][1] = transposed(pack_pair<T>(w[1][0], w[1][1]));
     }
     // the sums follow the maximum only when it moved
     if (__any_sync(0xffffffffu, moved)) {
@@ -548,8 +538,8 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
     const int d = lane * 4 + i * 4 * L;
     if (d < p.dim) {
       if (p.out_vectors)
-        *reinterpret_cast<uint2 *>(out + d) = make_uint2(pack2<T>(acc[i * 4] * inverse, acc[i * 4 + 1] * inverse),
-                                                         pack2<T>(acc[i * 4 + 2] * inverse, acc[i * 4 + 3] * inverse));
+        *reinterpret_cast<uint2 *>(out + d) = make_uint2(pack_pair<T>(acc[i * 4] * inverse, acc[i * 4 + 1] * inverse),
+                                                         pack_pair<T>(acc[i * 4 + 2] * inverse, acc[i * 4 + 3] * inverse));
       else
 #pragma unroll
         for (int e = 0; e < 4; ++e) out[d + e] = Elem<T>::put(acc[i * 4 + e] * inverse);

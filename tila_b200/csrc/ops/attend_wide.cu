@@ -521,7 +521,7 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
           const u64 x = tila::fma2(tila::pk2(s[k], s[k + 1]), scale_2, base_2);
           const float a = tila::exp2_ftz(tila::lo2(x)), b = tila::exp2_ftz(tila::hi2(x));
           sums[i & 1] = tila::add2(sums[i & 1], tila::pk2(a, b));
-          packed[i] = __uint_as_float(wide_pack<T>(a, b));
+          packed[i] = __uint_as_float(pack_pair<T>(a, b));
         }
         tila::tmem_st32(p_col + half * 32, packed);
       }
@@ -593,7 +593,7 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
             const float4 x = *reinterpret_cast<const float4 *>(from + i * W::kRowFloats);
             T *to = static_cast<T *>(p.out) + row_at + lane * 4;
             if (p.out_vectors) {
-              *reinterpret_cast<uint2 *>(to) = make_uint2(wide_pack<T>(x.x, x.y), wide_pack<T>(x.z, x.w));
+              *reinterpret_cast<uint2 *>(to) = make_uint2(pack_pair<T>(x.x, x.y), pack_pair<T>(x.z, x.w));
             } else {
               to[0] = Elem<T>::put(x.x);
               to[1] = Elem<T>::put(x.y);

@@ -9,14 +9,6 @@ struct WideGrid {
   int pairs;         // pairs of row tiles of 128
 };
 
-template <typename T> __device__ __forceinline__ u32 wide_pack(float lo, float hi);
-template <> __device__ __forceinline__ u32 wide_pack<__half>(float lo, float hi) { return tila::pack_f16x2(lo, hi); }
-template <> __device__ __forceinline__ u32 wide_pack<__nv_bfloat16>(float lo, float hi) {
-  u32 r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-
 // Whether the caches' strides allow tensor maps; and whether pages and head size
 // also fit the wide form: boxes of whole pages, or of 128 rows of one.
 bool tma_possible(const tila_attend_args &a);

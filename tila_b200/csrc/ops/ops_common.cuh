@@ -90,6 +90,22 @@ template <> struct Elem<__nv_bfloat16> {
   static __device__ __forceinline__ __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
 };
 
+// Two neighbouring elements as two floats, and back (each rounded to nearest).
+template <typename T> __device__ __forceinline__ float2 unpack_pair(u32 w);
+template <> __device__ __forceinline__ float2 unpack_pair<__half>(u32 w) {
+  return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+template <> __device__ __forceinline__ float2 unpack_pair<__nv_bfloat16>(u32 w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <typename T> __device__ __forceinline__ u32 pack_pair(float lo, float hi);
+template <> __device__ __forceinline__ u32 pack_pair<__half>(float lo, float hi) { return tila::pack_f16x2(lo, hi); }
+template <> __device__ __forceinline__ u32 pack_pair<__nv_bfloat16>(float lo, float hi) {
+  u32 r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
 // V elements moved by one access.
 template <typename T, int V> struct __align__(sizeof(T) * V) Vec { T e[V]; };
 

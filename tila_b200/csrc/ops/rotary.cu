@@ -11,24 +11,23 @@
 // stored.
 //
 // Bound by memory: a row is read once and written once (with norms, at 16 bits, the
-// instructions come close: 16 elements of a lane are 64 bytes and about 200
-// instructions).  A block takes a few tokens with all their heads, of every tensor of
-// the call, so that the sines of a token are computed once and shared through shared
-// memory, and so few or many that all blocks are whole waves of the GPU.  A row is
-// spread over as many lanes as it has units; a unit is the two V-element vectors that
-// hold both halves of V pairs, so that neither layout moves data between
+// instructions come close).  A block takes a few tokens with all their heads, of every
+// tensor of the call, so that the sines of a token are computed once and shared
+// through shared memory, and so few or many that all blocks are whole waves of the
+// GPU.  A row is spread over as many lanes as it has units; a unit is the two V-element
+// vectors that hold both halves of V pairs, so that neither layout moves data between
 // lanes, and V elements are one 16-byte access where sizes, strides and
 // addresses allow it.  Rows are taken tensor by tensor, so that pointers, flags and
 // weights stay where they are from row to row; a row is loaded one ahead, and no load
-// is conditional, so that all of a row's are in flight together.  Arithmetic is on
-// pairs of 32-bit floats.
+// is conditional, so that all of a row's are in flight together.  Arithmetic and
+// conversions are on pairs of floats.
 //
-// Measured (B200): rotate gradient of 4 x 2048 x 32 heads x 128, 32 bits: 46 us, 5.8
-// TB/s; norm_rotate of 8192 tokens x 40 heads x 128, bf16: 40 us, 4.2 TB/s, its
-// gradient 76 us; append of 16384 tokens with 32 queries heads and 8 key heads 77 us, 5.2 TB/s.
-// Tried and not kept: a warp for each token with sines and weights in registers
-// (norms 57 us), and the same with rows through a ring in shared memory (norms 41 us,
-// the gradient 70 us, but 107 us for the append and 7 us for 64 tokens).
+// Measured (B200): rotate gradient of 4 x 2048 tokens x 32 heads x 128, 32 bits: 46 us,
+// 5.8 TB/s; norm_rotate of 8192 tokens x 40 heads x 128, bf16: 35 us, 4.8 TB/s, its
+// gradient 58 us; append of 16384 tokens with 32 query and 8 key heads 72 us, 5.6 TB/s.
+// Tried and not kept: a warp for each token with sines and weights in registers (norms
+// 57 us where this form took 40), and the same with rows through a ring in shared
+// memory (norms 41 us, but 107 us for the append and 7 us for 64 tokens).
 
 #include "ops_common.cuh"
 
@@ -44,6 +43,8 @@ struct Rows {
   const void *weight;
   const void *grad;
   i64 src_stride[3], dst_stride[3], grad_stride[3];
+  // of tokens and heads, which fit 32 bits: a row's place is two multiplications
+  u32 src_token, src_head, dst_token, dst_head, grad_token, grad_head;
   int heads;
   u32 flags;
 };
@@ -73,6 +74,10 @@ struct Params {
   u32 *err;
   float *partial;        // backward: blocks x 2 x dim sums of the weights' gradients
 };
+
+__device__ __forceinline__ u64 row_at(int t, u32 token, int h, u32 head) {
+  return static_cast<u64>(static_cast<u32>(t)) * token + static_cast<u64>(static_cast<u32>(h)) * head;
+}
 
 __device__ __forceinline__ i64 index_at(const void *p, i64 i, int wide) {
   return wide ? static_cast<const i64 *>(p)[i] : static_cast<i64>(static_cast<const i32 *>(p)[i]);
@@ -126,8 +131,14 @@ __device__ __forceinline__ void unpack(const Params &p, const Units<V, K> &u, co
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int e = 2 * i;
-      x[k][i] = tila::pk2(Elem<T>::get(e < V ? r.a[k].e[e % V] : r.b[k].e[e % V]),
-                          Elem<T>::get(e + 1 < V ? r.a[k].e[(e + 1) % V] : r.b[k].e[(e + 1) % V]));
+      if constexpr (sizeof(T) == 2 && V > 1) {
+        const u32 *words = reinterpret_cast<const u32 *>(e < V ? r.a[k].e : r.b[k].e);
+        const float2 f = unpack_pair<T>(words[e % V / 2]);
+        x[k][i] = tila::pk2(f.x, f.y);
+      } else {
+        x[k][i] = tila::pk2(Elem<T>::get(e < V ? r.a[k].e[e % V] : r.b[k].e[e % V]),
+                            Elem<T>::get(e + 1 < V ? r.a[k].e[(e + 1) % V] : r.b[k].e[(e + 1) % V]));
+      }
     }
   if (p.full) return;
 #pragma unroll
@@ -145,8 +156,14 @@ __device__ __forceinline__ void store_row(const Units<V, K> &u, T *row, const La
     Vec<T, V> a, b;
 #pragma unroll
     for (int e = 0; e < 2 * V; ++e) {
-      const float f = e & 1 ? tila::hi2(x[k][e >> 1]) : tila::lo2(x[k][e >> 1]);
-      (e < V ? a.e[e % V] : b.e[e % V]) = Elem<T>::put(f);
+      if constexpr (sizeof(T) == 2 && V > 1) {
+        if (e & 1) continue;
+        u32 *words = reinterpret_cast<u32 *>(e < V ? a.e : b.e);
+        words[e % V / 2] = pack_pair<T>(tila::lo2(x[k][e >> 1]), tila::hi2(x[k][e >> 1]));
+      } else {
+        const float f = e & 1 ? tila::hi2(x[k][e >> 1]) : tila::lo2(x[k][e >> 1]);
+        (e < V ? a.e[e % V] : b.e[e % V]) = Elem<T>::put(f);
+      }
     }
     if (u.there[k]) *reinterpret_cast<Vec<T, V> *>(row + u.first[k]) = a;
     if (u.both[k]) *reinterpret_cast<Vec<T, V> *>(row + u.second[k]) = b;
@@ -235,7 +252,9 @@ __device__ __forceinline__ float row_sum(const Params &p, const Lane<V, K> &x, c
 #pragma unroll
     for (int i = 0; i < V; ++i) pair = tila::fma2(x[k][i], y[k][i], pair);
   float s = tila::lo2(pair) + tila::hi2(pair);
-  for (int m = p.lanes >> 1; m > 0; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1)
+    if (m < p.lanes) s += __shfl_xor_sync(0xffffffffu, s, m);
   return s;
 }
 
@@ -300,7 +319,7 @@ rotary_rows_kernel(const __grid_constant__ Params p) {
       t = min(job, jobs - 1) / rows.heads;
       h = min(job, jobs - 1) - t * rows.heads;
       base = static_cast<const T *>(rows.src) + b * rows.src_stride[0] + token0 * rows.src_stride[1];
-      load_row<T, V, K>(units, base + t * rows.src_stride[1] + h * rows.src_stride[2], raw);
+      load_row<T, V, K>(units, base + row_at(t, rows.src_token, h, rows.src_head), raw);
     }
     return r;
   };
@@ -323,12 +342,11 @@ rotary_rows_kernel(const __grid_constant__ Params p) {
   while (r < last_r) {
     const Rows &rows = p.rows[r];
     const u32 flags = rows.flags;
-    const i64 src_token = rows.src_stride[1], src_head = rows.src_stride[2];
-    const i64 dst_token = rows.dst_stride[1], dst_head = rows.dst_stride[2];
+    const u32 src_token = rows.src_token, src_head = rows.src_head, dst_token = rows.dst_token, dst_head = rows.dst_head;
     const int heads = rows.heads, all = jobs, this_r = r;
     const int dt = groups / heads, dh = groups - dt * heads;
     const float *w = weights + r * p.dim;
-    T *dst = static_cast<T *>(rows.dst) + (flags & TILA_ROWS_PAGED ? 0 : b * rows.dst_stride[0] + token0 * dst_token);
+    T *dst = static_cast<T *>(rows.dst) + (flags & TILA_ROWS_PAGED ? 0 : b * rows.dst_stride[0] + token0 * rows.dst_stride[1]);
     // every warp runs the same number of times: the norm's sum is over its lanes
     for (int first = 0; first < all; first += groups) {
       const bool valid = job < all;
@@ -345,7 +363,7 @@ rotary_rows_kernel(const __grid_constant__ Params p) {
             ++t;
           }
         }
-        load_row<T, V, K>(units, base + t * src_token + h * src_head, raw);
+        load_row<T, V, K>(units, base + row_at(t, src_token, h, src_head), raw);
       } else {
         r = begin(this_r + 1);
       }
@@ -354,14 +372,14 @@ rotary_rows_kernel(const __grid_constant__ Params p) {
         times_weight<V, K>(units, w, x);
       }
       if (flags & TILA_ROWS_ROTATE) turn<V, K>(p, units, tab + 2 * at * p.half, lane, x);
-      i64 to = head * dst_head;
       bool put = valid;
+      i64 to;
       if (flags & TILA_ROWS_PAGED) {
         const i64 place = places[3 * at + this_r];
         put = put && place >= 0;
-        to += place;
+        to = place + static_cast<i64>(row_at(0, 0, head, dst_head));
       } else {
-        to += at * dst_token;
+        to = static_cast<i64>(row_at(at, dst_token, head, dst_head));
       }
       if (put) store_row<T, V, K>(units, dst + to, x);
     }
@@ -403,12 +421,13 @@ rotary_norm_backward_kernel(const __grid_constant__ Params p) {
       if (jobs == 0) break;
       int job = group, t = min(job, jobs - 1) / r.heads, h = min(job, jobs - 1) - t * r.heads;
       const int dt = groups / r.heads, dh = groups - dt * r.heads;
+      const T *src = static_cast<const T *>(r.src) + b * r.src_stride[0] + token0 * r.src_stride[1];
+      const T *grad = static_cast<const T *>(r.grad) + b * r.grad_stride[0] + token0 * r.grad_stride[1];
+      T *dst = static_cast<T *>(r.dst) + b * r.dst_stride[0] + token0 * r.dst_stride[1];
       Raw<T, V, K> rx, rg;
       auto load = [&] {
-        load_row<T, V, K>(units, static_cast<const T *>(r.src) + b * r.src_stride[0] + (token0 + t) * r.src_stride[1] +
-                                 h * r.src_stride[2], rx);
-        load_row<T, V, K>(units, static_cast<const T *>(r.grad) + b * r.grad_stride[0] + (token0 + t) * r.grad_stride[1] +
-                                 h * r.grad_stride[2], rg);
+        load_row<T, V, K>(units, src + row_at(t, r.src_token, h, r.src_head), rx);
+        load_row<T, V, K>(units, grad + row_at(t, r.grad_token, h, r.grad_head), rg);
       };
       load();
       __syncthreads();
@@ -447,8 +466,7 @@ rotary_norm_backward_kernel(const __grid_constant__ Params p) {
           for (int i = 0; i < V; ++i) x[k][i] = tila::fma2(x[k][i], minus, g[k][i]);
         times<V, K>(rms, x);
         if (valid)
-          store_row<T, V, K>(units, static_cast<T *>(r.dst) + b * r.dst_stride[0] + (token0 + at) * r.dst_stride[1] +
-                                    head * r.dst_stride[2], x);
+          store_row<T, V, K>(units, dst + row_at(at, r.dst_token, head, r.dst_head), x);
       }
       from += tokens;
     }
@@ -536,6 +554,11 @@ int check(const tila_rotary_args *a, bool backward, char *log, size_t cap) {
         (r.src == 0 || r.dst == 0 || r.src % size != 0 || r.dst % size != 0 || r.grad % size != 0 ||
          (backward && r.grad == 0) || ((r.flags & TILA_ROWS_NORM) && r.weight == 0)))
       return fail(TILA_ERR_ARGUMENT, log, cap, "%s: an address is missing or not aligned to its elements", who);
+    const int64_t *strides[3] = {r.src_stride, r.dst_stride, r.grad_stride};
+    for (int k = 0; k < (backward ? 3 : 2); ++k)
+      for (int d = 1; d < 3; ++d)
+        if (strides[k][d] < 0 || strides[k][d] > 0xffffffffll)
+          return fail(TILA_ERR_ARGUMENT, log, cap, "%s: strides of tokens and heads must be below 2^32 elements", who);
     if (backward && (!(r.flags & TILA_ROWS_NORM) || (r.flags & TILA_ROWS_PAGED) || a->weight_grad[i] == 0))
       return fail(TILA_ERR_ARGUMENT, log, cap, "%s: rows must be normed and have a weight gradient", who);
     rotates = rotates || (r.flags & TILA_ROWS_ROTATE);
@@ -564,6 +587,9 @@ Params make_params(const tila_rotary_args &a, bool backward, int v) {
       o.dst_stride[k] = r.dst_stride[k];
       o.grad_stride[k] = r.grad_stride[k];
     }
+    o.src_token = static_cast<u32>(r.src_stride[1]), o.src_head = static_cast<u32>(r.src_stride[2]);
+    o.dst_token = static_cast<u32>(r.dst_stride[1]), o.dst_head = static_cast<u32>(r.dst_stride[2]);
+    o.grad_token = static_cast<u32>(r.grad_stride[1]), o.grad_head = static_cast<u32>(r.grad_stride[2]);
     o.heads = r.heads;
     o.flags = r.flags;
     p.heads += r.heads;
