@@ -702,11 +702,11 @@ Plan plan(const tila_attend_args &a) {
                        ? wide_chunk_of(p.prefix, (rows + 255) / 256 * p.kv_heads,
                                        r.own_wide ? 0. : 2. * own_keys * p.batch * p.kv_heads * p.dim, p.prefix_chunks)
                        : chunk_of(p.prefix, static_cast<i64>(r.prefix_tiles) * p.kv_heads, p.prefix_chunks);
-  const i64 own_blocks = r.own_wide ? (own_rows + 255) / 256 * p.kv_heads * p.batch
+  const i64 own_blocks = r.own_wide ? (own_rows + 127) / 128 * p.kv_heads * p.batch
                                     : static_cast<i64>(r.own_tiles) * p.kv_heads * p.batch;
   p.own_unit = r.own_wide ? 128 : kStep;
   p.own_chunks = own_keys == 0 ? 0
-                 : r.own_wide  ? static_cast<int>(std::max<i64>(1, std::min<i64>(kSms / own_blocks, (own_keys + 127) / 128)))
+                 : r.own_wide  ? static_cast<int>(std::max<i64>(1, std::min<i64>(2 * kSms / own_blocks, (own_keys + 127) / 128)))
                                : own_chunks_of(own_keys, own_blocks);
   p.own_least = p.own_unit;
   // where there are blocks enough, shorter sequences are not cut as finely as the longest:

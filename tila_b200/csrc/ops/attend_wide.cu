@@ -2,9 +2,9 @@
 // than 16 rows of queries that see the same keys.
 //
 // Up to 256 rows against one chunk of keys: GEMM-shaped, on the 5th-generation
-// tensor cores.  One block a multiprocessor:
+// tensor cores.  A block has
 //
-//   * two softmax warpgroups, one row a thread (a row is a TMEM lane), each with
+//   * one or two softmax warpgroups, one row a thread (a row is a TMEM lane), each with
 //     its own scores S (128 columns) and its own sums O in tensor memory;
 //   * a copy warp that streams tiles of 128 keys, then of their values, through
 //     one ring in shared memory: a TMA box for each page and each 64 elements of
@@ -15,12 +15,15 @@
 //     others through its weight of 0, so it is cleared there and put into the rows
 //     that see it at the end.
 //
-// With more than 128 rows the warpgroups hold two row tiles and share every
-// tile of keys (half the traffic from L2, which at 128 rows a tile would bound:
-// 64 KB for every 1024 cycles of MMA); with fewer, both hold the same rows and
-// take the tiles in turn, and their results are joined at the end.  Either way
-// the tensor core works for one while the other is in its softmax.  Weights P
-// (rounded to the values' type) go through tensor memory in the place of S.
+// The prefix: two softmax warpgroups and one block a multiprocessor.  With more than
+// 128 rows they hold two row tiles and share every tile of keys (half the traffic
+// from L2, which at 128 rows a tile would bound: 64 KB for every 1024 cycles of MMA);
+// with fewer, both hold the same rows and take the tiles in turn, and their results
+// are joined at the end.  Either way the tensor core works for one while the other is
+// in its softmax.  Sequences' own tokens: many blocks of few tiles, so one warpgroup
+// and 128 rows a block, two blocks a multiprocessor, which also hide each other's
+// beginnings and ends (11 us of a block's 15 at 4 tiles).  Weights P (rounded to the
+// values' type) go through tensor memory in the place of S.
 //
 // tcgen05 operations of one thread run in order: S of a warpgroup's next tile,
 // issued behind P V of its last, overwrites P only after that was read, and its
@@ -43,30 +46,38 @@ namespace {
 
 using tila::TensorMap;
 
-constexpr int kThreads = 384;
-// Registers a thread at launch (65536 / 384 in steps of 8), and what the
-// warpgroups keep of them: the softmax holds a whole row of scores.  The shares add up to
-// 256 * 216 + 128 * 64 = 63488, below the 384 * 168 = 64512 at launch; the host
-// checks that the compiler gave the kernel exactly those, since a warpgroup
-// would otherwise wait for registers that do not exist.
-constexpr int kLaunchRegisters = 168;
 constexpr int kTile = 128;                       // keys of a tile, rows of a row tile
 constexpr int kHalf = kTile * 128;               // bytes of 64 elements of a tile
 constexpr float kGrowth = 8.f;                   // log2 of what weights may reach before O is scaled
 
-template <int DP> struct Wide {
-  // At 64 elements tensor memory has room for P beside S: S of the next tile is
-  // issued as soon as the warpgroup has read S, and is there when it comes back.
+// G softmax warpgroups: two, one block a multiprocessor, for the prefix; one, two blocks
+// a multiprocessor, for sequences' own tokens.
+template <int DP, int G> struct Wide {
+  static constexpr int kThreads = G * 128 + 128;
+  static constexpr int kBlocks = G == 2 ? 1 : 2;            // of a multiprocessor
+  // Registers a thread at launch (65536 / (kBlocks * kThreads) in steps of 8), and what
+  // the warpgroups keep of them: the softmax holds a whole row of scores.  The shares
+  // add up to at most the total at launch (256 * 216 + 128 * 64 = 63488 of 384 * 168 =
+  // 64512; 128 * 200 + 128 * 56 = 256 * 128); the host checks that the compiler gave the
+  // kernel exactly those, since a warpgroup would otherwise wait for registers that do
+  // not exist.
+  static constexpr int kLaunchRegisters = G == 2 ? 168 : 128;
+  static constexpr int kSoftmaxRegisters = G == 2 ? 216 : 200, kOtherRegisters = G == 2 ? 64 : 56;
+  static_assert(G * 128 * kSoftmaxRegisters + 128 * kOtherRegisters <= kThreads * kLaunchRegisters, "registers");
+  // Tensor memory: S, P and O of each warpgroup.  At 64 elements there is room for P
+  // beside S: S of the next tile is issued as soon as the warpgroup has read S, and is
+  // there when it comes back.
   static constexpr bool kEarly = DP == 64;
-  static constexpr u32 kWeightsAt = kEarly ? 256 : 0, kWeightsStep = kEarly ? 64 : 128;   // columns of P
-  static constexpr u32 kSumsAt = kEarly ? 384 : 256;                                      // columns of O
+  static constexpr u32 kColumns = 256 * G;
+  static constexpr u32 kWeightsAt = kEarly ? 128 * G : 0, kWeightsStep = kEarly ? 64 : 128;   // columns of P
+  static constexpr u32 kSumsAt = kEarly ? 192 * G : 128 * G;                                  // columns of O
   static constexpr int kTileBytes = kTile * DP * 2;
-  static constexpr int kStages = DP == 128 ? 5 : 9;
-  static constexpr int kRing = 2 * kTileBytes;   // behind the two query tiles
+  static constexpr int kStages = G == 2 ? (DP == 128 ? 5 : 9) : (DP == 128 ? 2 : 5);
+  static constexpr int kRing = G * kTileBytes;   // behind the query tiles
   static constexpr int kBytes = kRing + kStages * kTileBytes + 1024;   // 1024: alignment of swizzled tiles
   static constexpr int kRowFloats = DP + 4;      // of a staged result row: no two rows start in one bank
-  static_assert(2 * kTile * kRowFloats * 4 <= kStages * kTileBytes, "results are staged in the ring");
-  static_assert(kBytes <= 227 * 1024, "shared memory of a block");
+  static_assert(G * kTile * kRowFloats * 4 <= kRing + kStages * kTileBytes, "results are staged in queries and ring");
+  static_assert(kBytes <= (G == 2 ? 226 : 112) * 1024, "shared memory of a block");
 };
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -147,7 +158,9 @@ struct Barriers {
 template <typename T, int DP, bool kOwn>
 __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMap &kmap, const TensorMap &vmap,
                                            const WideGrid &grid) {
-  using W = Wide<DP>;
+  constexpr int G = kOwn ? 1 : 2;                            // softmax warpgroups
+  using W = Wide<DP, G>;
+  constexpr int kCopies = 4 * G, kMmas = 4 * G + 1, kLooks = 4 * G + 2;   // first warps of the other roles
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) Barriers bars;
   __shared__ OddValues<kOwn ? DP : 1> odd;
@@ -189,14 +202,14 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
       const int keys = own_chunk(p, length);
       begin = chunk * keys;
       // the last token of the block's rows sees furthest
-      const int last = min((pair + 1) * 2 * kTile, rows) - 1;
+      const int last = min((pair + 1) * G * kTile, rows) - 1;
       end = min(begin + keys, limit0 + last / p.group);
       pages = p.table + b * p.table_stride;
     }
   }
-  const int row0 = pair * 2 * kTile;
+  const int row0 = pair * G * kTile;
   if (row0 >= rows || (begin >= end && !p.direct)) return;
-  const bool shared_rows = rows - row0 <= kTile;     // one row tile: the warpgroups take tiles in turn
+  const bool shared_rows = G == 2 && rows - row0 <= kTile;   // one row tile: the warpgroups take tiles in turn
   const int tiles = end > begin ? (end - begin + kTile - 1) / kTile : 0;
   const int ahead = shared_rows ? 2 : 1;             // S is issued so many tiles ahead of P V
   // tiles from here on hold keys that some rows see and others do not (3 at most: a
@@ -219,15 +232,15 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
       tila::mbar_init(&bars.loaded[i], 1);
       tila::mbar_init(&bars.checked[i], 2);
     }
-    tila::mbar_init(&bars.queries, 2 * kTile);
+    tila::mbar_init(&bars.queries, G * kTile);
     tila::mbar_init(&bars.done, 1);
     dead = 0;
     odd.any = 0;
     tila::mbar_fence_init();
   }
-  if (kOwn && warp >= 10 && mixed < tiles)
-    for (int i = threadIdx.x - 320; i < 3 * DP; i += 64) odd.first[i / DP][i % DP] = kNever;
-  if (warp == 9) tila::tmem_alloc(&tmem_slot, 512);
+  if (kOwn && warp >= kLooks && mixed < tiles)
+    for (int i = threadIdx.x - 32 * kLooks; i < 3 * DP; i += 64) odd.first[i / DP][i % DP] = kNever;
+  if (warp == kMmas) tila::tmem_alloc(&tmem_slot, W::kColumns);
   tila::tc_fence_before();
   __syncthreads();
   tila::tc_fence_after();
@@ -238,8 +251,8 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
   // tile j + ahead.
   const int first_keys = min(ahead, tiles);
 
-  if (warp >= 8) tila::reg_dealloc<64>();
-  if (warp == 8) {
+  if (warp >= kCopies) tila::reg_dealloc<W::kOtherRegisters>();
+  if (warp == kCopies) {
     // ---- copies -----------------------------------------------------------------
     // A lane copies one box: 64 elements of one page's rows in the tile.  Its page
     // is looked up one tile ahead.
@@ -285,12 +298,12 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
       values = next_values;
       keys = next_keys;
     }
-  } else if (warp == 9) {
+  } else if (warp == kMmas) {
     // ---- MMAs -------------------------------------------------------------------
     const u32 base4 = uniform(tila::smem_u32(smem)) >> 4, tm = uniform(tmem);
     const int n_tiles = static_cast<int>(uniform(tiles)), key_end = static_cast<int>(uniform(end));
     const bool turns = uniform(shared_rows) != 0;                 // the warpgroups take tiles in turn
-    const bool second = uniform(rows - row0 > kTile) != 0;        // the second row tile exists
+    const bool second = G == 2 && uniform(rows - row0 > kTile) != 0;        // the second row tile exists
     const int lead = turns ? 2 : 1, first_mixed = static_cast<int>(uniform(mixed));
     constexpr u32 kFormat = __is_same(T, __half) ? 0u : (1u << 7) | (1u << 10);
     constexpr u32 kScoresDesc = tila::idesc_f16_f32(128, 128, 0, 0) | kFormat;
@@ -378,7 +391,7 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
     }
     if (ok && n_tiles > 0 && elected()) tila::mma_commit(&bars.done);
     __syncwarp();
-  } else if (warp >= 10) {
+  } else if (warp >= kLooks) {
     if constexpr (kOwn) {
       // ---- values of mixed tiles -----------------------------------------------------
       bool ok = true;
@@ -388,7 +401,7 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
         // (not the ring's own barrier, whose phases this warp does not follow)
         ok = warp_wait(&bars.loaded[j - mixed], 0, p.err, __LINE__, dead_ptr);
         const int seen = min(kTile, end - (begin + j * kTile));
-        for (int i = threadIdx.x - 320; ok && i < seen * (DP / 8); i += 64) {
+        for (int i = threadIdx.x - 32 * kLooks; ok && i < seen * (DP / 8); i += 64) {
           const int r = i / (DP / 8), c = i % (DP / 8);
           unsigned char *at = v + (c / 8) * kHalf + r * 128 + (((c % 8) ^ (r & 7)) << 4);
           if (any_odd<T>(*reinterpret_cast<const uint4 *>(at))) {
@@ -408,9 +421,9 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
         if (lane == 0) tila::mbar_arrive(&bars.checked[j - mixed]);
       }
     }
-  } else if (warp < 8) {
+  } else {
     // ---- softmax: warpgroup w, one row a thread ------------------------------------
-    tila::reg_alloc<216>();
+    tila::reg_alloc<W::kSoftmaxRegisters>();
     const int w = warp >> 2, r = threadIdx.x & (kTile - 1);
     const int row = row0 + (shared_rows ? 0 : w * kTile) + r;
     const bool valid = row < rows;
@@ -537,10 +550,10 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
       tila::mbar_arrive(&bars.weights[w]);
     }
 
-    // ---- results: normalised, staged in the ring (free by now) ---------------
+    // ---- results: normalised, staged in queries and ring (free by now) --------
     if (tiles > 0) ok = warp_wait(&bars.done, 0, p.err, __LINE__, dead_ptr) && ok;
     tila::tc_fence_after();
-    float *staged = reinterpret_cast<float *>(smem + W::kRing) + (w * kTile + r) * W::kRowFloats;
+    float *staged = reinterpret_cast<float *>(smem) + (w * kTile + r) * W::kRowFloats;
     float lse = sum == 0.f ? kNegInf : top + log2f(sum);
     float mine = sum == 0.f ? 0.f : 1.f / sum, other = 0.f;   // factors of the two warpgroups' sums
     const float *partner = staged + kTile * W::kRowFloats;
@@ -607,13 +620,13 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
     tila::tc_fence_before();
   }
   __syncthreads();
-  if (warp == 9) tila::tmem_dealloc(tmem, 512);
+  if (warp == kMmas) tila::tmem_dealloc(tmem, W::kColumns);
 }
 
 // The first block ends after the previous kernel, beside which this one may run, so
 // that what waits for this grid waits for both.
 template <typename T, int DP, bool kOwn>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Wide<DP, kOwn ? 1 : 2>::kThreads, Wide<DP, kOwn ? 1 : 2>::kBlocks)
 attend_wide_kernel(const __grid_constant__ AttendParams p, const __grid_constant__ TensorMap kmap,
                    const __grid_constant__ TensorMap vmap, const __grid_constant__ WideGrid grid) {
   tila::grid_dep_release();
@@ -635,15 +648,16 @@ int encode(TensorMap *map, const tila_attend_args &a, int rows, u64 address, con
 template <typename T, int DP, bool kOwn>
 cudaError_t launch_form(const AttendParams &p, const TensorMap &k, const TensorMap &v, const WideGrid &grid,
                         unsigned blocks, bool after_previous, cudaStream_t stream) {
+  using W = Wide<DP, kOwn ? 1 : 2>;
   static const cudaError_t registers = [] {
     cudaFuncAttributes attr;
     const cudaError_t e = cudaFuncGetAttributes(&attr, attend_wide_kernel<T, DP, kOwn>);
-    return e != cudaSuccess ? e : attr.numRegs == kLaunchRegisters ? cudaSuccess : cudaErrorLaunchOutOfResources;
+    return e != cudaSuccess ? e : attr.numRegs == W::kLaunchRegisters ? cudaSuccess : cudaErrorLaunchOutOfResources;
   }();
   if (registers != cudaSuccess) return registers;
-  const cudaError_t e = allow_shared_memory<attend_wide_kernel<T, DP, kOwn>>(Wide<DP>::kBytes);
+  const cudaError_t e = allow_shared_memory<attend_wide_kernel<T, DP, kOwn>>(W::kBytes);
   if (e != cudaSuccess) return e;
-  return launch_kernel(attend_wide_kernel<T, DP, kOwn>, blocks, kThreads, Wide<DP>::kBytes, stream, after_previous, p, k, v,
+  return launch_kernel(attend_wide_kernel<T, DP, kOwn>, blocks, W::kThreads, W::kBytes, stream, after_previous, p, k, v,
                        grid);
 }
 
@@ -676,7 +690,8 @@ int launch_wide(const tila_attend_args &a, const AttendParams &p, bool prefix, b
   if (st != TILA_OK) return st;
   WideGrid grid{};
   const i64 rows = static_cast<i64>(prefix ? (a.query_offsets == 0 ? a.batch : a.tokens) : p.max_queries) * p.group;
-  grid.pairs = static_cast<int>((rows + 2 * kTile - 1) / (2 * kTile));
+  const int each = (prefix ? 2 : 1) * kTile;                // rows of a block
+  grid.pairs = static_cast<int>((rows + each - 1) / each);
   const i64 blocks = static_cast<i64>(grid.pairs) * p.kv_heads *
                      (prefix ? p.prefix_chunks : static_cast<i64>(p.own_chunks) * p.batch);
   if (blocks > 0x7fffffff) return fail(TILA_ERR_ARGUMENT, log, cap, "tila_attend_shared_prefix: too many blocks");

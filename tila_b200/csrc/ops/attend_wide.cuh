@@ -6,7 +6,7 @@
 namespace tila_ops {
 
 struct WideGrid {
-  int pairs;         // pairs of row tiles of 128
+  int pairs;         // blocks' shares of the rows: pairs of row tiles of 128 (prefix), or single ones
 };
 
 // Whether the caches' strides allow tensor maps; and whether pages and head size
