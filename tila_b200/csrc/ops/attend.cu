@@ -457,6 +457,58 @@ attend_narrow_kernel(const __grid_constant__ AttendParams p, const __grid_consta
   if (blockIdx.x == 0 && threadIdx.x == 0) tila::grid_dep_wait();
 }
 
+// The weighted sum of a row's partial results, N slots in flight at a time: the
+// running maximum lets rows be loaded beside their weights.  With short rows no load
+// is conditional (slots behind the last read the last one, with no weight): 16000 rows
+// of 3 slots of 64 elements take 6 us so and 10 us otherwise; with longer rows, of which
+// there are fewer with more slots, it costs 2 us.
+template <int I> struct Joined { float top = kNegInf, sum = 0.f, acc[I * 4] = {}; };
+template <int L, int I, int N>
+__device__ __forceinline__ void join_slots(const AttendParams &p, i64 at, i64 step, int slots, int lane, Joined<I> &j) {
+  constexpr bool kAlways = L == 16;
+  for (int s0 = 0; s0 < slots; s0 += N) {
+    float lse[N];
+    float4 row[N][I];
+#pragma unroll
+    for (int s = 0; s < N; ++s) {
+      lse[s] = kNegInf;
+      if (!kAlways && s0 + s >= slots) continue;
+      const i64 place = (kAlways ? min(s0 + s, slots - 1) : s0 + s) * step + at;
+      lse[s] = p.partial_lse[place];
+#pragma unroll
+      for (int i = 0; i < I; ++i) {
+        const int d = lane * 4 + i * 4 * L;
+        row[s][i] = *reinterpret_cast<const float4 *>(p.partial + place * p.dim + (d < p.dim ? d : 0));
+      }
+    }
+    float high = j.top;
+#pragma unroll
+    for (int s = 0; s < N; ++s) {
+      if (s0 + s >= slots) lse[s] = kNegInf;
+      high = fmaxf(high, lse[s]);
+    }
+    const float base = high == kNegInf ? 0.f : high;
+    const float f = exp2f(j.top - base);
+    j.top = high;
+    j.sum *= f;
+#pragma unroll
+    for (int i = 0; i < I * 4; ++i) j.acc[i] *= f;
+#pragma unroll
+    for (int s = 0; s < N; ++s) {
+      const float w = exp2f(lse[s] - base);
+      j.sum += w;
+      if (w != 0.f)                                          // (a slot that nothing was seen in may hold anything)
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+          j.acc[i * 4] = fmaf(w, row[s][i].x, j.acc[i * 4]);
+          j.acc[i * 4 + 1] = fmaf(w, row[s][i].y, j.acc[i * 4 + 1]);
+          j.acc[i * 4 + 2] = fmaf(w, row[s][i].z, j.acc[i * 4 + 2]);
+          j.acc[i * 4 + 3] = fmaf(w, row[s][i].w, j.acc[i * 4 + 3]);
+        }
+    }
+  }
+}
+
 // out = sum over slots of 2^(lse_s - lse) * partial_s, lse = log2 sum 2^lse_s: L lanes
 // for each row of q and head.  Bound by reading the partial results, which the
 // blocks before left in L2.  Which row, sequence and chunks is found out before the
@@ -470,8 +522,17 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
   const int head = static_cast<int>(at) - token * p.heads;
   // the row's sequence, and the chunks of its own tokens that it saw
   int b = token;
-  if (p.offsets != nullptr) {
-    int lo = 0, hi = p.batch;                 // the last b with offsets[b] <= token
+  if (p.offsets != nullptr && p.batch <= 8 * L) {
+    // the last b with offsets[b] <= token, all looked at in one go by the row's lanes
+    int before = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      before += lane + i * L < p.batch && p.offsets[min(lane + i * L, p.batch)] <= token;
+#pragma unroll
+    for (int x = L / 2; x > 0; x >>= 1) before += __shfl_xor_sync(0xffffffffu, before, x);
+    b = max(before - 1, 0);
+  } else if (p.offsets != nullptr) {
+    int lo = 0, hi = p.batch;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       (p.offsets[mid] <= token ? lo : hi) = mid;
@@ -489,48 +550,10 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
   tila::grid_dep_wait();
   if (!there || token < first || token >= first + count) return;
   const i64 step = p.tokens * p.heads;
-  // the running maximum over slots keeps each slot's lse and row one load away: 8
-  // slots' rows are in flight at a time, and none waits for the weights
-  float top = kNegInf, sum = 0.f;
-  float acc[I * 4] = {};
-  for (int s0 = 0; s0 < slots; s0 += 8) {
-    float lse[8];
-    float4 row[8][I];
-#pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      lse[s] = kNegInf;
-      if (s0 + s < slots) {
-        const i64 place = (s0 + s) * step + at;
-        lse[s] = p.partial_lse[place];
-#pragma unroll
-        for (int i = 0; i < I; ++i)
-          if (lane * 4 + i * 4 * L < p.dim)
-            row[s][i] = *reinterpret_cast<const float4 *>(p.partial + place * p.dim + lane * 4 + i * 4 * L);
-      }
-    }
-    float high = top;
-#pragma unroll
-    for (int s = 0; s < 8; ++s) high = fmaxf(high, lse[s]);
-    const float base = high == kNegInf ? 0.f : high;
-    const float f = exp2f(top - base);
-    top = high;
-    sum *= f;
-#pragma unroll
-    for (int i = 0; i < I * 4; ++i) acc[i] *= f;
-#pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      const float w = exp2f(lse[s] - base);
-      sum += w;
-      if (s0 + s < slots && w != 0.f)
-#pragma unroll
-        for (int i = 0; i < I; ++i) {
-          acc[i * 4] = fmaf(w, row[s][i].x, acc[i * 4]);
-          acc[i * 4 + 1] = fmaf(w, row[s][i].y, acc[i * 4 + 1]);
-          acc[i * 4 + 2] = fmaf(w, row[s][i].z, acc[i * 4 + 2]);
-          acc[i * 4 + 3] = fmaf(w, row[s][i].w, acc[i * 4 + 3]);
-        }
-    }
-  }
+  Joined<I> j;
+  join_slots<L, I, L == 16 ? 4 : 8>(p, at, step, slots, lane, j);
+  const float top = j.top, sum = j.sum;
+  const float (&acc)[I * 4] = j.acc;
   const float inverse = sum == 0.f ? 0.f : 1.f / sum;
   T *out = static_cast<T *>(p.out) + static_cast<i64>(token) * p.out_stride[0] + head * p.out_stride[1];
 #pragma unroll
