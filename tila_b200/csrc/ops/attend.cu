@@ -463,17 +463,20 @@ attend_narrow_kernel(const __grid_constant__ AttendParams p, const __grid_consta
 // of 3 slots of 64 elements take 6 us so and 10 us otherwise; with longer rows, of which
 // there are fewer with more slots, it costs 2 us.
 template <int I> struct Joined { float top = kNegInf, sum = 0.f, acc[I * 4] = {}; };
+// Slots `from`, `from` + `by` and so on.
 template <int L, int I, int N>
-__device__ __forceinline__ void join_slots(const AttendParams &p, i64 at, i64 step, int slots, int lane, Joined<I> &j) {
+__device__ __forceinline__ void join_slots(const AttendParams &p, i64 at, i64 step, int slots, int from, int by, int lane,
+                                           Joined<I> &j) {
   constexpr bool kAlways = L == 16;
-  for (int s0 = 0; s0 < slots; s0 += N) {
+  for (int s0 = from; s0 < slots; s0 += N * by) {
     float lse[N];
     float4 row[N][I];
 #pragma unroll
     for (int s = 0; s < N; ++s) {
       lse[s] = kNegInf;
-      if (!kAlways && s0 + s >= slots) continue;
-      const i64 place = (kAlways ? min(s0 + s, slots - 1) : s0 + s) * step + at;
+      const int slot = s0 + s * by;
+      if (!kAlways && slot >= slots) continue;
+      const i64 place = (kAlways ? min(slot, slots - 1) : slot) * step + at;
       lse[s] = p.partial_lse[place];
 #pragma unroll
       for (int i = 0; i < I; ++i) {
@@ -484,7 +487,7 @@ __device__ __forceinline__ void join_slots(const AttendParams &p, i64 at, i64 st
     float high = j.top;
 #pragma unroll
     for (int s = 0; s < N; ++s) {
-      if (s0 + s >= slots) lse[s] = kNegInf;
+      if (s0 + s * by >= slots) lse[s] = kNegInf;
       high = fmaxf(high, lse[s]);
     }
     const float base = high == kNegInf ? 0.f : high;
@@ -513,10 +516,13 @@ __device__ __forceinline__ void join_slots(const AttendParams &p, i64 at, i64 st
 // for each row of q and head.  Bound by reading the partial results, which the
 // blocks before left in L2.  Which row, sequence and chunks is found out before the
 // wait for them: lengths and offsets are older than the kernels waited for.
-template <typename T, int L, int I>
+// `kBlock`: a whole block for each row, its groups of L lanes take the slots in turn:
+// few rows of many slots, which would wait for one another's loads.
+template <typename T, int L, int I, bool kBlock>
 __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant__ AttendParams p) {
-  const int lane = threadIdx.x % L;
-  const i64 at = static_cast<i64>(blockIdx.x) * (256 / L) + threadIdx.x / L;
+  constexpr int kParts = kBlock ? 256 / L : 1;
+  const int lane = threadIdx.x % L, part = kBlock ? threadIdx.x / L : 0;
+  const i64 at = kBlock ? blockIdx.x : static_cast<i64>(blockIdx.x) * (256 / L) + threadIdx.x / L;
   const bool there = at < p.tokens * p.heads;
   const int token = there ? static_cast<int>(at) / p.heads : 0;
   const int head = static_cast<int>(at) - token * p.heads;
@@ -551,7 +557,35 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
   if (!there || token < first || token >= first + count) return;
   const i64 step = p.tokens * p.heads;
   Joined<I> j;
-  join_slots<L, I, L == 16 ? 4 : 8>(p, at, step, slots, lane, j);
+  join_slots<L, I, kBlock || L == 16 ? 4 : 8>(p, at, step, slots, part, kParts, lane, j);
+  if constexpr (kBlock) {
+    // the groups' sums, by the first group
+    __shared__ float2 seen[kParts];
+    __shared__ float4 sums[kParts][L * I];
+    if (lane == 0) seen[part] = make_float2(j.top, j.sum);
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+      sums[part][lane + i * L] = make_float4(j.acc[i * 4], j.acc[i * 4 + 1], j.acc[i * 4 + 2], j.acc[i * 4 + 3]);
+    __syncthreads();
+    if (part != 0) return;
+    j = Joined<I>{};
+#pragma unroll
+    for (int k = 0; k < kParts; ++k) j.top = fmaxf(j.top, seen[k].x);
+#pragma unroll
+    for (int k = 0; k < kParts; ++k) {
+      // (a group that saw nothing has sums of 0, or not a number)
+      const float f = seen[k].x == kNegInf ? 1.f : exp2f(seen[k].x - j.top);
+      j.sum += seen[k].y * f;
+#pragma unroll
+      for (int i = 0; i < I; ++i) {
+        const float4 x = sums[k][lane + i * L];
+        j.acc[i * 4] = fmaf(f, x.x, j.acc[i * 4]);
+        j.acc[i * 4 + 1] = fmaf(f, x.y, j.acc[i * 4 + 1]);
+        j.acc[i * 4 + 2] = fmaf(f, x.z, j.acc[i * 4 + 2]);
+        j.acc[i * 4 + 3] = fmaf(f, x.w, j.acc[i * 4 + 3]);
+      }
+    }
+  }
   const float top = j.top, sum = j.sum;
   const float (&acc)[I * 4] = j.acc;
   const float inverse = sum == 0.f ? 0.f : 1.f / sum;
@@ -775,9 +809,15 @@ cudaError_t launch(const Plan &r, const tila::TensorMap &k, const tila::TensorMa
   if (e != cudaSuccess || r.p.direct) return e;
   const int lanes = r.p.dim <= 64 ? 16 : 32;
   const unsigned blocks = static_cast<unsigned>((r.p.tokens * r.p.heads * lanes + 255) / 256);
-  return launch_kernel(r.p.dim <= 64    ? attend_join_kernel<T, 16, 1>
-                       : r.p.dim <= 128 ? attend_join_kernel<T, 32, 1>
-                                        : attend_join_kernel<T, 32, 2>,
+  const i64 rows = r.p.tokens * r.p.heads;
+  if (rows <= 4 * kSms && r.slots > 8)                        // 2048 rows of 20 slots take 5 us more so, 24 of 71 3 less
+    return launch_kernel(r.p.dim <= 64    ? attend_join_kernel<T, 16, 1, true>
+                         : r.p.dim <= 128 ? attend_join_kernel<T, 32, 1, true>
+                                          : attend_join_kernel<T, 32, 2, true>,
+                         static_cast<unsigned>(rows), 256, 0, stream, true, r.p);
+  return launch_kernel(r.p.dim <= 64    ? attend_join_kernel<T, 16, 1, false>
+                       : r.p.dim <= 128 ? attend_join_kernel<T, 32, 1, false>
+                                        : attend_join_kernel<T, 32, 2, false>,
                        blocks, 256, 0, stream, true, r.p);
 }
 
