@@ -44,6 +44,7 @@ def as_positions(positions, tokens):
 @pytest.mark.parametrize("batch,tokens,heads,dim,rotary", [
     (1, 1, 1, 2, 2), (1, 1, 32, 128, 128), (2, 37, 5, 64, 64), (3, 9, 3, 80, 40), (1, 130, 2, 96, 24),
     (2, 5, 7, 128, 32), (1, 17, 4, 33, 10), (1, 3, 1, 512, 512), (1, 4, 2, 511, 6), (2, 3, 2, 40, 0), (1, 600, 1, 20, 20),
+    (2, 65, 5, 80, 20), (1, 40, 3, 504, 250), (1, 33, 2, 8, 2), (1, 700, 3, 24, 22),
 ])
 def test_rotate(layout, dtype, batch, tokens, heads, dim, rotary):
     g = gen(dim + tokens)
@@ -99,7 +100,7 @@ def test_rotate_nothing():
 
 NORM_CASES = [  # tokens, heads, kv_heads, dim, rotary
     (1, 1, 1, 128, 128), (7, 32, 8, 128, 128), (700, 5, 2, 64, 64), (65, 3, 3, 80, 40), (33, 4, 1, 96, 24), (5, 2, 1, 33, 10),
-    (9, 2, 2, 512, 64), (3, 1, 2, 20, 0),
+    (9, 2, 2, 512, 64), (3, 1, 2, 20, 0), (301, 5, 2, 80, 20), (17, 3, 1, 504, 250), (40, 2, 1, 24, 22),
 ]
 
 

@@ -17,7 +17,11 @@
 // GPU.  A row is spread over as many lanes as it has units; a unit is the two V-element
 // vectors that hold both halves of V pairs, so that neither layout moves data between
 // lanes, and V elements are one 16-byte access where sizes, strides and
-// addresses allow it.  Rows are taken tensor by tensor, so that pointers, flags and
+// addresses allow it.  Where only the rotated part stands in the way (half of it is no
+// multiple of V), units are plain pieces of the row and pairs meet in shared memory
+// (16384 tokens of 32 heads, f16, 84 MB each way: 20 of 80 elements rotated, 176 us
+// with 4-byte accesses, 66 us so, 60 us interleaved; 40 of 80, 95 us with 8-byte
+// accesses, 68 and 62 us so).  Rows are taken tensor by tensor, so that pointers, flags and
 // weights stay where they are from row to row; a row is loaded one ahead, and no load
 // is conditional, so that all of a row's are in flight together.  Arithmetic and
 // conversions are on pairs of floats.
@@ -61,6 +65,10 @@ struct Params {
   int units;
   int full;              // every lane has whole units
   int tokens_per_block;
+  int across;            // V where pairs meet in shared memory (kAcross), else 0
+  int table_units;       // of those, the units that have a part in the table
+  int token_table;       // floats of the table for one token
+  int row_floats;        // of a row in shared memory
   int any_norm, any_paged;
   int apart;             // a block for each tensor: few tokens, where latency counts
   float sign;            // -1 rotates back
@@ -91,7 +99,7 @@ template <int V, int K> struct Units {
   __device__ __forceinline__ Units(const Params &p, int lane) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int u = lane + k * p.lanes, pairs = p.half / V;   // units that rotate
+      const int u = lane + k * p.lanes, pairs = p.across ? 0 : p.half / V;   // units that rotate by themselves
       there[k] = u < p.units;
       turns[k] = u < pairs;
       const int at = there[k] ? u : 0;
@@ -216,8 +224,56 @@ __device__ __forceinline__ void turn(const Params &p, const Units<V, K> &u, cons
   }
 }
 
+// The same for units that are plain pieces of the row.  Each element meets its
+// partner in `row` (a group's own shared memory) or, interleaved, in its own
+// register; the table holds two cosines and two signed sines for each two elements.
+// Both lie by place in the unit first, then by unit: neighbouring lanes read
+// neighbouring words.
+template <int V, int K> struct Partners {
+  u32 at[K][V];                                               // places in `row`: two of 16 bits
+  __device__ __forceinline__ Partners(const Params &p, const Units<V, K> &u) {
+    auto place = [&](int e) {
+      const int partner = e < p.half ? e + p.half : e < 2 * p.half ? e - p.half : 0;
+      return static_cast<u32>(partner % (2 * V) * p.units + partner / (2 * V));
+    };
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) at[k][i] = place(u.first[k] + 2 * i) | place(u.first[k] + 2 * i + 1) << 16;
+  }
+};
+
+template <int V, int K>
+__device__ __forceinline__ void turn_across(const Params &p, const Units<V, K> &u, const Partners<V, K> &partners,
+                                            const float *tab, float *row, int lane, Lane<V, K> &x) {
+  if (!p.interleaved) {
+    __syncwarp();                                             // (the row before has been read)
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (u.there[k]) {                                     // (all of the unit: it has its places)
+          row[2 * i * p.units + lane + k * p.lanes] = tila::lo2(x[k][i]);
+          row[(2 * i + 1) * p.units + lane + k * p.lanes] = tila::hi2(x[k][i]);
+        }
+    __syncwarp();
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (u.there[k] && u.first[k] + 2 * i < 2 * p.half) {
+        const ulonglong2 t = *reinterpret_cast<const ulonglong2 *>(tab + 4 * (i * p.table_units + lane + k * p.lanes));
+        const u64 other = p.interleaved ? tila::pk2(tila::hi2(x[k][i]), tila::lo2(x[k][i]))
+                                        : tila::pk2(row[partners.at[k][i] & 0xffff], row[partners.at[k][i] >> 16]);
+        x[k][i] = tila::fma2(x[k][i], t.x, tila::mul2(other, t.y));
+      }
+}
+
 // Floats of the table: what follows it is 16-byte aligned.
-__host__ __device__ __forceinline__ int table_size(const Params &p) { return (2 * p.tokens_per_block * p.half + 3) & ~3; }
+__host__ __device__ __forceinline__ int table_size(const Params &p) {
+  return (p.token_table * p.tokens_per_block + 3) & ~3;
+}
 
 __device__ __forceinline__ void fill_table(const Params &p, int b, i64 token0, int tokens, float *tab) {
   for (int i = threadIdx.x; i < tokens * p.half; i += blockDim.x) {
@@ -227,8 +283,20 @@ __device__ __forceinline__ void fill_table(const Params &p, int b, i64 token0, i
     turns -= rint(turns);
     float s, c;
     sincospif(static_cast<float>(2.0 * turns), &s, &c);
-    tab[2 * t * p.half + j] = c * p.amplitude;
-    tab[(2 * t + 1) * p.half + j] = s * p.amplitude * p.sign;
+    c *= p.amplitude;
+    s *= p.amplitude * p.sign;
+    if (p.across) {
+      const int low = p.interleaved ? 2 * j : j, high = p.interleaved ? 2 * j + 1 : j + p.half;
+      auto at = [&](int e) {
+        return tab + t * p.token_table + 4 * ((e >> 1) % p.across * p.table_units + (e >> 1) / p.across) + (e & 1);
+      };
+      at(low)[0] = at(high)[0] = c;
+      at(low)[2] = -s;
+      at(high)[2] = s;
+    } else {
+      tab[2 * t * p.half + j] = c;
+      tab[(2 * t + 1) * p.half + j] = s;
+    }
   }
 }
 
@@ -289,7 +357,7 @@ template <typename T, int V> struct Resident {
   static constexpr int kBackward = 2;
 };
 
-template <typename T, int V, int K>
+template <typename T, int V, int K, bool kAcross>
 __global__ void __launch_bounds__(256, Resident<T, V>::kForward)
 rotary_rows_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(16) float tab[];
@@ -303,6 +371,7 @@ rotary_rows_kernel(const __grid_constant__ Params p) {
   const int groups = blockDim.x / p.lanes;
   const int lane = threadIdx.x & (p.lanes - 1), group = threadIdx.x / p.lanes;
   const Units<V, K> units(p, lane);
+  const Partners<V, K> partners(p, units);
 
   // Rows are taken tensor by tensor: its heads of one token, then of the next, one
   // to a group; each group's next row is `groups` on.  A group that has none left
@@ -371,7 +440,13 @@ rotary_rows_kernel(const __grid_constant__ Params p) {
         times<V, K>(rsqrtf(row_sum<V, K>(p, x, x) * p.inv_dim + p.eps), x);
         times_weight<V, K>(units, w, x);
       }
-      if (flags & TILA_ROWS_ROTATE) turn<V, K>(p, units, tab + 2 * at * p.half, lane, x);
+      if (flags & TILA_ROWS_ROTATE) {
+        if constexpr (kAcross)
+          turn_across<V, K>(p, units, partners, tab + at * p.token_table,
+                            weights + (p.any_norm ? (p.num_rows * p.dim + 3) & ~3 : 0) + group * p.row_floats, lane, x);
+        else
+          turn<V, K>(p, units, tab + 2 * at * p.half, lane, x);
+      }
       bool put = valid;
       i64 to;
       if (flags & TILA_ROWS_PAGED) {
@@ -392,7 +467,7 @@ rotary_rows_kernel(const __grid_constant__ Params p) {
 // equal share of the tokens, so that each sums its rows' dw in registers (first of the
 // queries, then of the keys) and leaves one partial sum; the partial sums are added in a
 // fixed order by the kernel below (no atomics: the same call gives the same bits).
-template <typename T, int V, int K>
+template <typename T, int V, int K, bool kAcross>
 __global__ void __launch_bounds__(256, Resident<T, V>::kBackward)
 rotary_norm_backward_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(16) float tab[];
@@ -401,6 +476,7 @@ rotary_norm_backward_kernel(const __grid_constant__ Params p) {
   const int groups = blockDim.x / p.lanes;
   const int lane = threadIdx.x & (p.lanes - 1), group = threadIdx.x / p.lanes;
   const Units<V, K> units(p, lane);
+  const Partners<V, K> partners(p, units);
   tila::grid_dep_release();
   fill_weights<T>(p, weights, p.num_rows);
   const i64 all = p.batch * p.tokens;
@@ -449,7 +525,10 @@ rotary_norm_backward_kernel(const __grid_constant__ Params p) {
           }
         }
         if (first + groups < jobs) load();
-        if (valid && (r.flags & TILA_ROWS_ROTATE)) turn<V, K>(p, units, tab + 2 * at * p.half, lane, g);
+        if (r.flags & TILA_ROWS_ROTATE) {
+          if constexpr (kAcross) turn_across<V, K>(p, units, partners, tab + at * p.token_table, scratch + group * p.row_floats, lane, g);
+          else turn<V, K>(p, units, tab + 2 * at * p.half, lane, g);
+        }
         const float rms = rsqrtf(row_sum<V, K>(p, x, x) * p.inv_dim + p.eps);
         times<V, K>(rms, x);                                        // xh
         if (valid)
@@ -520,17 +599,21 @@ bool aligned(u64 address, const int64_t *stride, int v, int size) {
   return address % (static_cast<u64>(v) * size) == 0 && stride[0] % v == 0 && stride[1] % v == 0 && stride[2] % v == 0;
 }
 
-// The widest vector that sizes, strides and addresses of the call allow.
-int vector_width(const tila_rotary_args &a, bool backward) {
+// The widest vector that sizes, strides and addresses of the call allow; `across`
+// where half of the rotated part is no multiple of it.
+int vector_width(const tila_rotary_args &a, bool backward, bool &across) {
   const int size = a.dtype == TILA_F32 ? 4 : 2;
+  across = false;
   for (int v = 16 / size; v > 1; v >>= 1) {
-    bool ok = (a.rotary / 2) % v == 0 && a.dim % v == 0;
+    bool ok = a.dim % v == 0;
     for (int i = 0; ok && i < a.num_rows; ++i) {
       const tila_op_rows &r = a.rows[i];
       ok = aligned(r.src, r.src_stride, v, size) && aligned(r.dst, r.dst_stride, v, size) &&
            (!backward || aligned(r.grad, r.grad_stride, v, size));
     }
-    if (ok) return v;
+    if (!ok) continue;
+    across = (a.rotary / 2) % v != 0 && v == 16 / size;
+    if (across || (a.rotary / 2) % v == 0) return v;
   }
   return 1;
 }
@@ -572,7 +655,7 @@ int check(const tila_rotary_args *a, bool backward, char *log, size_t cap) {
   return TILA_OK;
 }
 
-Params make_params(const tila_rotary_args &a, bool backward, int v) {
+Params make_params(const tila_rotary_args &a, bool backward, int v, bool across) {
   Params p{};
   bool rotates = false;
   for (int i = 0; i < a.num_rows; ++i) {
@@ -628,16 +711,21 @@ Params make_params(const tila_rotary_args &a, bool backward, int v) {
   p.page_size = a.page_size;
   p.index64 = a.index64;
   p.err = reinterpret_cast<u32 *>(a.err);
-  p.units = p.half / v + (a.dim - 2 * p.half + 2 * v - 1) / (2 * v);
+  p.across = across ? v : 0;
+  p.units = across ? (a.dim + 2 * v - 1) / (2 * v) : p.half / v + (a.dim - 2 * p.half + 2 * v - 1) / (2 * v);
+  p.table_units = (p.half + v - 1) / v;
+  p.token_table = across ? 4 * v * p.table_units : 2 * p.half;
   p.lanes = 1;
   while (p.lanes < p.units && p.lanes < 32) p.lanes <<= 1;
+  // an odd number of times the lanes: the groups of a warp lie in different banks
+  p.row_floats = across ? ((2 * v * p.units + p.lanes - 1) / p.lanes | 1) * p.lanes : 0;
   return p;
 }
 
 // Tokens of a block: rows for 256 threads at least; where there are more than
 // `resident` blocks a multiprocessor could take, as many as fill whole waves.
 int tokens_per_block(const Params &p, int resident) {
-  const i64 most = std::min(32, 2048 / std::max(1, p.half));
+  const i64 most = std::min(32, (p.across ? 1024 : 2048) / std::max(1, p.half));
   const i64 rows = 256 / std::max(1, p.heads * p.lanes);
   const i64 wave = static_cast<i64>(resident) * kSms, all = p.batch * p.tokens;
   const i64 waves = (all + wave * most - 1) / (wave * most);
@@ -648,7 +736,7 @@ int backward_blocks(const Params &p) {
   return static_cast<int>(std::min<i64>(p.batch * p.tokens, 2 * kSms));   // as many as run at once (Resident)
 }
 
-template <typename T, int V, int K>
+template <typename T, int V, int K, bool kAcross>
 int launch_forward(Params p, cudaStream_t stream, char *log, size_t cap) {
   p.full = p.dim % (2 * V) == 0 && p.units == p.lanes * K;
   p.tokens_per_block = tokens_per_block(p, Resident<T, V>::kForward);
@@ -661,24 +749,25 @@ int launch_forward(Params p, cudaStream_t stream, char *log, size_t cap) {
   const int threads = static_cast<int>(std::min<i64>(256, (lanes + 31) / 32 * 32));
   const size_t smem = sizeof(float) * table_size(p) +
                       (p.any_paged ? sizeof(i64) * ((3 * p.tokens_per_block + 1) / 2 * 2) : 0) +
-                      (p.any_norm ? 3 * sizeof(float) * p.dim : 0) + 16;
-  rotary_rows_kernel<T, V, K><<<static_cast<unsigned>(blocks), threads, smem, stream>>>(p);
+                      (p.any_norm ? sizeof(float) * ((p.num_rows * p.dim + 3) & ~3) : 0) +
+                      (kAcross ? sizeof(float) * p.row_floats * (threads / p.lanes) : 0);
+  rotary_rows_kernel<T, V, K, kAcross><<<static_cast<unsigned>(blocks), threads, smem, stream>>>(p);
   return launch_status(cudaGetLastError(), "tila_rotary_rows", log, cap);
 }
 
-template <typename T, int V, int K>
+template <typename T, int V, int K, bool kAcross>
 int launch_backward(Params p, const tila_rotary_args &a, cudaStream_t stream, char *log, size_t cap) {
   p.full = p.dim % (2 * V) == 0 && p.units == p.lanes * K;
-  p.tokens_per_block = std::min(32, 2048 / std::max(1, p.half));
+  p.tokens_per_block = std::min(32, (p.across ? 1024 : 2048) / std::max(1, p.half));
   const int blocks = backward_blocks(p);
   const int groups = kBackwardThreads / p.lanes;
-  const size_t smem = sizeof(float) * table_size(p) + sizeof(float) * p.dim * (2 + groups) + 16;
+  const size_t smem = sizeof(float) * table_size(p) + sizeof(float) * (2 * p.dim + std::max(p.dim, p.row_floats) * groups) + 16;
   cudaError_t e = cudaSuccess;
   if (smem > 48 * 1024)
-    e = cudaFuncSetAttribute(rotary_norm_backward_kernel<T, V, K>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    e = cudaFuncSetAttribute(rotary_norm_backward_kernel<T, V, K, kAcross>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(smem));
   if (e != cudaSuccess) return launch_status(e, "tila_rotary_norm_backward", log, cap);
-  rotary_norm_backward_kernel<T, V, K><<<blocks, kBackwardThreads, smem, stream>>>(p);
+  rotary_norm_backward_kernel<T, V, K, kAcross><<<blocks, kBackwardThreads, smem, stream>>>(p);
   e = cudaGetLastError();
   if (e == cudaSuccess)
     e = launch_kernel(weight_grad_kernel, (p.dim + 31) / 32 * 2, 1024, 0, stream, true,
@@ -691,24 +780,28 @@ template <typename T>
 int dispatch(const Params &p, const tila_rotary_args &a, int v, bool backward, char *log, size_t cap) {
   const cudaStream_t stream = reinterpret_cast<cudaStream_t>(a.stream);
   const int per_lane = (p.units + p.lanes - 1) / p.lanes;
-#define TILA_ROTARY(V, K) \
-  return backward ? launch_backward<T, V, K>(p, a, stream, log, cap) : launch_forward<T, V, K>(p, stream, log, cap)
+#define TILA_ROTARY(V, K, X)                                                     \
+  return backward ? launch_backward<T, V, K, X>(p, a, stream, log, cap)           \
+                  : launch_forward<T, V, K, X>(p, stream, log, cap)
   if constexpr (sizeof(T) == 2) {
-    if (v == 8) TILA_ROTARY(8, 1);
+    if (v == 8 && p.across) TILA_ROTARY(8, 1, true);
+    if (v == 8) TILA_ROTARY(8, 1, false);
   } else {
-    if (v == 4 && per_lane == 1) TILA_ROTARY(4, 1);
+    if (v == 4 && p.across) TILA_ROTARY(4, 2, true);
+    if (v == 4 && per_lane == 1) TILA_ROTARY(4, 1, false);
   }
-  if (v == 4) TILA_ROTARY(4, 2);
-  if (v == 2) TILA_ROTARY(2, 4);
-  TILA_ROTARY(1, 8);
+  if (v == 4) TILA_ROTARY(4, 2, false);
+  if (v == 2) TILA_ROTARY(2, 4, false);
+  TILA_ROTARY(1, 8, false);
 #undef TILA_ROTARY
 }
 
 int run(const tila_rotary_args *a, bool backward, char *log, size_t cap) {
   int st = check(a, backward, log, cap);
   if (st != TILA_OK) return st;
-  const int v = vector_width(*a, backward);
-  Params p = make_params(*a, backward, v);
+  bool across;
+  const int v = vector_width(*a, backward, across);
+  Params p = make_params(*a, backward, v, across);
   const cudaStream_t stream = reinterpret_cast<cudaStream_t>(a->stream);
   if (p.batch * p.tokens == 0 || p.heads == 0) {
     // no row: nothing to write, but the weights' gradients are zero
@@ -739,7 +832,9 @@ extern "C" int tila_rotary_norm_backward(const tila_rotary_args *args, char *log
 
 extern "C" uint64_t tila_rotary_workspace(const tila_rotary_args *a) {
   if (check(a, true, nullptr, 0) != TILA_OK) return 0;
-  Params p = make_params(*a, true, vector_width(*a, true));
+  bool across;
+  const int v = vector_width(*a, true, across);
+  Params p = make_params(*a, true, v, across);
   if (p.batch * p.tokens == 0 || p.heads == 0) return 0;
   return static_cast<uint64_t>(backward_blocks(p)) * 2 * a->dim * sizeof(float);
 }
