@@ -750,8 +750,13 @@ Plan plan(const tila_attend_args &a) {
   const i64 own_keys = a.max_length > 0 ? std::min<i64>(a.max_length, table_keys) : table_keys;
   const bool wide = wide_possible(a);
   r.narrow_tma = tma_possible(a) && a.page_size % kSlice == 0;
+  // The prefix: the narrow form would take longer, however few keys (256 rows a head on 512
+  // keys 32 us, wide 23; on 2048 44 and 27; 28 rows on 425 19 and 17).  Own tokens:
+  // up to 32 rows fill a quarter of a row tile, and two blocks of 16 that read the keys
+  // twice, once from L2, are faster (28 rows, 21 sequences of up to 3462 tokens: 32 us, wide
+  // 39; 20 rows, 64 of up to 1000: 34 and 48; 64 rows 43 either way).
   r.prefix_wide = wide && p.prefix > 0 && rows > 16;
-  r.own_wide = wide && own_keys > 0 && own_rows > 16;
+  r.own_wide = wide && own_keys > 0 && own_rows > 32;
   r.narrow_rows = (r.own_wide || own_rows <= 8) && (r.prefix_wide || rows <= 8) ? 8 : 16;
   r.prefix_tiles = static_cast<int>((rows + r.narrow_rows - 1) / r.narrow_rows);
   r.own_tiles = static_cast<int>((own_rows + r.narrow_rows - 1) / r.narrow_rows);
@@ -762,8 +767,12 @@ Plan plan(const tila_attend_args &a) {
   const i64 own_blocks = r.own_wide ? (own_rows + 127) / 128 * p.kv_heads * p.batch
                                     : static_cast<i64>(r.own_tiles) * p.kv_heads * p.batch;
   p.own_unit = r.own_wide ? 128 : kStep;
+  // wide: two blocks a multiprocessor, or up to four while a chunk has 8 tiles, since the
+  // longest sequence is what the last block waits for (168 blocks of up to 27 tiles: 72 us
+  // in three chunks, 99 in one; 256 of up to 8: 68 us in one, 73 in two)
   p.own_chunks = own_keys == 0 ? 0
-                 : r.own_wide  ? static_cast<int>(std::max<i64>(1, std::min<i64>(2 * kSms / own_blocks, (own_keys + 127) / 128)))
+                 : r.own_wide  ? static_cast<int>(std::max<i64>({1, std::min<i64>(2 * kSms / own_blocks, (own_keys + 127) / 128),
+                                                                  std::min<i64>(4 * kSms / own_blocks, (own_keys + 1023) / 1024)}))
                                : own_chunks_of(own_keys, own_blocks);
   p.own_least = p.own_unit;
   // where there are blocks enough, shorter sequences are not cut as finely as the longest:

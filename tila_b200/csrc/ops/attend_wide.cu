@@ -1,5 +1,5 @@
 // Attention over a paged cache with a shared prefix: the wide form, for more
-// than 16 rows of queries that see the same keys.
+// than 16 rows of queries that see the same prefix, or 32 that see the same sequence.
 //
 // Up to 256 rows against one chunk of keys: GEMM-shaped, on the 5th-generation
 // tensor cores.  A block has
