@@ -52,6 +52,7 @@ POS = torch.arange(6)
     (dict(x=dev(6, 2, 64, dtype=torch.float64)), "float32"),
     (dict(x=dev(6, 64)), "tokens, heads, dim"),
     (dict(x=dev(6, 2, 513)), "512"),
+    (dict(x=dev(6, 1, 64).expand(6, (1 << 20) + 1, 64)), "2\\^20 heads"),
     (dict(x=dev(6, 2, 128)[..., ::2]), "contiguous"),
     (dict(x=dev(6, 2, 62)), "rotates 64"),
     (dict(positions=POS[:5]), "one position per token"),

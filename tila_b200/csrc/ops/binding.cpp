@@ -233,6 +233,8 @@ void rows_shape(const char *fn, const char *what, const Tensor &x) {
     refuse("%s: %s must be (tokens, heads, dim) or (batch, tokens, heads, dim)", fn, what);
   if (x.size(-1) < 1 || x.size(-1) > 512)
     refuse("%s: %s must have heads of 1 to 512 elements, not %lld", fn, what, static_cast<long long>(x.size(-1)));
+  if (x.size(-2) > (1 << 20))
+    refuse("%s: %s must have at most 2^20 heads, not %lld", fn, what, static_cast<long long>(x.size(-2)));
   unit_last(fn, what, x);
 }
 
@@ -277,11 +279,17 @@ void layout(const char *fn, PyObject *o, tila_rotary_args &a) {
   }
 }
 
+// A stride of tokens or heads; that of a single one is never used and may be any (the
+// kernels take those strides in 32 bits).
+int64_t inner_stride(const Tensor &t, int d) {
+  return t.size(d) == 1 && t.stride(d) > int64_t{0xffffffff} ? 0 : t.stride(d);
+}
+
 void strides3(const Tensor &t, int64_t (&s)[3]) {
   const bool batch = t.dim() == 4;
   s[0] = batch ? t.stride(0) : 0;
-  s[1] = t.stride(batch ? 1 : 0);
-  s[2] = t.stride(batch ? 2 : 1);
+  s[1] = inner_stride(t, batch ? 1 : 0);
+  s[2] = inner_stride(t, batch ? 2 : 1);
 }
 
 uint32_t weight(const char *fn, const char *what, const Tensor &w, const Tensor &x, tila_op_rows &r) {
@@ -509,7 +517,7 @@ PyObject *append_paged(PyObject *const *o) {
     apart(fn, names[i], c, "v", v);
     tila_op_rows &r = a.rows[i];
     r.dst = address(c);
-    for (int d = 0; d < 3; ++d) r.dst_stride[d] = c.stride(d);
+    strides3(c, r.dst_stride);
     r.flags = TILA_ROWS_PAGED;
   }
   apart(fn, "k_cache", *caches[0], "v_cache", *caches[1]);
