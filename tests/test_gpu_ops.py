@@ -258,6 +258,41 @@ def test_append_reports_a_slot_outside_the_cache():
     assert torch.equal(vc.view(8, 1, 64)[:3], k)
 
 
+def test_an_error_met_in_a_capture_is_raised_again_after_it():
+    """A capture cannot reset the device's record: the error stays until a call
+    outside of one raises it, and later errors are recorded again."""
+    g = gen(4)
+    kc, vc = torch.zeros(1, 4, 1, 64, device="cuda"), torch.zeros(1, 4, 1, 64, device="cuda")
+    k = normal(g, 1, 1, 64)
+    good, bad = torch.tensor([1], device="cuda"), torch.tensor([4], device="cuda")
+    ops.append_paged(k, k, kc, vc, good)
+    for _ in range(2):
+        ops.append_paged(k, k, kc, vc, bad)
+        torch.cuda.synchronize()
+        with pytest.raises(native.NativeError, match="outside its pool"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                ops.append_paged(k, k, kc, vc, good)
+        with pytest.raises(native.NativeError, match="outside its pool"):
+            ops.append_paged(k, k, kc, vc, good)
+        ops.append_paged(k, k, kc, vc, good)
+        torch.cuda.synchronize()
+        ops.check_errors()
+
+
+def test_strides_of_single_tokens_and_heads_may_be_any():
+    x = normal(gen(6), 4, 64)
+    positions, inv = torch.tensor([7], device="cuda"), freqs(64)
+    want = ops.rotate(x.view(1, 4, 64), positions, inv)
+    assert torch.equal(ops.rotate(x.as_strided((1, 4, 64), (1 << 33, 64, 1)), positions, inv), want)
+    assert torch.equal(ops.rotate(x[:1].as_strided((1, 1, 64), (1 << 33, (1 << 40) + 1, 1)), positions, inv), want[:, :1])
+    cache = torch.zeros(3, 64, device="cuda")
+    pages = cache.as_strided((3, 1, 1, 64), (64, 1 << 40, 1 << 35, 1))
+    values = torch.zeros(3, 1, 1, 64, device="cuda")
+    ops.append_paged(x[:1].view(1, 1, 64), x[1:2].view(1, 1, 64), pages, values, torch.tensor([2], device="cuda"),
+                     positions=positions, inv_freq=inv)
+    assert torch.equal(cache[2], want[0, 0]) and torch.equal(values[2, 0, 0], x[1]) and not cache[:2].any()
+
+
 # ---------------------------------------------------------------------------
 # attention over the paged cache
 # ---------------------------------------------------------------------------

@@ -85,8 +85,9 @@ def check_errors(device=None) -> None:
         return
     word = b.word.value
     with torch.cuda.device(index):
-        b.block[0].zero_()
-    b.word.value = 0
+        if not torch.cuda.is_current_stream_capturing():    # (a graph would record the reset: the next call raises again)
+            b.block[0].zero_()
+            b.word.value = 0
     code, where = word >> 24, word & 0xFFFFFF
     raise native.NativeError(native.TILA_ERR_ARGUMENT if code == 5 else native.TILA_ERR_DRIVER,
                              f"an operator launched earlier on cuda:{index} failed: "
