@@ -477,6 +477,34 @@ def test_attend_odd_values_reach_only_who_sees_them(dtype, counts, lengths, pref
     ops.check_errors()
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("counts,lengths,prefix,heads,kv,dim", [
+    ([1] * 4, [50, 3, 200, 9], 300, 8, 2, 128), ([1] * 30, [50] * 30, 300, 8, 2, 128), ([40, 20], [100, 30], 200, 8, 2, 64),
+    ([100], [150], 0, 4, 1, 128),
+])
+def test_attend_queries_that_are_no_numbers(dtype, counts, lengths, prefix, heads, kv, dim):
+    """They show in their own row and nowhere else; scores of minus infinity
+    throughout count as nothing seen."""
+    q, kc, vc, table, lens, pages, offsets = paged(3, counts, lengths, prefix, heads, kv, dim, 16, dtype)
+    args = dict(prefix_pages=pages, prefix_length=prefix, query_offsets=offsets, max_queries=max(counts), return_lse=True)
+    want, wlse = ops.attend_shared_prefix(q, kc, vc, table, lens, **args)
+    others = torch.ones(q.shape[:2], dtype=torch.bool, device="cuda")
+    others[-1, -1] = False
+    old = q[-1, -1].clone()
+    for value in (math.nan, math.inf):
+        q[-1, -1, 5] = value
+        got, lse = ops.attend_shared_prefix(q, kc, vc, table, lens, **args)
+        q[-1, -1] = old
+        assert torch.equal(got[others], want[others]) and torch.equal(lse[others], wlse[others])
+        assert got[-1, -1].isnan().all() and lse[-1, -1].isnan()
+    q[-1, -1] = 0
+    q[-1, -1, 5] = 1
+    kc[..., kv - 1, :] = 0
+    kc[..., kv - 1, 5] = -math.inf
+    got, lse = ops.attend_shared_prefix(q, kc, vc, table, lens, **args)
+    assert not got[-1, -1].any() and lse[-1, -1] == -math.inf
+
+
 def test_attend_query_strides():
     counts, lengths = [1, 1, 1], [20, 9, 33]
     q, kc, vc, table, lens, pages, _ = paged(8, counts, lengths, 40, 6, 2, 64, 16, F16)

@@ -238,7 +238,8 @@ def attend_shared_prefix(q, k_cache, v_cache, page_table, lengths, *, prefix_pag
     it (int32, batch + 1 entries) rows ``query_offsets[b]`` to ``query_offsets[b + 1]`` are
     its new tokens, at most ``max_queries`` of them; each sees the tokens up to
     itself.  Rows of ``q`` behind the last sequence may be anything, and theirs of
-    ``out`` are left as they were.  A token that sees nothing gets zeros.
+    ``out`` are left as they were.  A token that sees nothing, or whose scores are all
+    minus infinity, gets zeros (and -inf for its log).
 
     ``max_length``, the longest of ``lengths`` where the host knows it, only steers how
     the work is split (by default the table's width, which may be far more).
