@@ -387,6 +387,20 @@ def test_attend_several_tokens(dtype, heads_first, counts, lengths, prefix, head
     check_attend(case, counts, lengths, prefix)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("count,prefix,heads,kv,dim,page", [
+    (40, 13, 32, 8, 128, 16), (40, 200, 32, 8, 128, 128), (33, 128, 24, 8, 64, 32), (50, 257, 16, 8, 80, 8), (129, 1, 8, 8, 64, 256),
+])
+def test_attend_many_chunks_on_a_short_prefix(dtype, count, prefix, heads, kv, dim, page):
+    """Sequences' own blocks take the prefix too; some sequences have fewer new
+    tokens or none, none beside the new ones, or a tile and more."""
+    counts = [count] * 20 + [0, 1, count - 1, 5]
+    lengths = [n + (0, 1, 100, 250)[i % 4] for i, n in enumerate(counts)]
+    lengths[20] = 0
+    case = paged(prefix, counts, lengths, prefix, heads, kv, dim, page, dtype, spare=2)
+    check_attend(case, counts, lengths, prefix)
+
+
 @pytest.mark.parametrize("spare,hint", [(0, 300), (0, 1), (500, None), (500, 300)])
 def test_attend_wide_tables_and_hints(spare, hint):
     """A table far wider than its sequences, and hints about the longest, right or
@@ -425,7 +439,7 @@ def test_attend_leaves_rows_behind_the_last_sequence():
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("counts,lengths,prefix,heads,kv,dim", [
     ([6, 2], [40, 2], 30, 2, 2, 64), ([3], [20], 0, 4, 1, 128), ([150, 40], [300, 40], 64, 4, 2, 128), ([200], [210], 0, 1, 1, 64),
-    ([5, 9], [100, 9], 20, 2, 1, 256), ([70, 3], [1000, 200], 0, 4, 2, 80),
+    ([5, 9], [100, 9], 20, 2, 1, 256), ([70, 3], [1000, 200], 0, 4, 2, 80), ([40] * 30, [50] * 30, 200, 16, 4, 64),
 ])
 def test_attend_odd_values_reach_only_who_sees_them(dtype, counts, lengths, prefix, heads, kv, dim):
     """Keys and values of new tokens that are infinite or not a number: tokens

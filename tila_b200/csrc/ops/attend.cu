@@ -24,6 +24,7 @@
 #include "attend_wide.cuh"
 
 #include <algorithm>
+#include <cmath>
 
 namespace {
 
@@ -704,6 +705,26 @@ int own_chunks_of(i64 keys, i64 blocks) {
   return static_cast<int>(std::max<i64>(1, std::min<i64>({(keys + kStep - 1) / kStep, 256, std::max(fill, even)})));
 }
 
+// Whether blocks of own tokens (wide, one chunk a sequence) should go through the prefix
+// too: then there are no partial results and no join, but a tile of keys serves 128
+// rows of one sequence where the prefix's own blocks fill 256 from all.  Estimates in us;
+// a tile takes 2.1 either way (at 64 elements 2.0 and 1.4), a wave of the prefix's blocks
+// 9.5 beside that, partial results are written and read at about 5 TB/s.  Measured so and
+// apart: 110 sequences of 42 tokens on 13 shared, 40 heads 82 and 200 us; 34 of up to 104 on
+// 1000, 56 heads 128 and 235, on 4000 302 and 378; 8 of 512 on 1000 87 and 173; 16 of 128
+// on 4096, 16 heads of 64 elements 88 and 68; 87 of 40 on 1000, 4 heads 59 and 44.
+bool inside_is_faster(const AttendParams &p, i64 rows, i64 own_blocks) {
+  const double tiles = (p.prefix + 127) / 128, chunks = p.prefix_chunks;
+  const i64 blocks = std::min<i64>(own_blocks, (rows / 128 + p.batch) * p.kv_heads);   // that have rows
+  double waves = blocks / (2. * kSms);
+  if (waves < 2) waves = std::ceil(waves);
+  const double inside = waves * tiles * (p.dim <= 64 ? 2.0 : 2.1);
+  const double prefix_waves = std::ceil((rows + 255) / 256 * p.kv_heads * chunks / kSms);
+  const double apart = prefix_waves * (9.5 + std::ceil(tiles / chunks) * (p.dim <= 64 ? 1.4 : 2.1));
+  const double join = 3 + 8. * (chunks + 1) * rows * p.kv_heads * p.dim / 5e6;
+  return inside < 0.9 * (apart + join);
+}
+
 Plan plan(const tila_attend_args &a) {
   Plan r{};
   AttendParams &p = r.p;
@@ -781,6 +802,11 @@ Plan plan(const tila_attend_args &a) {
     p.own_least = static_cast<int>(std::min<i64>(512, (own_keys / p.own_chunks + kStep - 1) / kStep * kStep));
   p.own_least = std::max(p.own_least, p.own_unit);
   if (p.own_chunks == 0 && p.prefix_chunks == 0) p.own_chunks = 1;   // no keys at all: a block writes the zeros
+  if (r.own_wide && r.prefix_wide && p.own_chunks == 1 && inside_is_faster(p, rows, own_blocks)) {
+    p.prefix_inside = 1;
+    p.prefix_chunks = 0;
+    r.prefix_wide = false;
+  }
   r.slots = p.prefix_chunks + p.own_chunks;
   p.direct = r.slots == 1 && p.prefix_chunks == 0;
   return r;

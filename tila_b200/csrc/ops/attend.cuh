@@ -36,6 +36,7 @@ struct AttendParams {
   int own_chunks, own_unit;         // slots prefix_chunks ..: a sequence's own tokens in equal parts of whole units,
   int own_least;                    // and of so many keys at least
   int direct;                       // one chunk in all: blocks write the result itself
+  int prefix_inside;                // own tokens' blocks (wide, one chunk) take the prefix too
   int q_words, q_vectors;           // q can be read in 4-byte words, in 16-byte vectors
   int out_vectors;                  // out can be written in vectors of 4 elements
 };

@@ -22,7 +22,8 @@
 // are joined at the end.  Either way the tensor core works for one while the other is
 // in its softmax.  Sequences' own tokens: many blocks of few tiles, so one warpgroup
 // and 128 rows a block, two blocks a multiprocessor, which also hide each other's
-// beginnings and ends (11 us of a block's 15 at 4 tiles).  Weights P (rounded to the
+// beginnings and ends (11 us of a block's 15 at 4 tiles); where that is faster, they go
+// through the prefix first and write the result itself.  Weights P (rounded to the
 // values' type) go through tensor memory in the place of S.
 //
 // tcgen05 operations of one thread run in order: S of a warpgroup's next tile,
@@ -209,13 +210,17 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
   }
   const int row0 = pair * G * kTile;
   if (row0 >= rows || (begin >= end && !p.direct)) return;
+  // own tokens: tiles of the prefix before them, where the block takes it too
+  const int before = kOwn && p.prefix_inside ? (p.prefix + kTile - 1) / kTile : 0;
+  const auto first_key = [&](int tile) { return tile < before ? tile * kTile : begin + (tile - before) * kTile; };
+  const auto keys_end = [&](int tile) { return tile < before ? p.prefix : end; };
   const bool shared_rows = G == 2 && rows - row0 <= kTile;   // one row tile: the warpgroups take tiles in turn
-  const int tiles = end > begin ? (end - begin + kTile - 1) / kTile : 0;
+  const int tiles = before + (end > begin ? (end - begin + kTile - 1) / kTile : 0);
   const int ahead = shared_rows ? 2 : 1;             // S is issued so many tiles ahead of P V
   // tiles from here on hold keys that some rows see and others do not (3 at most: a
   // block's tokens are 256 or fewer)
   const int least = kOwn ? limit0 + row0 / p.group : end;
-  const int mixed = least >= end ? tiles : max(0, least - begin) / kTile;
+  const int mixed = least >= end ? tiles : before + max(0, least - begin) / kTile;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < W::kStages; ++i) {
@@ -260,16 +265,16 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
     const int box_rows = min(p.page_size, kTile);
     const int box = lane / kHalves, half = lane % kHalves;
     auto look_up = [&](int tile) {
-      const int key = begin + tile * kTile + box * box_rows;
-      if (box * box_rows >= kTile || key >= end) return 0;
+      const int key = first_key(tile) + box * box_rows;
+      if (box * box_rows >= kTile || key >= keys_end(tile)) return 0;
       int page, row;
       split_key(p, key, page, row);
-      return pages[page];
+      return tile < before ? p.prefix_pages[page] : pages[page];
     };
     auto copy = [&](int item, int tile, int page, const TensorMap *map) -> bool {
       const int stage = item % W::kStages;
-      const int key0 = begin + tile * kTile;
-      const int boxes = (min(kTile, end - key0) + box_rows - 1) / box_rows;   // pages that hold seen keys
+      const int key0 = first_key(tile);
+      const int boxes = (min(kTile, keys_end(tile) - key0) + box_rows - 1) / box_rows;   // pages that hold seen keys
       int index, row;
       split_key(p, key0 + box * box_rows, index, row);
       if (item >= W::kStages &&
@@ -301,7 +306,7 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
   } else if (warp == kMmas) {
     // ---- MMAs -------------------------------------------------------------------
     const u32 base4 = uniform(tila::smem_u32(smem)) >> 4, tm = uniform(tmem);
-    const int n_tiles = static_cast<int>(uniform(tiles)), key_end = static_cast<int>(uniform(end));
+    const int n_tiles = static_cast<int>(uniform(tiles));
     const bool turns = uniform(shared_rows) != 0;                 // the warpgroups take tiles in turn
     const bool second = G == 2 && uniform(rows - row0 > kTile) != 0;        // the second row tile exists
     const int lead = turns ? 2 : 1, first_mixed = static_cast<int>(uniform(mixed));
@@ -347,7 +352,7 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
       ok = wait_full(values) && (!more || wait_full(keys));
       if (!ok) break;
       if (kOwn && j >= first_mixed && elected()) tila::mbar_arrive(&bars.loaded[j - first_mixed]);
-      const int seen = min(kTile, key_end - (begin + j * kTile));
+      const int seen = static_cast<int>(uniform(min(kTile, keys_end(j) - first_key(j))));
       const int steps = static_cast<int>(uniform((seen + 15) >> 4));
       if (seen & 15) {
         // values behind the end, up to the group of 16 that P V covers
@@ -400,7 +405,7 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
         unsigned char *v = smem + W::kRing + (item % W::kStages) * W::kTileBytes;
         // (not the ring's own barrier, whose phases this warp does not follow)
         ok = warp_wait(&bars.loaded[j - mixed], 0, p.err, __LINE__, dead_ptr);
-        const int seen = min(kTile, end - (begin + j * kTile));
+        const int key0 = first_key(j), seen = min(kTile, end - key0);
         for (int i = threadIdx.x - 32 * kLooks; ok && i < seen * (DP / 8); i += 64) {
           const int r = i / (DP / 8), c = i % (DP / 8);
           unsigned char *at = v + (c / 8) * kHalf + r * 128 + (((c % 8) ^ (r & 7)) << 4);
@@ -410,7 +415,7 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
             for (int k = 0; k < 8; ++k) {
               const float x = Elem<T>::get(e[k]);
               if (fabsf(x) < __builtin_huge_valf()) continue;
-              atomicMin(&odd.first[x != x ? 0 : x > 0.f ? 1 : 2][c * 8 + k], begin + j * kTile + r);
+              atomicMin(&odd.first[x != x ? 0 : x > 0.f ? 1 : 2][c * 8 + k], key0 + r);
               odd.any = 1;
               e[k] = Elem<T>::put(0.f);
             }
@@ -486,8 +491,7 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
         tila::tc_fence_before();
         tila::mbar_arrive(&bars.taken[w]);
       }
-      const int key0 = begin + j * kTile;
-      const int seen = min(end, limit) - key0;              // columns that the row sees
+      const int seen = (j < before ? p.prefix : min(end, limit)) - first_key(j);   // columns that the row sees
       if (__any_sync(0xffffffffu, seen < kTile)) {
 #pragma unroll
         for (int i = 0; i < kTile; ++i) s[i] = i < seen ? s[i] : kNegInf;
