@@ -27,7 +27,7 @@
 // conversions are on pairs of floats.
 //
 // Measured (B200): rotate gradient of 4 x 2048 tokens x 32 heads x 128, 32 bits: 46 us,
-// 5.8 TB/s; norm_rotate of 8192 tokens x 40 heads x 128, bf16: 35 us, 4.8 TB/s, its
+// 5.8 TB/s; norm_rotate of 8192 tokens x 40 heads x 128, bf16: 33 us, 5.1 TB/s, its
 // gradient 58 us; append of 16384 tokens with 32 query and 8 key heads 72 us, 5.6 TB/s.
 // Tried and not kept: a warp for each token with sines and weights in registers (norms
 // 57 us where this form took 40), and the same with rows through a ring in shared
@@ -803,6 +803,8 @@ int dispatch(const Params &p, const tila_rotary_args &a, int v, bool backward, c
     if (v == 8 && p.across) TILA_ROTARY(8, 1, true);
     if (v == 8) TILA_ROTARY(8, 1, false);
   } else {
+    // (one unit a lane where that is enough: 20 of 80 elements, 84 MB each way 70 -> 45 us)
+    if (v == 4 && p.across && per_lane == 1) TILA_ROTARY(4, 1, true);
     if (v == 4 && p.across) TILA_ROTARY(4, 2, true);
     if (v == 4 && per_lane == 1) TILA_ROTARY(4, 1, false);
   }
