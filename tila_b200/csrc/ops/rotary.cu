@@ -28,7 +28,7 @@
 //
 // Measured (B200): rotate gradient of 4 x 2048 tokens x 32 heads x 128, 32 bits: 46 us,
 // 5.8 TB/s; norm_rotate of 8192 tokens x 40 heads x 128, bf16: 33 us, 5.1 TB/s, its
-// gradient 58 us; append of 16384 tokens with 32 query and 8 key heads 72 us, 5.6 TB/s.
+// gradient 57 us; append of 16384 tokens with 32 query and 8 key heads 72 us, 5.6 TB/s.
 // Tried and not kept: a warp for each token with sines and weights in registers (norms
 // 57 us where this form took 40), and the same with rows through a ring in shared
 // memory (norms 41 us, but 107 us for the append and 7 us for 64 tokens).
@@ -127,6 +127,18 @@ __device__ __forceinline__ void load_row(const Units<V, K> &u, const T *row, Raw
   for (int k = 0; k < K; ++k) {
     r.a[k] = *reinterpret_cast<const Vec<T, V> *>(row + u.first[k]);
     r.b[k] = *reinterpret_cast<const Vec<T, V> *>(row + u.second[k]);
+  }
+}
+
+// Asks for a row that will be loaded later: into L2, no registers wait for it.  The
+// gradient's two rows of 16 warps a multiprocessor are too few bytes in flight (59.5 ->
+// 57.4 us); the forward kernel's 32 warps have enough and would lose (append 74 -> 87 us).
+template <typename T, int V, int K>
+__device__ __forceinline__ void fetch_row(const Units<V, K> &u, const T *row) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(row + u.first[k]));
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(row + u.second[k]));
   }
 }
 
@@ -339,6 +351,27 @@ __device__ __forceinline__ float row_sum(const Params &p, const Lane<V, K> &x, c
   return s;
 }
 
+// Those of x x and x y, whose exchanges run side by side.
+template <int V, int K>
+__device__ __forceinline__ float2 row_sums(const Params &p, const Lane<V, K> &x, const Lane<V, K> &y) {
+  u64 xx = 0, xy = 0;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      xx = tila::fma2(x[k][i], x[k][i], xx);
+      xy = tila::fma2(x[k][i], y[k][i], xy);
+    }
+  float2 s = make_float2(tila::lo2(xx) + tila::hi2(xx), tila::lo2(xy) + tila::hi2(xy));
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1)
+    if (m < p.lanes) {
+      s.x += __shfl_xor_sync(0xffffffffu, s.x, m);
+      s.y += __shfl_xor_sync(0xffffffffu, s.y, m);
+    }
+  return s;
+}
+
 // x * w of the elements that a lane holds.
 template <int V, int K>
 __device__ __forceinline__ void times_weight(const Units<V, K> &u, const float *w, Lane<V, K> &x) {
@@ -538,24 +571,35 @@ rotary_norm_backward_kernel(const __grid_constant__ Params p) {
           }
         }
         if (first + groups < jobs) load();
+        if (job + groups < jobs) {
+          const int over = h + dh >= r.heads, at_t = t + dt + over, at_h = h + dh - (over ? r.heads : 0);
+          fetch_row<T, V, K>(units, src + row_at(at_t, r.src_token, at_h, r.src_head));
+          fetch_row<T, V, K>(units, grad + row_at(at_t, r.grad_token, at_h, r.grad_head));
+        }
         if (r.flags & TILA_ROWS_ROTATE) {
           if constexpr (kAcross) turn_across<V, K>(p, units, partners, tab + at * p.token_table, scratch + group * p.row_floats, lane, g);
           else turn<V, K>(p, units, tab + 2 * at * p.half, lane, g);
         }
-        const float rms = rsqrtf(row_sum<V, K>(p, x, x) * p.inv_dim + p.eps);
+        Lane<V, K> wg;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int i = 0; i < V; ++i) wg[k][i] = g[k][i];
+        times_weight<V, K>(units, weights + tensor * p.weight_floats, wg);
+        const float2 sums = row_sums<V, K>(p, x, wg);                // of x^2 and w g x, at once
+        const float rms = rsqrtf(sums.x * p.inv_dim + p.eps);
         times<V, K>(rms, x);                                        // xh
         if (valid)
 #pragma unroll
           for (int k = 0; k < K; ++k)
 #pragma unroll
             for (int i = 0; i < V; ++i) sum[k][i] = tila::fma2(g[k][i], x[k][i], sum[k][i]);
-        times_weight<V, K>(units, weights + tensor * p.weight_floats, g);   // w g
-        const float mean = row_sum<V, K>(p, g, x) * p.inv_dim;
+        const float mean = rms * sums.y * p.inv_dim;
         const u64 minus = tila::pk2(-mean, -mean);
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-          for (int i = 0; i < V; ++i) x[k][i] = tila::fma2(x[k][i], minus, g[k][i]);
+          for (int i = 0; i < V; ++i) x[k][i] = tila::fma2(x[k][i], minus, wg[k][i]);
         times<V, K>(rms, x);
         if (valid)
           store_row<T, V, K>(units, dst + row_at(at, r.dst_token, head, r.dst_head), x);
