@@ -1,5 +1,6 @@
 """The decode-path operators on the GPU against their definitions in 64 bits."""
 
+import ctypes
 import math
 
 import pytest
@@ -695,3 +696,47 @@ def test_attend_on_another_stream_and_in_two_graphs():
     torch.cuda.synchronize()
     for got in outs:
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---------------------------------------------------------------------------
+# the C entries
+# ---------------------------------------------------------------------------
+
+def test_c_entry_of_a_tensor_without_heads():
+    """It has no rows, and none of its addresses is read: they may all be 0."""
+    from test_ops import FLAG_NORM, FLAG_ROTATE, HEAD, ROTARY_BYTES, ROWS
+    g = gen(13)
+    tokens, heads, dim = 5, 3, 64
+    x, gy, w = normal(g, tokens, heads, dim), normal(g, tokens, heads, dim), 1 + 0.3 * normal(g, dim)
+    positions, inv = torch.arange(tokens, device="cuda"), freqs(dim)
+    none = x[:, :0]
+    want = ops.norm_rotate(x, none, w, w, positions, inv)[0]
+    want_dx, _, want_dw, _ = ops.norm_rotate_backward(gy, none, x, none, w, w, positions, inv)
+    entries = native.library()
+    entries.tila_rotary_workspace.restype = ctypes.c_uint64
+
+    def call(entry, out, grad, weight_grads, first):
+        flags = FLAG_ROTATE | FLAG_NORM
+        full = ROWS.pack(x.data_ptr(), out.data_ptr(), w.data_ptr(), grad, 0, heads * dim, dim, 0, heads * dim, dim, 0,
+                         heads * dim, dim, heads, flags | 8)
+        empty = ROWS.pack(0, 0, 0, 0, *[0] * 9, 0, flags)
+        rows = (full + empty if first else empty + full) + bytes(ROWS.size)
+
+        def args(space, size):
+            return HEAD.pack(ROTARY_BYTES, 0, 1, tokens, dim, dim, 0, 0, 1.0, 1e-6, positions.data_ptr(), 0, 1,
+                             inv.data_ptr(), 0, 0, 0, 0, 1, 2, 0, 0, torch.cuda.current_stream().cuda_stream, space, size,
+                             *weight_grads) + rows
+
+        size = entries.tila_rotary_workspace(args(0, 0)) if grad else 0
+        space = torch.empty(max(size, 1), dtype=torch.uint8, device="cuda")
+        log = ctypes.create_string_buffer(512)
+        assert getattr(entries, entry)(args(space.data_ptr(), size), log, ctypes.c_size_t(512)) == native.TILA_OK, log.value
+        torch.cuda.synchronize()
+
+    for first in (True, False):
+        out, dx = torch.empty_like(x), torch.empty_like(x)
+        dw = torch.full((2, dim), 7.0, device="cuda")
+        call("tila_rotary_rows", out, 0, (0, 0), first)
+        call("tila_rotary_norm_backward", dx, gy.data_ptr(), (dw[0].data_ptr(), dw[1].data_ptr()), first)
+        assert torch.equal(out, want) and torch.equal(dx, want_dx)
+        assert torch.equal(dw[0 if first else 1], want_dw) and not dw[1 if first else 0].any()

@@ -731,9 +731,10 @@ Params make_params(const tila_rotary_args &a, bool backward, int v, bool across)
     o.dst_token = static_cast<u32>(r.dst_stride[1]), o.dst_head = static_cast<u32>(r.dst_stride[2]);
     o.grad_token = static_cast<u32>(r.grad_stride[1]), o.grad_head = static_cast<u32>(r.grad_stride[2]);
     o.heads = r.heads;
-    o.flags = r.flags;
+    // a tensor without heads has no addresses to be read, its weight's among them
+    o.flags = r.heads > 0 ? r.flags : r.flags & ~TILA_ROWS_NORM;
     p.heads += r.heads;
-    p.any_norm |= (r.flags & TILA_ROWS_NORM) != 0;
+    p.any_norm |= (o.flags & TILA_ROWS_NORM) != 0;
     p.any_paged |= (r.flags & TILA_ROWS_PAGED) != 0;
     rotates = rotates || (r.flags & TILA_ROWS_ROTATE);
   }
