@@ -287,3 +287,34 @@ def test_c_attend_workspace():
     assert workspace("tila_attend_workspace", attend_args(prefix_length=0, table_width=1)) == 0
     assert workspace("tila_attend_workspace", attend_args(tokens=0, batch=0)) == 0
     assert native.library().tila_attend_shared_prefix(attend_args(tokens=0, batch=0), None, ctypes.c_size_t(0)) == native.TILA_OK
+
+
+def rotary_rows(flags, weight=4096, grad=0, heads=2):
+    """One tensor of tila_rotary_args, as rotary_args makes it."""
+    return ROWS.pack(4096, 4096, weight, grad, 0, 128, 64, 0, 128, 64, 0, 128, 64, heads, flags)
+
+
+FLAG_WEIGHT_F32 = 8
+
+
+@pytest.mark.parametrize("entry,change,row", [
+    ("tila_rotary_rows", dict(positions=4100), rotary_rows(FLAG_ROTATE)),                            # 64-bit positions
+    ("tila_rotary_rows", dict(positions=4098, index64=0), rotary_rows(FLAG_ROTATE)),
+    ("tila_rotary_rows", dict(inv_freq=4100), rotary_rows(FLAG_ROTATE)),
+    ("tila_rotary_rows", dict(err=4100), rotary_rows(FLAG_ROTATE)),
+    ("tila_rotary_rows", dict(dtype=1), rotary_rows(FLAG_NORM, weight=4097)),
+    ("tila_rotary_rows", dict(dtype=1), rotary_rows(FLAG_NORM | FLAG_WEIGHT_F32, weight=4098)),
+    ("tila_rotary_rows", dict(slots=4100, num_slots=8, page=4, index64=2), rotary_rows(FLAG_PAGED)),
+    ("tila_rotary_rows", dict(slots=4098, num_slots=8, page=4, index64=0), rotary_rows(FLAG_PAGED)),
+    ("tila_rotary_norm_backward", dict(dw0=4098, workspace=4096, workspace_bytes=1 << 20),
+     rotary_rows(FLAG_NORM | FLAG_WEIGHT_F32, grad=4096)),
+])
+def test_c_entry_refuses_unaligned_addresses(entry, change, row):
+    refused(entry, rotary_args(rows=1, **change)[:HEAD.size] + row + bytes(2 * ROWS.size))
+
+
+@pytest.mark.parametrize("change", [dict(lengths=4098), dict(page_table=4097), dict(prefix_pages=4098),
+                                    dict(query_offsets=4098, max_queries=4), dict(err=4100)])
+def test_c_attend_refuses_unaligned_addresses(change):
+    # (a workspace that is large enough, so that only the address is at fault)
+    refused("tila_attend_shared_prefix", attend_args(workspace=4096, workspace_bytes=1 << 40, **change))

@@ -634,6 +634,8 @@ int check(const tila_attend_args *a, char *log, size_t cap) {
       return fail(TILA_ERR_ARGUMENT, log, cap, "%s: an address is missing or not aligned to its elements", who);
     if (a->lengths == 0 || (a->table_width > 0 && a->page_table == 0) || (a->prefix_length > 0 && a->prefix_pages == 0))
       return fail(TILA_ERR_ARGUMENT, log, cap, "%s: lengths or pages are missing", who);
+    if ((a->lengths | a->page_table | a->query_offsets | a->prefix_pages) % 4 != 0 || a->err % 8 != 0)
+      return fail(TILA_ERR_ARGUMENT, log, cap, "%s: lengths, offsets, pages or err are not aligned to their elements", who);
     bool ok = a->k_cache % 16 == 0 && a->v_cache % 16 == 0;
     for (int i = 0; i < 3; ++i) ok = ok && a->k_stride[i] % 8 == 0 && a->v_stride[i] % 8 == 0;
     if (!ok || (a->num_pages > 0 && (a->k_cache == 0 || a->v_cache == 0)))

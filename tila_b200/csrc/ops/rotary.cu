@@ -692,19 +692,26 @@ int check(const tila_rotary_args *a, bool backward, char *log, size_t cap) {
     const u64 size = a->dtype == TILA_F32 ? 4 : 2;
     if (a->batch > 0 && a->tokens > 0 && r.heads > 0 &&
         (r.src == 0 || r.dst == 0 || r.src % size != 0 || r.dst % size != 0 || r.grad % size != 0 ||
-         (backward && r.grad == 0) || ((r.flags & TILA_ROWS_NORM) && r.weight == 0)))
+         (backward && r.grad == 0) ||
+         ((r.flags & TILA_ROWS_NORM) &&
+          (r.weight == 0 || r.weight % ((r.flags & TILA_ROWS_WEIGHT_F32) ? 4 : size) != 0))))
       return fail(TILA_ERR_ARGUMENT, log, cap, "%s: an address is missing or not aligned to its elements", who);
     const int64_t *strides[3] = {r.src_stride, r.dst_stride, r.grad_stride};
     for (int k = 0; k < (backward ? 3 : 2); ++k)
       for (int d = 1; d < 3; ++d)
         if (strides[k][d] < 0 || strides[k][d] > 0xffffffffll)
           return fail(TILA_ERR_ARGUMENT, log, cap, "%s: strides of tokens and heads must be below 2^32 elements", who);
-    if (backward && (!(r.flags & TILA_ROWS_NORM) || (r.flags & TILA_ROWS_PAGED) || a->weight_grad[i] == 0))
+    if (backward && (!(r.flags & TILA_ROWS_NORM) || (r.flags & TILA_ROWS_PAGED) || a->weight_grad[i] == 0 ||
+                     a->weight_grad[i] % 4 != 0))
       return fail(TILA_ERR_ARGUMENT, log, cap, "%s: rows must be normed and have a weight gradient", who);
     rotates = rotates || (r.flags & TILA_ROWS_ROTATE);
     paged = paged || (r.flags & TILA_ROWS_PAGED);
   }
   const bool any = a->batch > 0 && a->tokens > 0;
+  if (a->err % 8 != 0 ||
+      (any && ((rotates && (a->positions % ((a->index64 & 1) ? 8 : 4) != 0 || a->inv_freq % 8 != 0)) ||
+               (paged && a->slots % ((a->index64 & 2) ? 8 : 4) != 0))))
+    return fail(TILA_ERR_ARGUMENT, log, cap, "%s: positions, inv_freq, slots or err are not aligned to their elements", who);
   if (any && rotates && a->rotary > 0 && (a->positions == 0 || a->inv_freq == 0))
     return fail(TILA_ERR_ARGUMENT, log, cap, "%s: positions and inv_freq are needed to rotate", who);
   if (paged && ((any && a->slots == 0) || a->page_size < 1 || a->num_slots < 0 || a->batch != 1))
