@@ -318,3 +318,13 @@ def test_c_entry_refuses_unaligned_addresses(entry, change, row):
 def test_c_attend_refuses_unaligned_addresses(change):
     # (a workspace that is large enough, so that only the address is at fault)
     refused("tila_attend_shared_prefix", attend_args(workspace=4096, workspace_bytes=1 << 40, **change))
+
+
+def test_c_entries_refuse_sizes_whose_product_passes_64_bits():
+    for batch in (1, 4):
+        refused("tila_rotary_rows", rotary_args(batch=batch, tokens=1 << 62))
+        args = rotary_args(batch=batch, tokens=1 << 62, dw0=4096)[:HEAD.size] + rotary_rows(FLAG_NORM, grad=4096) + bytes(2 * ROWS.size)
+        refused("tila_rotary_norm_backward", args)
+        assert workspace("tila_rotary_workspace", args) == 0
+    refused("tila_attend_shared_prefix", attend_args(tokens=1 << 61, workspace=4096, workspace_bytes=1 << 60))
+    assert workspace("tila_attend_workspace", attend_args(tokens=1 << 61)) == 0

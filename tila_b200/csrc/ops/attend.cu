@@ -623,7 +623,7 @@ int check(const tila_attend_args *a, char *log, size_t cap) {
   if (a->page_size < 1 || a->table_width < 0 || a->max_queries < 1 || a->num_pages < 0 || a->prefix_length < 0)
     return fail(TILA_ERR_ARGUMENT, log, cap, "%s: a size is out of range", who);
   constexpr i64 most = 1ll << 30;
-  if (a->num_pages > 0x7fffffff || a->prefix_length > most ||
+  if (a->num_pages > 0x7fffffff || a->prefix_length > most || a->tokens > most ||
       static_cast<i64>(a->table_width) * a->page_size > most || a->tokens * a->heads > most ||
       static_cast<i64>(a->max_queries) * a->heads > most)
     return fail(TILA_ERR_ARGUMENT, log, cap, "%s: more than 2^30 tokens or rows", who);

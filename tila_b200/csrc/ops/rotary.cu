@@ -683,6 +683,8 @@ int check(const tila_rotary_args *a, bool backward, char *log, size_t cap) {
   if (a->batch < 0 || a->tokens < 0 || a->batch > 0x7fffffff || a->dim < 1 || a->dim > 512 || a->rotary < 0 || a->rotary > a->dim ||
       a->rotary % 2 != 0)
     return fail(TILA_ERR_ARGUMENT, log, cap, "%s: dim must be 1 to 512 and rotary an even number up to dim", who);
+  if (a->batch > 0 && a->tokens > (1ll << 46) / a->batch)     // (times blocks and threads that is still below 2^63)
+    return fail(TILA_ERR_ARGUMENT, log, cap, "%s: more than 2^46 tokens", who);
   if (a->num_rows < 1 || a->num_rows > (backward ? 2 : 3))
     return fail(TILA_ERR_ARGUMENT, log, cap, "%s: num_rows out of range", who);
   bool rotates = false, paged = false;
