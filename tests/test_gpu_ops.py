@@ -740,3 +740,15 @@ def test_c_entry_of_a_tensor_without_heads():
         call("tila_rotary_norm_backward", dx, gy.data_ptr(), (dw[0].data_ptr(), dw[1].data_ptr()), first)
         assert torch.equal(out, want) and torch.equal(dx, want_dx)
         assert torch.equal(dw[0 if first else 1], want_dw) and not dw[1 if first else 0].any()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("counts,prefix,heads,kv,dim,page", [
+    ([256, 100, 156], 2000, 64, 8, 64, 24), ([130, 3, 77], 1700, 64, 8, 256, 16), ([300, 1], 1100, 96, 32, 80, 1),
+])
+def test_attend_many_rows_in_the_narrow_form(dtype, counts, prefix, heads, kv, dim, page):
+    """Page and head sizes that the wide form does not take, with blocks enough
+    for chunks of the prefix longer than 512 keys."""
+    lengths = [n + 7 * i for i, n in enumerate(counts)]
+    case = paged(sum(counts), counts, lengths, prefix, heads, kv, dim, page, dtype)
+    check_attend(case, counts, lengths, prefix)

@@ -328,3 +328,34 @@ def test_c_entries_refuse_sizes_whose_product_passes_64_bits():
         assert workspace("tila_rotary_workspace", args) == 0
     refused("tila_attend_shared_prefix", attend_args(tokens=1 << 61, workspace=4096, workspace_bytes=1 << 60))
     assert workspace("tila_attend_workspace", attend_args(tokens=1 << 61)) == 0
+
+
+def attend_slots(tokens, batch, heads, kv, dim, page, prefix, own, queries):
+    """Partial results of each row that a call's workspace holds."""
+    space = workspace("tila_attend_workspace", attend_args(
+        tokens=tokens, batch=batch, heads=heads, kv_heads=kv, dim=dim, page_size=page, table_width=-(-own // page),
+        prefix_length=prefix, max_queries=queries, query_offsets=0 if queries == 1 else 4096, kp=page * kv * dim,
+        kr=kv * dim, kh=dim, vp=page * kv * dim, vr=kv * dim, vh=dim, num_pages=1 << 20))
+    slots, rest = divmod(space, tokens * heads * (dim + 1) * 4)
+    assert rest == 0
+    return slots
+
+
+@pytest.mark.parametrize("page", [1, 4, 24, 48, 96, 64])
+@pytest.mark.parametrize("tokens,batch,heads,kv,dim,prefix,own,queries,most", [
+    (64 * 128, 64, 32, 8, 128, 32768, 1024, 128, 2),       # chunks of prompts: 270 MB a slot
+    (8192, 1, 32, 8, 128, 131072, 8192, 8192, 2),          # one prompt on a long document
+    (2048, 16, 32, 8, 256, 32768, 512, 128, 4),
+    (128, 128, 32, 8, 256, 32768, 4096, 1, 24),            # a decode step: 17 MB a slot, and a prefix of 134 MB
+])
+def test_attend_workspace_is_bounded_for_any_page_size(page, tokens, batch, heads, kv, dim, prefix, own, queries, most):
+    """Where many rows are taken by the narrow form (these page sizes and heads of 256
+    elements), chunks are not cut finer than the blocks need."""
+    assert 1 <= attend_slots(tokens, batch, heads, kv, dim, page, prefix, own, queries) <= most
+
+
+def test_attend_few_rows_keep_their_chunks():
+    """One token each of few sequences: 74 chunks of a prefix fill the GPU, and
+    none of a longer one passes 512 keys."""
+    assert attend_slots(4, 4, 32, 8, 256, 16, 32768, 64, 1) == 74 + 1
+    assert attend_slots(4, 4, 32, 32, 256, 16, 32768, 64, 1) == 64 + 1
