@@ -3,7 +3,11 @@
 
 import ctypes
 import math
+import shutil
 import struct
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -359,3 +363,16 @@ def test_attend_few_rows_keep_their_chunks():
     none of a longer one passes 512 keys."""
     assert attend_slots(4, 4, 32, 8, 256, 16, 32768, 64, 1) == 74 + 1
     assert attend_slots(4, 4, 32, 32, 256, 16, 32768, 64, 1) == 64 + 1
+
+
+def test_a_copy_of_the_package_uses_its_own_library(tmp_path):
+    package = Path(ops.__file__).parent
+    copy = tmp_path / "tila_b200"
+    copy.mkdir()
+    for f in [*package.glob("*.py"), *package.glob("*.so")]:
+        shutil.copy(f, copy)
+    code = ("import sys; sys.path.insert(0, sys.argv[1]); from tila_b200 import ops\n"
+            "print({l.split()[-1] for l in open('/proc/self/maps') if 'libtila_b200.so' in l})")
+    got = subprocess.run([sys.executable, "-c", code, str(tmp_path)], check=True, capture_output=True, text=True,
+                         cwd=tmp_path).stdout
+    assert got.strip() == str({str(copy / "libtila_b200.so")})

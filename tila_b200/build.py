@@ -57,7 +57,8 @@ def build_library(verbose=False) -> Path:
 def build_binding(verbose=False) -> Path:
     """The operators' Python binding (csrc/ops/binding.cpp, module
     ``tila_b200._ops``): host C++ against the installed torch, linked with
-    ``libtila_b200.so`` beside it."""
+    ``libtila_b200.so`` beside it, by name: a copy of the package elsewhere
+    uses its own."""
     import sysconfig
     out = PKG / "_ops.so"
     lib = build_library(verbose)
@@ -71,7 +72,7 @@ def build_binding(verbose=False) -> Path:
            f"-I{home / 'include'}", f"-I{home / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
            f"-I{CUDA / 'include'}", f"-I{sysconfig.get_paths()['include']}", str(src),
            f"-L{home / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
-           str(lib), "-Wl,-rpath,$ORIGIN", "-o", str(out) + ".tmp"]
+           f"-L{lib.parent}", f"-l:{lib.name}", "-Wl,-rpath,$ORIGIN", "-o", str(out) + ".tmp"]
     subprocess.run(cmd, check=True, capture_output=not verbose)
     os.replace(str(out) + ".tmp", out)
     return out
