@@ -752,3 +752,46 @@ def test_attend_many_rows_in_the_narrow_form(dtype, counts, prefix, heads, kv, d
     lengths = [n + 7 * i for i, n in enumerate(counts)]
     case = paged(sum(counts), counts, lengths, prefix, heads, kv, dim, page, dtype)
     check_attend(case, counts, lengths, prefix)
+
+
+# ---------------------------------------------------------------------------
+# beside autograd
+# ---------------------------------------------------------------------------
+
+def test_tensors_written_in_place_count_it():
+    """A tensor that another operation saved for its backward pass and that an
+    operator then wrote is found out, as after torch's own in-place operations."""
+    g = gen(17)
+    positions, inv, w = torch.arange(6, device="cuda"), freqs(64), torch.ones(64, device="cuda")
+    q, k, gq, gk = (normal(g, 6, h, 64, dtype=BF16) for h in (4, 2, 4, 2))
+    kc, vc = normal(g, 2, 16, 2, 64, dtype=BF16), normal(g, 2, 16, 2, 64, dtype=BF16)
+    out = torch.empty_like(q)
+    table, lens = torch.zeros(6, 1, dtype=torch.int32, device="cuda"), torch.ones(6, dtype=torch.int32, device="cuda")
+    slots = torch.arange(6, device="cuda")
+    calls = [
+        (lambda: ops.rotate(q, positions, inv, out=out), [out]),
+        (lambda: ops.rotate(q, positions, inv, out=q), [q]),
+        (lambda: ops.rotate_backward(gq, positions, inv, out=gq), [gq]),
+        (lambda: ops.norm_rotate(q, k, w, w, positions, inv, q_out=q, k_out=k), [q, k]),
+        (lambda: ops.norm_rotate_backward(gq, gk, q, k, w, w, positions, inv, dq=q, dk=gk), [q, gk]),
+        (lambda: ops.append_paged(k, k, kc, vc, slots), [kc, vc]),
+        (lambda: ops.append_paged(k, k, kc, vc, slots, q=q, q_out=out), [kc, vc, out]),
+        (lambda: ops.attend_shared_prefix(q, kc, vc, table, lens, out=out), [out]),
+    ]
+    everything = [q, k, gq, gk, kc, vc, out, w, inv, positions, table, lens, slots]
+    for call, wrote in calls:
+        before = [t._version for t in everything]
+        call()
+        for t, v in zip(everything, before):
+            assert (t._version > v) == any(t is x for x in wrote)
+    scale = torch.ones((), device="cuda", requires_grad=True)
+    y = (q.float() * scale).sum() + (out * scale).float().sum()      # saves `out`
+    ops.rotate(q, positions, inv, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():                                     # tensors without versions
+        x = q.clone()
+        assert ops.rotate(x, positions, inv, out=x) is x
+        cache = kc.clone()
+        ops.append_paged(k, k, cache, vc, slots)
+    assert torch.equal(x, out)

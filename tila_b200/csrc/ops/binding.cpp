@@ -218,6 +218,12 @@ std::optional<Tensor> result(const char *fn, const char *what, PyObject *o, cons
   return out;
 }
 
+// Tells autograd that a tensor of the caller's was written: a backward pass that had
+// saved it finds out.
+void written(const Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 Tensor empty(at::IntArrayRef sizes, at::ScalarType dtype, const Tensor &like) {
   return Tensor(at::detail::empty_cuda(sizes, dtype, like.device(), std::nullopt));
 }
@@ -362,8 +368,9 @@ PyObject *rotate(PyObject *const *o) {
   destination(out, a.rows[0]);
   a.rows[0].flags = TILA_ROWS_ROTATE;
   run(tila_rotary_rows, "tila_rotary_rows", x, a, nullptr);
-  if (given) return Py_NewRef(o[5]);
-  return THPVariable_Wrap(std::move(out));
+  if (!given) return THPVariable_Wrap(std::move(out));
+  written(out);
+  return Py_NewRef(o[5]);
 }
 
 PyObject *pair_of(PyObject *a, PyObject *b) {
@@ -410,6 +417,8 @@ PyObject *norm_rotate(PyObject *const *o) {
   a.rows[0].flags |= TILA_ROWS_ROTATE;
   a.rows[1].flags |= TILA_ROWS_ROTATE;
   run(tila_rotary_rows, "tila_rotary_rows", q, a, nullptr);
+  if (q_given) written(q_out);
+  if (k_given) written(k_out);
   return pair_of(q_given ? Py_NewRef(o[9]) : THPVariable_Wrap(std::move(q_out)),
                  k_given ? Py_NewRef(o[10]) : THPVariable_Wrap(std::move(k_out)));
 }
@@ -460,6 +469,8 @@ PyObject *norm_rotate_backward(PyObject *const *o) {
   a.weight_grad[1] = address(dkw);
   Tensor workspace;
   run(tila_rotary_norm_backward, "tila_rotary_norm_backward", q, a, &workspace);
+  if (q_given) written(dq);
+  if (k_given) written(dk);
   PyObject *r = PyTuple_New(4);
   if (r == nullptr) throw Raised();
   PyTuple_SET_ITEM(r, 0, q_given ? Py_NewRef(o[11]) : THPVariable_Wrap(std::move(dq)));
@@ -558,6 +569,8 @@ PyObject *append_paged(PyObject *const *o) {
   a.page_size = static_cast<int32_t>(caches[0]->size(1));
   a.index64 |= slots.scalar_type() == at::kLong ? 2 : 0;
   run(tila_rotary_rows, "tila_rotary_rows", k, a, nullptr);
+  for (const Tensor *c : caches) written(*c);
+  if (given) written(q_out);
   if (q == nullptr) return Py_NewRef(Py_None);
   return given ? Py_NewRef(o[12]) : THPVariable_Wrap(std::move(q_out));
 }
@@ -690,6 +703,7 @@ PyObject *attend_shared_prefix(PyObject *const *o) {
   }
   char log[512] = "";
   check_status(tila_attend_shared_prefix(&a, log, sizeof(log)), "tila_attend_shared_prefix", log);
+  if (given) written(out);
   PyObject *out_o = given ? Py_NewRef(o[10]) : THPVariable_Wrap(std::move(out));
   return want_lse ? pair_of(out_o, THPVariable_Wrap(std::move(lse))) : out_o;
 }
