@@ -376,3 +376,28 @@ def test_a_copy_of_the_package_uses_its_own_library(tmp_path):
     got = subprocess.run([sys.executable, "-c", code, str(tmp_path)], check=True, capture_output=True, text=True,
                          cwd=tmp_path).stdout
     assert got.strip() == str({str(copy / "libtila_b200.so")})
+
+
+def test_what_autograd_would_have_to_record_is_refused():
+    """With gradients enabled; without them (under no_grad, in a Function's forward)
+    the call goes on to the next check, which here is that there is no GPU."""
+    offsets = dict(query_offsets=ints(4), max_queries=2)
+    calls = [
+        (lambda x, inv: ops.rotate(x, POS, inv), [dev(6, 2, 64), INV.clone()]),
+        (lambda x, out: ops.rotate(x, POS, INV, out=out), [dev(6, 2, 64), dev(6, 2, 64)]),
+        (lambda x: ops.rotate_backward(x, POS, INV), [dev(6, 2, 64)]),
+        (lambda *t: ops.norm_rotate(*t, POS, INV), [t.clone() for t in NORM.values()]),
+        (lambda *t: ops.norm_rotate_backward(*t, POS, INV), [dev(6, 4, 64), dev(6, 2, 64), *(t.clone() for t in NORM.values())]),
+        (lambda k, v, kc, vc, kw, q, qw: ops.append_paged(k, v, kc, vc, torch.arange(6), k_weight=kw, q=q, q_weight=qw),
+         [dev(6, 2, 64), dev(6, 2, 64), dev(3, 4, 2, 64), dev(3, 4, 2, 64), dev(64), dev(6, 4, 64), dev(64)]),
+        (lambda q, k, v: ops.attend_shared_prefix(q, k, v, ints(3, 2), ints(3), **offsets),
+         [ATTEND[n].clone() for n in ("q", "k_cache", "v_cache")]),
+    ]
+    for call, tensors in calls:
+        for t in tensors:
+            t.requires_grad_()
+            with pytest.raises(ValueError, match="requires a gradient"):
+                call(*tensors)
+            with torch.no_grad(), pytest.raises(ValueError, match="must be a CUDA"):
+                call(*tensors)
+            t.requires_grad_(False)

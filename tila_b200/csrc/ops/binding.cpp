@@ -10,6 +10,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/core/Tensor.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -197,16 +198,28 @@ void apart(const char *fn, const char *what, const Tensor &a, const char *other,
   refuse("%s: %s overlaps %s", fn, what, other);
 }
 
-// The caller's result after its checks (None: one is made once everything else is
-// checked).
 struct Named {
   const char *what;
   const Tensor *t;
 };
+
+// Refuses a call that autograd would have to record: its result would pass for a
+// constant, and gradients upstream of it would silently be zero.
+void unrecorded(const char *fn, std::initializer_list<Named> tensors) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Named &n : tensors)
+    if (n.t->requires_grad())
+      refuse("%s: %s requires a gradient, which autograd does not record here: call it under torch.no_grad(), or in a "
+             "torch.autograd.Function", fn, n.what);
+}
+
+// The caller's result after its checks (None: one is made once everything else is
+// checked).
 std::optional<Tensor> result(const char *fn, const char *what, PyObject *o, const Tensor &like,
                              std::initializer_list<Named> own, std::initializer_list<Named> others) {
   if (o == Py_None) return std::nullopt;
   const Tensor &out = tensor(fn, what, o);
+  unrecorded(fn, {{what, &out}});
   on_device_of(fn, what, out, like);
   of_dtype(fn, what, out, like.scalar_type());
   if (out.sizes() != like.sizes())
@@ -269,6 +282,7 @@ void positions(const char *fn, PyObject *pos_o, PyObject *freq_o, const Tensor &
     refuse("%s: inv_freq rotates %lld elements, the heads have %lld", fn, static_cast<long long>(2 * freq.size(0)),
            static_cast<long long>(x.size(-1)));
   if (freq.size(0) > 1 && freq.stride(0) != 1) refuse("%s: inv_freq must be contiguous", fn);
+  unrecorded(fn, {{"inv_freq", &freq}});
   a.rotary = static_cast<int32_t>(2 * freq.size(0));
   a.positions = address(pos);
   a.inv_freq = address(freq);
@@ -361,6 +375,7 @@ PyObject *rotate(PyObject *const *o) {
   a.amplitude = static_cast<float>(number(o[4]));
   a.inverse = inverse;
   std::optional<Tensor> given = result(fn, "out", o[5], x, {{what, &x}}, {});
+  unrecorded(fn, {{what, &x}});
   on_gpu(fn, what, x);
   Tensor out = given ? *given : empty(x.sizes(), x.scalar_type(), x);
   a.num_rows = 1;
@@ -397,8 +412,9 @@ PyObject *norm_rotate(PyObject *const *o) {
   const Tensor &q = tensor(fn, "q", o[0]), &k = tensor(fn, "k", o[1]);
   query_key(fn, q, k);
   tila_rotary_args a = rotary_args(q);
-  weight(fn, "q_weight", tensor(fn, "q_weight", o[2]), q, a.rows[0]);
-  weight(fn, "k_weight", tensor(fn, "k_weight", o[3]), k, a.rows[1]);
+  const Tensor &q_weight = tensor(fn, "q_weight", o[2]), &k_weight = tensor(fn, "k_weight", o[3]);
+  weight(fn, "q_weight", q_weight, q, a.rows[0]);
+  weight(fn, "k_weight", k_weight, k, a.rows[1]);
   layout(fn, o[6], a);
   positions(fn, o[4], o[5], q, a);
   a.amplitude = static_cast<float>(number(o[7]));
@@ -406,6 +422,7 @@ PyObject *norm_rotate(PyObject *const *o) {
   std::optional<Tensor> q_given = result(fn, "q_out", o[9], q, {{"q", &q}}, {{"k", &k}});
   std::optional<Tensor> k_given = result(fn, "k_out", o[10], k, {{"k", &k}}, {{"q", &q}});
   if (q_given && k_given) apart(fn, "k_out", *k_given, "q_out", *q_given);
+  unrecorded(fn, {{"q", &q}, {"k", &k}, {"q_weight", &q_weight}, {"k_weight", &k_weight}});
   on_gpu(fn, "q", q);
   Tensor q_out = q_given ? *q_given : empty(q.sizes(), q.scalar_type(), q);
   Tensor k_out = k_given ? *k_given : empty(k.sizes(), k.scalar_type(), k);
@@ -429,8 +446,9 @@ PyObject *norm_rotate_backward(PyObject *const *o) {
   const Tensor &q = tensor(fn, "q", o[2]), &k = tensor(fn, "k", o[3]);
   query_key(fn, q, k);
   tila_rotary_args a = rotary_args(q);
-  weight(fn, "q_weight", tensor(fn, "q_weight", o[4]), q, a.rows[0]);
-  weight(fn, "k_weight", tensor(fn, "k_weight", o[5]), k, a.rows[1]);
+  const Tensor &q_weight = tensor(fn, "q_weight", o[4]), &k_weight = tensor(fn, "k_weight", o[5]);
+  weight(fn, "q_weight", q_weight, q, a.rows[0]);
+  weight(fn, "k_weight", k_weight, k, a.rows[1]);
   layout(fn, o[8], a);
   positions(fn, o[6], o[7], q, a);
   a.amplitude = static_cast<float>(number(o[9]));
@@ -454,6 +472,8 @@ PyObject *norm_rotate_backward(PyObject *const *o) {
   std::optional<Tensor> k_given =
       result(fn, "dk", o[12], k, {{"k", &k}, {"k_grad", grads[1]}}, {{"q", &q}, {"q_grad", grads[0]}});
   if (q_given && k_given) apart(fn, "dk", *k_given, "dq", *q_given);
+  unrecorded(fn, {{"q_grad", grads[0]}, {"k_grad", grads[1]}, {"q", &q}, {"k", &k}, {"q_weight", &q_weight},
+                  {"k_weight", &k_weight}});
   on_gpu(fn, "q", q);
   Tensor dq = q_given ? *q_given : empty(q.sizes(), q.scalar_type(), q);
   Tensor dk = k_given ? *k_given : empty(k.sizes(), k.scalar_type(), k);
@@ -533,7 +553,12 @@ PyObject *append_paged(PyObject *const *o) {
   }
   apart(fn, "k_cache", *caches[0], "v_cache", *caches[1]);
   rk.flags |= turned;
-  if (o[9] != Py_None) weight(fn, "k_weight", tensor(fn, "k_weight", o[9]), k, rk);
+  unrecorded(fn, {{"k", &k}, {"v", &v}, {names[0], caches[0]}, {names[1], caches[1]}});
+  if (o[9] != Py_None) {
+    const Tensor &w = tensor(fn, "k_weight", o[9]);
+    weight(fn, "k_weight", w, k, rk);
+    unrecorded(fn, {{"k_weight", &w}});
+  }
   source(k, rk);
   source(v, rv);
   a.num_rows = 2;
@@ -548,7 +573,12 @@ PyObject *append_paged(PyObject *const *o) {
         q->size(2) != k.size(2))
       refuse("%s: q must be (%lld, heads, %lld) of k's device and dtype", fn, static_cast<long long>(k.size(0)),
              static_cast<long long>(k.size(2)));
-    if (o[11] != Py_None) weight(fn, "q_weight", tensor(fn, "q_weight", o[11]), *q, rq);
+    unrecorded(fn, {{"q", q}});
+    if (o[11] != Py_None) {
+      const Tensor &w = tensor(fn, "q_weight", o[11]);
+      weight(fn, "q_weight", w, *q, rq);
+      unrecorded(fn, {{"q_weight", &w}});
+    }
     given = result(fn, "q_out", o[12], *q, {{"q", q}},
                    {{"k", &k}, {"v", &v}, {"k_cache", caches[0]}, {"v_cache", caches[1]}});
     apart(fn, "k_cache", *caches[0], "q", *q);
@@ -664,6 +694,7 @@ PyObject *attend_shared_prefix(PyObject *const *o) {
   a.scale = o[9] == Py_None ? static_cast<float>(1.0 / std::sqrt(static_cast<double>(dim))) : static_cast<float>(number(o[9]));
   std::optional<Tensor> given =
       result(fn, "out", o[10], q, {}, {{"q", &q}, {"k_cache", caches[0]}, {"v_cache", caches[1]}});
+  unrecorded(fn, {{"q", &q}, {"k_cache", caches[0]}, {"v_cache", caches[1]}});
   on_gpu(fn, "q", q);
   Tensor out = given ? *given : empty(q.sizes(), q.scalar_type(), q);
   const bool want_lse = o[11] == Py_True;

@@ -14,7 +14,9 @@ kernels behind the C ABI (``include/tila_b200.h``, ``csrc/ops``).
 Like the kernels of a Tila program they take CUDA tensors of any strides whose
 last dimension is contiguous, write into tensors that the caller may supply,
 and run asynchronously on the current PyTorch stream of the tensors' device.
-They are not recorded by autograd: a gradient is a call of its own.  Every call
+They are not recorded by autograd: a gradient is a call of its own, and with
+gradients enabled a tensor that requires one is refused (``torch.no_grad()``, or a
+``torch.autograd.Function`` around the call and its gradient's).  Every call
 can be captured into a CUDA graph once an operator has run on the device.
 Wrong arguments raise ``ValueError`` before anything is launched.  What only the
 device can see (a slot outside the cache) leaves the access out, is recorded as
