@@ -2,6 +2,9 @@
 
 import ctypes
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -795,3 +798,33 @@ def test_tensors_written_in_place_count_it():
         cache = kc.clone()
         ops.append_paged(k, k, cache, vc, slots)
     assert torch.equal(x, out)
+
+
+def test_first_operator_in_inference_mode():
+    """The error block that it makes outlives the mode: a device error is raised
+    and reset outside of it too."""
+    code = """
+import torch
+from tila_b200 import native, ops
+kc, k = torch.zeros(1, 4, 1, 64, device="cuda"), torch.ones(1, 1, 64, device="cuda")
+vc = kc.clone()
+good, bad = torch.tensor([1], device="cuda"), torch.tensor([4], device="cuda")
+with torch.inference_mode():
+    ops.append_paged(k, k, kc, vc, good)
+for _ in range(2):
+    ops.append_paged(k, k, kc, vc, bad)
+    torch.cuda.synchronize()
+    try:
+        ops.append_paged(k, k, kc, vc, good)
+    except native.NativeError as e:
+        assert "outside its pool" in str(e)
+    else:
+        raise SystemExit("no error")
+    ops.append_paged(k, k, kc, vc, good)
+    torch.cuda.synchronize()
+    ops.check_errors()
+print("raised and reset")
+"""
+    got = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120,
+                         cwd=Path(__file__).resolve().parents[1])
+    assert got.returncode == 0 and "raised and reset" in got.stdout, got.stderr

@@ -57,7 +57,8 @@ class _ErrorBlock:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("the first operator on a device cannot be captured into a CUDA graph: "
                                "call it once before the capture")
-        with torch.cuda.device(index):
+        # (in inference mode it would be a tensor that check_errors could not reset outside of it)
+        with torch.inference_mode(False), torch.cuda.device(index):
             self.block = torch.zeros(native.ERROR_BLOCK_BYTES // 4, dtype=torch.int32, device="cuda")
             host, address = native.host_word_alloc()
             self.block.view(torch.int64)[1] = address
