@@ -401,3 +401,44 @@ def test_what_autograd_would_have_to_record_is_refused():
             with torch.no_grad(), pytest.raises(ValueError, match="must be a CUDA"):
                 call(*tensors)
             t.requires_grad_(False)
+
+
+def apart_rows(*size, stride):
+    """A tensor of that size whose rows lie far apart (nothing is allocated)."""
+    return torch.empty_strided(size, stride, device="meta")
+
+
+def test_sizes_and_strides_beyond_the_kernels_are_refused():
+    """As wrong arguments, before anything is allocated."""
+    far = 1 << 32
+    x, near = apart_rows(6, 2, 64, stride=(1 << 34, far, 1)), apart_rows(6, 2, 64, stride=(128, 64, 1))
+    pos, inv = torch.empty(6, dtype=torch.int64, device="meta"), torch.empty(32, dtype=torch.float64, device="meta")
+    w, text = torch.empty(64, device="meta"), "below 2\\^32 elements"
+    with pytest.raises(ValueError, match=f"x's.*{text}"):
+        ops.rotate(x, pos, inv)
+    with pytest.raises(ValueError, match=f"k's.*{text}"):
+        ops.norm_rotate(near, x, w, w, pos, inv)
+    with pytest.raises(ValueError, match=f"q_grad's.*{text}"):
+        ops.norm_rotate_backward(x, near, near, near, w, w, pos, inv)
+    # (empty ones, which do not overlap)
+    x, near, pos = x[:0], near[:0], pos[:0]
+    with pytest.raises(ValueError, match=f"out's.*{text}"):
+        ops.rotate(near, pos, inv, out=x)
+    cache = apart_rows(0, 4, 2, 64, stride=(512, 128, 64, 1))
+    with pytest.raises(ValueError, match=f"v's.*{text}"):
+        ops.append_paged(near, x, cache, cache, pos)
+    with pytest.raises(ValueError, match=f"v_cache's.*{text}"):
+        ops.append_paged(near, near, cache, apart_rows(0, 4, 2, 64, stride=(1 << 40, far, 64, 1)), pos)
+    with pytest.raises(ValueError, match=f"q's.*{text}"):
+        ops.append_paged(near, near, cache, cache, pos, q=x)
+
+    q, k = dev(1, 1, 64, dtype=H), dev(1, 1, 1, 64, dtype=H)
+    many = lambda rows, heads: q.expand(rows, heads, 64)                                  # noqa: E731
+    offsets = dict(query_offsets=ints(4), max_queries=1 << 21)
+    pages = k.expand(5, 1 << 20, 1, 64)
+    for args, kwargs in (((many(1 << 21, 1 << 10), *[k.expand(5, 8, 1, 64)] * 2, ints(3, 2), ints(3)), offsets),
+                         ((many(3, 1), pages, pages, ints(3, 1025), ints(3)), {}),
+                         ((many(3, 1), pages, pages, ints(3, 1), ints(3)),
+                          dict(prefix_pages=ints(1025), prefix_length=(1 << 30) + 1))):
+        with pytest.raises(ValueError, match="more than 2\\^30"):
+            ops.attend_shared_prefix(*args, **kwargs)

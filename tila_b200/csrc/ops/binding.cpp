@@ -90,6 +90,7 @@ uint64_t error_block(int index) {
 
 void check_status(int status, const char *entry, const char *log) {
   if (status == TILA_OK) return;
+  if (status == TILA_ERR_ARGUMENT) refuse("%s", log);
   const std::string message = std::string(entry) + ": " + tila_status_string(status);
   PyObject *e = PyObject_CallFunction(g_native_error, "iss", status, message.c_str(), log);
   if (e != nullptr) {
@@ -299,17 +300,21 @@ void layout(const char *fn, PyObject *o, tila_rotary_args &a) {
   }
 }
 
-// A stride of tokens or heads; that of a single one is never used and may be any (the
-// kernels take those strides in 32 bits).
-int64_t inner_stride(const Tensor &t, int d) {
-  return t.size(d) == 1 && t.stride(d) > int64_t{0xffffffff} ? 0 : t.stride(d);
+// A stride of tokens or heads, which the kernels take in 32 bits; that of a single one
+// is never used and may be any.
+int64_t inner_stride(const char *fn, const char *what, const Tensor &t, int d) {
+  if (t.stride(d) <= int64_t{0xffffffff}) return t.stride(d);
+  if (t.size(d) > 1)
+    refuse("%s: strides of %s's tokens and heads must be below 2^32 elements, not %lld", fn, what,
+           static_cast<long long>(t.stride(d)));
+  return 0;
 }
 
-void strides3(const Tensor &t, int64_t (&s)[3]) {
+void strides3(const char *fn, const char *what, const Tensor &t, int64_t (&s)[3]) {
   const bool batch = t.dim() == 4;
   s[0] = batch ? t.stride(0) : 0;
-  s[1] = inner_stride(t, batch ? 1 : 0);
-  s[2] = inner_stride(t, batch ? 2 : 1);
+  s[1] = inner_stride(fn, what, t, batch ? 1 : 0);
+  s[2] = inner_stride(fn, what, t, batch ? 2 : 1);
 }
 
 uint32_t weight(const char *fn, const char *what, const Tensor &w, const Tensor &x, tila_op_rows &r) {
@@ -336,14 +341,21 @@ tila_rotary_args rotary_args(const Tensor &x) {
   return a;
 }
 
-void source(const Tensor &x, tila_op_rows &r) {
+void source(const char *fn, const char *what, const Tensor &x, tila_op_rows &r) {
   r.src = address(x);
-  strides3(x, r.src_stride);
+  strides3(fn, what, x, r.src_stride);
   r.heads = static_cast<int32_t>(x.size(-2));
 }
-void destination(const Tensor &x, tila_op_rows &r) {
-  r.dst = address(x);
-  strides3(x, r.dst_stride);
+// The caller's result, whose strides are checked with the other arguments, or one made
+// for it.
+void destination(const char *fn, const char *what, const std::optional<Tensor> &given, tila_op_rows &r) {
+  if (given) strides3(fn, what, *given, r.dst_stride);
+}
+Tensor result_of(const std::optional<Tensor> &given, const Tensor &like, tila_op_rows &r) {
+  Tensor out = given ? *given : empty(like.sizes(), like.scalar_type(), like);
+  if (!given) strides3("", "", out, r.dst_stride);
+  r.dst = address(out);
+  return out;
 }
 
 // Launches on x's device and its current stream.
@@ -376,11 +388,11 @@ PyObject *rotate(PyObject *const *o) {
   a.inverse = inverse;
   std::optional<Tensor> given = result(fn, "out", o[5], x, {{what, &x}}, {});
   unrecorded(fn, {{what, &x}});
+  source(fn, what, x, a.rows[0]);
+  destination(fn, "out", given, a.rows[0]);
   on_gpu(fn, what, x);
-  Tensor out = given ? *given : empty(x.sizes(), x.scalar_type(), x);
+  Tensor out = result_of(given, x, a.rows[0]);
   a.num_rows = 1;
-  source(x, a.rows[0]);
-  destination(out, a.rows[0]);
   a.rows[0].flags = TILA_ROWS_ROTATE;
   run(tila_rotary_rows, "tila_rotary_rows", x, a, nullptr);
   if (!given) return THPVariable_Wrap(std::move(out));
@@ -423,14 +435,13 @@ PyObject *norm_rotate(PyObject *const *o) {
   std::optional<Tensor> k_given = result(fn, "k_out", o[10], k, {{"k", &k}}, {{"q", &q}});
   if (q_given && k_given) apart(fn, "k_out", *k_given, "q_out", *q_given);
   unrecorded(fn, {{"q", &q}, {"k", &k}, {"q_weight", &q_weight}, {"k_weight", &k_weight}});
+  source(fn, "q", q, a.rows[0]);
+  source(fn, "k", k, a.rows[1]);
+  destination(fn, "q_out", q_given, a.rows[0]);
+  destination(fn, "k_out", k_given, a.rows[1]);
   on_gpu(fn, "q", q);
-  Tensor q_out = q_given ? *q_given : empty(q.sizes(), q.scalar_type(), q);
-  Tensor k_out = k_given ? *k_given : empty(k.sizes(), k.scalar_type(), k);
+  Tensor q_out = result_of(q_given, q, a.rows[0]), k_out = result_of(k_given, k, a.rows[1]);
   a.num_rows = 2;
-  source(q, a.rows[0]);
-  destination(q_out, a.rows[0]);
-  source(k, a.rows[1]);
-  destination(k_out, a.rows[1]);
   a.rows[0].flags |= TILA_ROWS_ROTATE;
   a.rows[1].flags |= TILA_ROWS_ROTATE;
   run(tila_rotary_rows, "tila_rotary_rows", q, a, nullptr);
@@ -464,7 +475,7 @@ PyObject *norm_rotate_backward(PyObject *const *o) {
              text(g.sizes()).c_str());
     unit_last(fn, names[i], g);
     a.rows[i].grad = address(g);
-    strides3(g, a.rows[i].grad_stride);
+    strides3(fn, names[i], g, a.rows[i].grad_stride);
     grads[i] = &g;
   }
   std::optional<Tensor> q_given =
@@ -474,15 +485,14 @@ PyObject *norm_rotate_backward(PyObject *const *o) {
   if (q_given && k_given) apart(fn, "dk", *k_given, "dq", *q_given);
   unrecorded(fn, {{"q_grad", grads[0]}, {"k_grad", grads[1]}, {"q", &q}, {"k", &k}, {"q_weight", &q_weight},
                   {"k_weight", &k_weight}});
+  source(fn, "q", q, a.rows[0]);
+  source(fn, "k", k, a.rows[1]);
+  destination(fn, "dq", q_given, a.rows[0]);
+  destination(fn, "dk", k_given, a.rows[1]);
   on_gpu(fn, "q", q);
-  Tensor dq = q_given ? *q_given : empty(q.sizes(), q.scalar_type(), q);
-  Tensor dk = k_given ? *k_given : empty(k.sizes(), k.scalar_type(), k);
+  Tensor dq = result_of(q_given, q, a.rows[0]), dk = result_of(k_given, k, a.rows[1]);
   Tensor dqw = empty({q.size(-1)}, at::kFloat, q), dkw = empty({q.size(-1)}, at::kFloat, q);
   a.num_rows = 2;
-  source(q, a.rows[0]);
-  destination(dq, a.rows[0]);
-  source(k, a.rows[1]);
-  destination(dk, a.rows[1]);
   a.rows[0].flags |= TILA_ROWS_ROTATE;
   a.rows[1].flags |= TILA_ROWS_ROTATE;
   a.weight_grad[0] = address(dqw);
@@ -548,7 +558,7 @@ PyObject *append_paged(PyObject *const *o) {
     apart(fn, names[i], c, "v", v);
     tila_op_rows &r = a.rows[i];
     r.dst = address(c);
-    strides3(c, r.dst_stride);
+    strides3(fn, names[i], c, r.dst_stride);
     r.flags = TILA_ROWS_PAGED;
   }
   apart(fn, "k_cache", *caches[0], "v_cache", *caches[1]);
@@ -559,8 +569,8 @@ PyObject *append_paged(PyObject *const *o) {
     weight(fn, "k_weight", w, k, rk);
     unrecorded(fn, {{"k_weight", &w}});
   }
-  source(k, rk);
-  source(v, rv);
+  source(fn, "k", k, rk);
+  source(fn, "v", v, rv);
   a.num_rows = 2;
   std::optional<Tensor> given;
   const Tensor *q = nullptr;
@@ -584,12 +594,14 @@ PyObject *append_paged(PyObject *const *o) {
     apart(fn, "k_cache", *caches[0], "q", *q);
     apart(fn, "v_cache", *caches[1], "q", *q);
   }
+  if (q != nullptr) {
+    source(fn, "q", *q, rq);
+    destination(fn, "q_out", given, rq);
+  }
   on_gpu(fn, "k", k);
   Tensor q_out;
   if (q != nullptr) {
-    q_out = given ? *given : empty(q->sizes(), q->scalar_type(), *q);
-    source(*q, rq);
-    destination(q_out, rq);
+    q_out = result_of(given, *q, rq);
     rq.flags |= turned;
     a.num_rows = 3;
   }
@@ -689,8 +701,9 @@ PyObject *attend_shared_prefix(PyObject *const *o) {
     a.max_length = static_cast<int32_t>(std::min<int64_t>(longest, INT32_MAX));
   }
   constexpr int64_t limit = int64_t{1} << 30;
-  if (tokens > limit || batch > limit || table.size(1) > limit || most > limit)
-    refuse("%s: more than 2^30 tokens, sequences or pages", fn);
+  if (tokens > limit / heads || batch > limit || table.size(1) > limit / page_size || most > limit / heads ||
+      a.prefix_length > limit)
+    refuse("%s: more than 2^30 rows of queries, sequences, or tokens of one sequence or of the prefix", fn);
   a.scale = o[9] == Py_None ? static_cast<float>(1.0 / std::sqrt(static_cast<double>(dim))) : static_cast<float>(number(o[9]));
   std::optional<Tensor> given =
       result(fn, "out", o[10], q, {}, {{"q", &q}, {"k_cache", caches[0]}, {"v_cache", caches[1]}});
