@@ -442,3 +442,16 @@ def test_sizes_and_strides_beyond_the_kernels_are_refused():
                           dict(prefix_pages=ints(1025), prefix_length=(1 << 30) + 1))):
         with pytest.raises(ValueError, match="more than 2\\^30"):
             ops.attend_shared_prefix(*args, **kwargs)
+
+
+@pytest.mark.parametrize("kwargs", [
+    dict(base=1.0, scaling="yarn", original_length=100), dict(base=0.5, scaling="yarn", original_length=100),
+    dict(scaling="yarn", original_length=math.inf), dict(scaling="yarn", original_length=math.nan),
+    dict(scaling="yarn", original_length=100, beta_fast=math.inf), dict(base=math.inf), dict(base=math.nan),
+    dict(scaling="linear", factor=math.inf), dict(scaling="yarn", factor=math.inf, original_length=100),
+    dict(scaling="ntk", factor=1e300), dict(scaling="ntk", factor=1e298, base=1e10), dict(base=1e-320),
+])
+def test_frequencies_that_do_not_exist_are_refused(kwargs):
+    with pytest.raises(ValueError, match="rotary_frequencies"):
+        ops.rotary_frequencies(64, device="cpu", **kwargs)
+    assert ops.rotary_frequencies(64, base=1.0, device="cpu")[0].tolist() == [1.0] * 32

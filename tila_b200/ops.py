@@ -128,21 +128,28 @@ def rotary_frequencies(rotary, base=10000.0, scaling=None, factor=1.0, original_
     name = "rotary_frequencies"
     if rotary < 0 or rotary % 2:
         _fail(name, f"rotary must be an even number of elements, not {rotary}")
-    if not (base > 0 and factor >= 1.0):
-        _fail(name, "base must be positive and factor at least 1")
+    if not (0 < base < math.inf and 1.0 <= factor < math.inf):
+        _fail(name, "base must be positive and factor at least 1, both finite")
     if scaling not in (None, "linear", "ntk", "yarn"):
         _fail(name, f"scaling must be None, 'linear', 'ntk' or 'yarn', not {scaling!r}")
-    if scaling == "ntk" and rotary > 2:
-        base = base * factor ** (rotary / (rotary - 2))
-    freq = [base ** (-2.0 * i / rotary) for i in range(rotary // 2)]
+    try:
+        if scaling == "ntk" and rotary > 2:
+            base = base * factor ** (rotary / (rotary - 2))
+            if base == math.inf:
+                raise OverflowError
+        freq = [base ** (-2.0 * i / rotary) for i in range(rotary // 2)]
+    except OverflowError:
+        _fail(name, f"base {base} and factor {factor} give frequencies beyond 64-bit numbers")
     amplitude = 1.0
     if scaling == "linear":
         freq = [f / factor for f in freq]
     elif scaling == "yarn":
-        if not original_length or original_length < 1:
+        if base <= 1:
+            _fail(name, f"'yarn' needs frequencies that fall from pair to pair: a base above 1, not {base}")
+        if not original_length or not 1 <= original_length < math.inf:
             _fail(name, "'yarn' needs original_length, the length that the model was trained on")
-        if not beta_fast > beta_slow > 0:
-            _fail(name, "beta_fast must be above beta_slow, and both positive")
+        if not math.inf > beta_fast > beta_slow > 0:
+            _fail(name, "beta_fast must be above beta_slow, both positive and finite")
 
         def pair(turns):     # the pair (not whole) that turns so often over original_length
             return rotary * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(base))
