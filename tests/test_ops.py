@@ -455,3 +455,16 @@ def test_frequencies_that_do_not_exist_are_refused(kwargs):
     with pytest.raises(ValueError, match="rotary_frequencies"):
         ops.rotary_frequencies(64, device="cpu", **kwargs)
     assert ops.rotary_frequencies(64, base=1.0, device="cpu")[0].tolist() == [1.0] * 32
+
+
+def test_views_that_negate_are_refused():
+    """The imaginary part of a conjugate holds its values with the opposite sign."""
+    lazy = torch.zeros(6, 2, 1, dtype=torch.complex64).conj().imag
+    assert lazy.is_neg()
+    none = torch.ones(0, dtype=torch.float64)
+    for call in (lambda: ops.rotate(lazy, POS, none), lambda: ops.rotate(dev(6, 2, 1), POS, none, out=lazy),
+                 lambda: ops.norm_rotate(lazy, dev(6, 2, 1), dev(1), dev(1), POS, none)):
+        with pytest.raises(ValueError, match="negates"):
+            call()
+    with pytest.raises(ValueError, match="must be a CUDA"):
+        ops.rotate(lazy.resolve_neg(), POS, none)

@@ -106,7 +106,10 @@ void check_status(int status, const char *entry, const char *log) {
 
 const Tensor &tensor(const char *fn, const char *what, PyObject *o) {
   if (!THPVariable_Check(o)) mistyped("%s: %s must be a tensor, not %s", fn, what, Py_TYPE(o)->tp_name);
-  return THPVariable_Unpack(o);
+  const Tensor &t = THPVariable_Unpack(o);
+  // (its memory holds the values with their signs turned)
+  if (t.is_neg()) refuse("%s: %s is a view that negates (of a conjugate's imaginary part): resolve_neg() it", fn, what);
+  return t;
 }
 
 void on_device_of(const char *fn, const char *what, const Tensor &t, const Tensor &like) {
