@@ -468,3 +468,12 @@ def test_views_that_negate_are_refused():
             call()
     with pytest.raises(ValueError, match="must be a CUDA"):
         ops.rotate(lazy.resolve_neg(), POS, none)
+
+
+@pytest.mark.parametrize("scale", [math.nan, math.inf, -math.inf, 1e300, 3e38])
+def test_attend_refuses_a_scale_that_is_no_number(scale):
+    args = [ATTEND[n] for n in ("q", "k_cache", "v_cache", "page_table", "lengths")]
+    with pytest.raises(ValueError, match="scale must be finite"):
+        ops.attend_shared_prefix(*args, scale=scale)
+    scale = math.copysign(min(abs(scale), 3.4e38), scale)             # in 32 bits
+    refused("tila_attend_shared_prefix", attend_args(scale=scale, workspace=4096, workspace_bytes=1 << 40))

@@ -620,6 +620,8 @@ int check(const tila_attend_args *a, char *log, size_t cap) {
     return fail(TILA_ERR_ARGUMENT, log, cap, "%s: heads must be a multiple of kv_heads", who);
   if (a->dim < 8 || a->dim > 256 || a->dim % 8 != 0)
     return fail(TILA_ERR_ARGUMENT, log, cap, "%s: dim must be a multiple of 8 up to 256", who);
+  if (!std::isfinite(a->scale * 1.4426950408889634f))
+    return fail(TILA_ERR_ARGUMENT, log, cap, "%s: scale must be finite", who);
   if (a->page_size < 1 || a->table_width < 0 || a->max_queries < 1 || a->num_pages < 0 || a->prefix_length < 0)
     return fail(TILA_ERR_ARGUMENT, log, cap, "%s: a size is out of range", who);
   constexpr i64 most = 1ll << 30;

@@ -708,6 +708,10 @@ PyObject *attend_shared_prefix(PyObject *const *o) {
       a.prefix_length > limit)
     refuse("%s: more than 2^30 rows of queries, sequences, or tokens of one sequence or of the prefix", fn);
   a.scale = o[9] == Py_None ? static_cast<float>(1.0 / std::sqrt(static_cast<double>(dim))) : static_cast<float>(number(o[9]));
+  // (base 2 in the kernels; a score times an infinite or missing scale is no number, but the wide form would have
+  // taken the latter for 0)
+  if (!std::isfinite(a.scale * 1.4426950408889634f))
+    refuse("%s: scale must be finite, also times log2(e) in 32 bits, is %g", fn, static_cast<double>(a.scale));
   std::optional<Tensor> given =
       result(fn, "out", o[10], q, {}, {{"q", &q}, {"k_cache", caches[0]}, {"v_cache", caches[1]}});
   unrecorded(fn, {{"q", &q}, {"k_cache", caches[0]}, {"v_cache", caches[1]}});
