@@ -3,6 +3,7 @@
 
 import ctypes
 import math
+import re
 import shutil
 import struct
 import subprocess
@@ -477,3 +478,17 @@ def test_attend_refuses_a_scale_that_is_no_number(scale):
         ops.attend_shared_prefix(*args, scale=scale)
     scale = math.copysign(min(abs(scale), 3.4e38), scale)             # in 32 bits
     refused("tila_attend_shared_prefix", attend_args(scale=scale, workspace=4096, workspace_bytes=1 << 40))
+
+
+def test_wide_attention_kernels_have_the_registers_they_share_out(tmp_path):
+    """Their warpgroups would otherwise wait for registers that do not exist (the
+    library then takes the narrow form): a compiler that gives them others shows here."""
+    from tila_b200 import build
+    source = build.PKG / "csrc" / "ops" / "attend_wide.cu"
+    text = source.read_text()
+    two, one = map(int, re.search(r"kLaunchRegisters = G == 2 \? (\d+) : (\d+);", text).groups())
+    r = subprocess.run([str(build.CUDA / "bin" / "nvcc"), "-std=c++17", "-O2", "-gencode", "arch=compute_100a,code=sm_100a",
+                        "-lineinfo", "-diag-suppress", "550", "-Xptxas", "-v", "-cubin", "-o", str(tmp_path / "x.cubin"),
+                        str(source)], check=True, capture_output=True, text=True)
+    used = re.findall(r"entry function '\S*attend_wide_kernelI\S*Lb([01])E\S*'.*?Used (\d+) registers", r.stdout + r.stderr, re.S)
+    assert sorted(used) == sorted([("0", str(two)), ("1", str(one))] * 4)

@@ -785,8 +785,8 @@ Plan plan(const tila_attend_args &a) {
   // up to 32 rows fill a quarter of a row tile, and two blocks of 16 that read the keys
   // twice, once from L2, are faster (28 rows, 21 sequences of up to 3462 tokens: 32 us, wide
   // 39; 20 rows, 64 of up to 1000: 34 and 48; 64 rows 43 either way).
-  r.prefix_wide = wide && p.prefix > 0 && rows > 16;
-  r.own_wide = wide && own_keys > 0 && own_rows > 32;
+  r.prefix_wide = wide && p.prefix > 0 && rows > 16 && wide_fits(a, false);
+  r.own_wide = wide && own_keys > 0 && own_rows > 32 && wide_fits(a, true);
   r.narrow_rows = (r.own_wide || own_rows <= 8) && (r.prefix_wide || rows <= 8) ? 8 : 16;
   r.prefix_tiles = static_cast<int>((rows + r.narrow_rows - 1) / r.narrow_rows);
   r.own_tiles = static_cast<int>((own_rows + r.narrow_rows - 1) / r.narrow_rows);

@@ -40,6 +40,7 @@
 #include "attend.cuh"
 #include "attend_wide.cuh"
 
+#include <atomic>
 #include <type_traits>
 
 namespace tila_ops {
@@ -61,7 +62,7 @@ template <int DP, int G> struct Wide {
   // add up to at most the total at launch (256 * 216 + 128 * 64 = 63488 of 384 * 168 =
   // 64512; 128 * 200 + 128 * 56 = 256 * 128); the host checks that the compiler gave the
   // kernel exactly those, since a warpgroup would otherwise wait for registers that do
-  // not exist.
+  // not exist, and leaves the rows to the narrow form where it did not.
   static constexpr int kLaunchRegisters = G == 2 ? 168 : 128;
   static constexpr int kSoftmaxRegisters = G == 2 ? 216 : 200, kOtherRegisters = G == 2 ? 64 : 56;
   static_assert(G * 128 * kSoftmaxRegisters + 128 * kOtherRegisters <= kThreads * kLaunchRegisters, "registers");
@@ -649,17 +650,29 @@ int encode(TensorMap *map, const tila_attend_args &a, int rows, u64 address, con
   return tila_encode_tensor_map(map, a.dtype == TILA_F16 ? 6 : 9, 4, address, dims, strides, box, 3, log, cap);
 }
 
+// Whether the kernel was given the registers that its warpgroups share out.  What the
+// compiler did is looked up once; a lookup that fails is made again at the next call.
+template <typename T, int DP, bool kOwn> cudaError_t registers_fit(bool &fit) {
+  static std::atomic<int> registers{0};
+  int n = registers.load(std::memory_order_relaxed);
+  if (n == 0) {
+    cudaFuncAttributes attr;
+    const cudaError_t e = cudaFuncGetAttributes(&attr, attend_wide_kernel<T, DP, kOwn>);
+    if (e != cudaSuccess) return e;
+    registers.store(n = attr.numRegs, std::memory_order_relaxed);
+  }
+  fit = n == Wide<DP, kOwn ? 1 : 2>::kLaunchRegisters;
+  return cudaSuccess;
+}
+
 template <typename T, int DP, bool kOwn>
 cudaError_t launch_form(const AttendParams &p, const TensorMap &k, const TensorMap &v, const WideGrid &grid,
                         unsigned blocks, bool after_previous, cudaStream_t stream) {
   using W = Wide<DP, kOwn ? 1 : 2>;
-  static const cudaError_t registers = [] {
-    cudaFuncAttributes attr;
-    const cudaError_t e = cudaFuncGetAttributes(&attr, attend_wide_kernel<T, DP, kOwn>);
-    return e != cudaSuccess ? e : attr.numRegs == W::kLaunchRegisters ? cudaSuccess : cudaErrorLaunchOutOfResources;
-  }();
-  if (registers != cudaSuccess) return registers;
-  const cudaError_t e = allow_shared_memory<attend_wide_kernel<T, DP, kOwn>>(W::kBytes);
+  bool fit = false;
+  cudaError_t e = registers_fit<T, DP, kOwn>(fit);
+  if (e == cudaSuccess && !fit) e = cudaErrorLaunchOutOfResources;
+  if (e == cudaSuccess) e = allow_shared_memory<attend_wide_kernel<T, DP, kOwn>>(W::kBytes);
   if (e != cudaSuccess) return e;
   return launch_kernel(attend_wide_kernel<T, DP, kOwn>, blocks, W::kThreads, W::kBytes, stream, after_previous, p, k, v,
                        grid);
@@ -680,6 +693,20 @@ bool tma_possible(const tila_attend_args &a) {
 bool wide_possible(const tila_attend_args &a) {
   return tma_possible(a) && a.dim <= 128 && a.page_size % 8 == 0 &&
          (a.page_size < kTile ? kTile % a.page_size == 0 : a.page_size % kTile == 0);
+}
+
+namespace {
+template <typename T> cudaError_t form_fits(const tila_attend_args &a, bool own, bool &fit) {
+  if (a.dim <= 64) return own ? registers_fit<T, 64, true>(fit) : registers_fit<T, 64, false>(fit);
+  return own ? registers_fit<T, 128, true>(fit) : registers_fit<T, 128, false>(fit);
+}
+}  // namespace
+
+bool wide_fits(const tila_attend_args &a, bool own) {
+  bool fit = true;
+  const cudaError_t e = a.dtype == TILA_F16 ? form_fits<__half>(a, own, fit) : form_fits<__nv_bfloat16>(a, own, fit);
+  if (e != cudaSuccess) cudaGetLastError();                 // the launch asks again, and reports it
+  return fit;
 }
 
 int encode_caches(const tila_attend_args &a, int rows, tila::TensorMap *k, tila::TensorMap *v, char *log, size_t cap) {

@@ -13,6 +13,9 @@ struct WideGrid {
 // also fit the wide form: boxes of whole pages, or of 128 rows of one.
 bool tma_possible(const tila_attend_args &a);
 bool wide_possible(const tila_attend_args &a);
+// Whether the compiler gave the wide form's kernel for these sizes the registers it
+// needs (true also where that cannot be looked up).
+bool wide_fits(const tila_attend_args &a, bool own);
 
 // Tensor maps of both caches with boxes of 64 elements of `rows` rows, 128-byte
 // swizzled.
