@@ -828,3 +828,29 @@ print("raised and reset")
     got = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120,
                          cwd=Path(__file__).resolve().parents[1])
     assert got.returncode == 0 and "raised and reset" in got.stdout, got.stderr
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_rotate_sines_near_zero(layout):
+    """Angles close to whole half turns, whose sines are far smaller than the
+    rounding of the angle itself to 32 bits."""
+    g = gen(23)
+    half, tokens = 32, 200
+    positions = torch.arange(1, tokens + 1, device="cuda")
+    # position * inv_freq = a few half turns and up to 1e-5 of one
+    inv = math.pi * (1 + 1e-5 * torch.rand(half, generator=g, device="cuda", dtype=torch.float64)) * torch.arange(
+        1, half + 1, device="cuda")
+    x = torch.zeros(tokens, 1, 2 * half, device="cuda")
+    first = slice(0, half) if layout == "half" else slice(0, None, 2)
+    second = slice(half, None) if layout == "half" else slice(1, None, 2)
+    x[..., first] = 1
+    y = ops.rotate(x, positions, inv, layout=layout).double()[:, 0]
+    angle = positions.double()[:, None] * inv
+    c, s = angle.cos(), angle.sin()
+    # sincospi is off by 2 ulp (4 U); the sum with its correction, the amplitude and the row's product by U each;
+    # the correction itself (at most pi 2^-25 < 1e-7) by 3 U of it (remainder, pi, product); the angle in 64 bits by
+    # 2^-51 of itself (position * inv_freq * 1/2pi, here and in the reference)
+    bound, least = 8 * U, 2 ** -50 * angle + 4 * U * 1e-7
+    assert ((y[:, second] - s).abs() <= bound * s.abs() + least).all()
+    assert ((y[:, first] - c).abs() <= bound * c.abs() + least).all()
+    assert bool((s.abs() < 1e-3).any())

@@ -7,7 +7,9 @@
 // elements behind `rotary` as they are.  The angle is reduced to a part of one
 // turn in 64 bits (positions in the millions keep 1e-10 of a turn there, where
 // 32 bits would lose the angle), and only that part goes through sincospi in 32
-// bits.  All products and sums are 32-bit; a result is rounded once, when it is
+// bits, corrected to first order by what its own rounding to 32 bits left (up to 1e-7
+// of a sine, which could be that small itself; once for each token and pair, not for
+// each head).  All products and sums are 32-bit; a result is rounded once, when it is
 // stored.
 //
 // Bound by memory: a row is read once and written once (with norms, at 16 bits, the
@@ -305,10 +307,12 @@ __device__ __forceinline__ void fill_table(const Params &p, int b, i64 token0, i
     const i64 pos = index_at(p.positions, b * p.position_stride[0] + (token0 + t) * p.position_stride[1], p.index64 & 1);
     double turns = static_cast<double>(pos) * p.inv_freq[j] * 0.15915494309189535;
     turns -= rint(turns);
-    float s, c;
-    sincospif(static_cast<float>(2.0 * turns), &s, &c);
-    c *= p.amplitude;
-    s *= p.amplitude * p.sign;
+    const float angle = static_cast<float>(2.0 * turns);              // of half turns
+    const float left = static_cast<float>(2.0 * turns - static_cast<double>(angle)) * 3.14159265f;
+    float sine, cosine;
+    sincospif(angle, &sine, &cosine);
+    const float c = fmaf(-left, sine, cosine) * p.amplitude;
+    const float s = fmaf(left, cosine, sine) * p.amplitude * p.sign;
     if (p.across) {
       const int low = p.interleaved ? 2 * j : j, high = p.interleaved ? 2 * j + 1 : j + p.half;
       auto at = [&](int e) {
