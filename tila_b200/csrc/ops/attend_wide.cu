@@ -218,8 +218,8 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
   const bool shared_rows = G == 2 && rows - row0 <= kTile;   // one row tile: the warpgroups take tiles in turn
   const int tiles = before + (end > begin ? (end - begin + kTile - 1) / kTile : 0);
   const int ahead = shared_rows ? 2 : 1;             // S is issued so many tiles ahead of P V
-  // tiles from here on hold keys that some rows see and others do not (3 at most: a
-  // block's tokens are 256 or fewer)
+  // tiles from here on hold keys that some rows see and others do not (2 at most: a
+  // block's tokens are 128 or fewer)
   const int least = kOwn ? limit0 + row0 / p.group : end;
   const int mixed = least >= end ? tiles : before + max(0, least - begin) / kTile;
 

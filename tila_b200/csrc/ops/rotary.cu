@@ -835,14 +835,10 @@ int launch_backward(Params p, const tila_rotary_args &a, cudaStream_t stream, ch
   p.tokens_per_block = std::min(32, (p.across ? 1024 : 2048) / std::max(1, p.half));
   const int blocks = backward_blocks(p);
   const int groups = kBackwardThreads / p.lanes;
+  // (at most 44144 bytes whatever the sizes: no more than any kernel may have)
   const size_t smem = sizeof(float) * table_size(p) + sizeof(float) * (2 * p.weight_floats + std::max(p.dim, p.row_floats) * groups) + 16;
-  cudaError_t e = cudaSuccess;
-  if (smem > 48 * 1024)
-    e = cudaFuncSetAttribute(rotary_norm_backward_kernel<T, V, K, kAcross>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(smem));
-  if (e != cudaSuccess) return launch_status(e, "tila_rotary_norm_backward", log, cap);
   rotary_norm_backward_kernel<T, V, K, kAcross><<<blocks, kBackwardThreads, smem, stream>>>(p);
-  e = cudaGetLastError();
+  cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess)
     e = launch_kernel(weight_grad_kernel, (p.dim + 31) / 32 * 2, 1024, 0, stream, true,
                       static_cast<const float *>(p.partial), blocks, p.dim, reinterpret_cast<float *>(a.weight_grad[0]),
