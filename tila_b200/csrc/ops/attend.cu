@@ -270,8 +270,12 @@ __device__ __forceinline__ void narrow_block(const AttendParams &p, const tila::
     const int key0 = begin + step * kStep;
     if constexpr (kTma) {
       if (!__all_sync(0xffffffffu, tila::mbar_wait(&full[warp][step % kStages], (step / kStages) & 1, p.err, __LINE__,
-                                                   nullptr)))
+                                                   nullptr))) {
+        // the copies behind it land before their places are used for the join
+        for (int s = step; s < min(step + kStages, steps); ++s)
+          tila::mbar_wait(&full[warp][s % kStages], (s / kStages) & 1, p.err, __LINE__, nullptr);
         break;
+      }
       if (key0 + kSlice > it.end) {
         // values behind the end: whatever the page holds there, for a weight of 0
         for (int i = lane; i < (key0 + kSlice - it.end) * (DP / 8); i += 32)

@@ -304,6 +304,11 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
       values = next_values;
       keys = next_keys;
     }
+    // (where a wait gave up nobody else waits for the copies in flight: they land before
+    // the block leaves its shared memory)
+    const int issued = ok ? item : item - 1;
+    for (int i = max(0, issued - W::kStages); i < issued; ++i)
+      warp_wait(&bars.full[i % W::kStages], (i / W::kStages) & 1, p.err, __LINE__, nullptr);
   } else if (warp == kMmas) {
     // ---- MMAs -------------------------------------------------------------------
     const u32 base4 = uniform(tila::smem_u32(smem)) >> 4, tm = uniform(tmem);
@@ -395,8 +400,12 @@ __device__ __forceinline__ void wide_block(const AttendParams &p, const TensorMa
       }
       __syncwarp();
     }
-    if (ok && n_tiles > 0 && elected()) tila::mma_commit(&bars.done);
-    __syncwarp();
+    // (also where a wait gave up: products in flight end before tensor memory is given back)
+    if (n_tiles > 0) {
+      if (elected()) tila::mma_commit(&bars.done);
+      __syncwarp();
+      warp_wait(&bars.done, 0, p.err, __LINE__, nullptr);
+    }
   } else if (warp >= kLooks) {
     if constexpr (kOwn) {
       // ---- values of mixed tiles -----------------------------------------------------
