@@ -3,6 +3,8 @@ header declares, and its NVRTC half compiles generated CUDA for sm_100a."""
 
 import ctypes
 import re
+import subprocess
+import sys
 from pathlib import Path
 
 import pytest
@@ -73,3 +75,17 @@ def test_gather_entry_points_validate_arguments():
     assert lib.tila_mg_comm_destroy(None) == -6
     with pytest.raises(ValueError):
         native.mg_comm_init(b"short", 1, 0)
+
+
+def test_without_tila_its_tests_are_skipped_and_the_others_run():
+    try:
+        import tila_b200._reference  # noqa: F401
+    except ImportError:
+        pass
+    else:
+        pytest.skip("Tila is installed")
+    run = subprocess.run([sys.executable, "-m", "pytest", "tests/test_plugin.py", "tests/test_ops.py", "-x", "-q", "-rs",
+                          "-k", "plugin or frequencies", "-p", "no:cacheprovider"],
+                         cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stdout
+    assert "1 skipped" in run.stdout and "Tila is not installed" in run.stdout and " passed" in run.stdout
