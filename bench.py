@@ -30,7 +30,7 @@ with NCCL (timed separately as ``gather_ms``).
 
 ``--impl reference`` times the reference itself - Tila's NumPy interpreter,
 its only CPU execution path - on the same workloads and prints the same line
-with ``"impl": "reference"``.
+with ``"impl": "reference"`` (where Tila is not installed, a line that says so).
 """
 
 from __future__ import annotations
@@ -908,6 +908,11 @@ def main():
 
     if args.impl == "reference":
         if rank != 0:
+            return
+        try:
+            import tila_b200._reference  # noqa: F401
+        except ImportError as e:
+            print(json.dumps({"impl": "reference", "unavailable": str(e)}))
             return
         out = {}
         for key in keys:

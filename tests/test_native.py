@@ -2,6 +2,7 @@
 header declares, and its NVRTC half compiles generated CUDA for sm_100a."""
 
 import ctypes
+import json
 import re
 import subprocess
 import sys
@@ -89,3 +90,16 @@ def test_without_tila_its_tests_are_skipped_and_the_others_run():
                          cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert run.returncode == 0, run.stdout
     assert "1 skipped" in run.stdout and "Tila is not installed" in run.stdout and " passed" in run.stdout
+
+
+def test_reference_arm_without_tila_says_so():
+    try:
+        import tila_b200._reference  # noqa: F401
+    except ImportError as e:
+        why = str(e)
+    else:
+        pytest.skip("Tila is installed")
+    run = subprocess.run([sys.executable, "bench.py", "--impl", "reference", "--steps", "3"], cwd=ROOT, capture_output=True,
+                         text=True, timeout=300)
+    assert run.returncode == 0, run.stderr
+    assert json.loads(run.stdout) == {"impl": "reference", "unavailable": why}
