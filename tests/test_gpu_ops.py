@@ -854,3 +854,16 @@ def test_rotate_sines_near_zero(layout):
     assert ((y[:, second] - s).abs() <= bound * s.abs() + least).all()
     assert ((y[:, first] - c).abs() <= bound * c.abs() + least).all()
     assert bool((s.abs() < 1e-3).any())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("page", [16, 128])
+@pytest.mark.parametrize("dim", [8, 40, 56, 72, 104, 136, 200, 248])
+def test_attend_head_sizes_that_end_inside_a_box(dtype, page, dim):
+    """Boxes of 64 elements that are wider than the rows, or lie behind them wholly: few
+    rows (narrow form), many (wide form up to 128 elements: prefix and own tokens
+    apart, and own blocks that take a short prefix too)."""
+    for counts, lengths, prefix in (([1, 1, 1], [40, 129, 3], 300), ([40, 33, 2], [200, 33, 70], 300),
+                                    ([70] * 20, [75] * 20, 13)):
+        case = paged(dim + prefix, counts, lengths, prefix, 8, 2, dim, page, dtype)
+        check_attend(case, counts, lengths, prefix)
