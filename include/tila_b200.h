@@ -206,7 +206,9 @@ int tila_mg_comm_destroy(void *comm);
  * and runs on the current device; nothing is allocated and nothing is kept
  * after the call.  `err` is the address of an error block
  * (TILA_ERROR_BLOCK_BYTES, 0 = none) that takes device errors: an index outside
- * its pool (the access is left out) or a wait that gave up. */
+ * its pool (the row of a slot is left out, a page reads as zeros, a length or an
+ * offset is cut to the table or to q) or a wait that gave up.  Addresses are
+ * multiples of their elements' size; others are refused. */
 
 /* Element types. */
 enum { TILA_F32 = 0, TILA_F16 = 1, TILA_BF16 = 2 };

@@ -660,6 +660,10 @@ struct Plan {
 
 // Chunks of the wide form, one block a multiprocessor.  A block takes about 2.1 us
 // for a tile of 128 keys and 9.5 us beside that (queries, filling the ring, results).
+// That is the tile at 128 elements and the price at any size: at 64, where a tile takes
+// 1.4, that price would split most calls alike and some better (16 of 128 new tokens on
+// 4096, 16 heads 94.1 us with either; 64 on 8192, 8 key heads 46.7 us with 2.1, 45.2 with
+// 1.4).
 // Where the narrow form follows (`narrow_bytes`, half of what the longest sequences
 // would be), it starts beside the wide form on the multiprocessors that are left,
 // which fetch about 58 GB/s each, 6.7 TB/s in all, and takes 8 us beside that: the

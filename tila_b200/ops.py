@@ -19,9 +19,11 @@ gradients enabled a tensor that requires one is refused (``torch.no_grad()``, or
 ``torch.autograd.Function`` around the call and its gradient's).  Every call
 can be captured into a CUDA graph once an operator has run on the device.
 Wrong arguments raise ``ValueError`` before anything is launched.  What only the
-device can see (a slot outside the cache) leaves the access out, is recorded as
-a device error, and is raised by the next operator on that device or by
-:func:`check_errors`.
+device can see is kept from any access outside the caches, recorded as a device
+error, and raised by the next operator on that device or by :func:`check_errors`:
+a row whose slot is outside the cache is left out; a page outside it reads as zeros
+(its keys score 0 and take their weight in the softmax); lengths and offsets are cut
+to the table and to ``q``.
 """
 
 from __future__ import annotations
@@ -45,7 +47,8 @@ except ImportError as exc:
 ERROR_CODES = {
     1: "a bounded wait timed out; the operator stopped early and its outputs are incomplete",
     2: "tensor memory allocation failed",
-    5: "an index outside its pool (a cache slot, a page, a length or an offset) was left out",
+    5: "an index outside its pool: a cache slot (its row was left out), a page (read as zeros), a length or an offset "
+       "(cut to the table or to q)",
 }
 
 
