@@ -867,3 +867,41 @@ def test_attend_head_sizes_that_end_inside_a_box(dtype, page, dim):
                                     ([70] * 20, [75] * 20, 13)):
         case = paged(dim + prefix, counts, lengths, prefix, 8, 2, dim, page, dtype)
         check_attend(case, counts, lengths, prefix)
+
+
+@pytest.mark.parametrize("what", ["norm", "append", "attend narrow", "attend wide", "attend chunks"])
+def test_first_call_of_an_operator_in_a_capture(what):
+    """In a process where only another operator has run on the device: its kernels
+    are loaded, and given their shared memory, while the graph is captured."""
+    code = """
+import sys, torch
+sys.path.insert(0, "tests")
+from test_gpu_ops import *
+what = sys.argv[1]
+x, w, inv, positions = normal(gen(1), 40, 4, 64, dtype=BF16), torch.ones(64, device="cuda"), freqs(64), torch.arange(40, device="cuda")
+ops.rotate(x, positions, inv)
+if what.startswith("attend"):
+    counts = [40, 3] if "chunks" in what else [1] * (2 if "narrow" in what else 20)
+    q, kc, vc, table, lens, pages, offsets = paged(1, counts, [60] * len(counts), 300, 8, 2, 64, 16, BF16)
+    f = lambda: [ops.attend_shared_prefix(q, kc, vc, table, lens, prefix_pages=pages, prefix_length=300,
+                                          query_offsets=offsets, max_queries=max(counts))]
+elif what == "norm":
+    f = lambda: [*ops.norm_rotate(x, x, w, w, positions, inv), *ops.norm_rotate_backward(x, x, x, x, w, w, positions, inv)]
+else:
+    caches = torch.zeros(2, 3, 16, 4, 64, dtype=BF16, device="cuda")
+    f = lambda: [ops.append_paged(x, x, *caches, positions, positions=positions, inv_freq=inv, q=x), caches]
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = f()
+for t in got:
+    t.zero_()
+graph.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in got]
+assert all(torch.equal(a, b) for a, b in zip(got, f())) and bool(got[0].any())
+ops.check_errors()
+print("captured")
+"""
+    got = subprocess.run([sys.executable, "-c", code, what], capture_output=True, text=True, timeout=120,
+                         cwd=Path(__file__).resolve().parents[1])
+    assert got.returncode == 0 and "captured" in got.stdout, got.stderr

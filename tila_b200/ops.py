@@ -250,7 +250,9 @@ def attend_shared_prefix(q, k_cache, v_cache, page_table, lengths, *, prefix_pag
     Without ``query_offsets`` row b of ``q`` is the one new token of sequence b.  With
     it (int32, batch + 1 entries) rows ``query_offsets[b]`` to ``query_offsets[b + 1]`` are
     its new tokens, at most ``max_queries`` of them; each sees the tokens up to
-    itself.  Rows of ``q`` behind the last sequence may be anything, and theirs of
+    itself.  By default ``max_queries`` is the number of rows of ``q``: right, but every
+    sequence is given blocks for so many (64 sequences of 128 of them 1219 us instead
+    of 303), so pass it where the host knows it.  Rows of ``q`` behind the last sequence may be anything, and theirs of
     ``out`` are left as they were.  A token that sees nothing, or whose scores are all
     minus infinity, gets zeros (and -inf for its log).
 
